@@ -28,40 +28,40 @@ def _size(case):
 def listed():
     return [
         # one token of a BERT-large encoder: what its latency costs
-        dict(name="norm forward, one token", op="norm_forward", type="fp16", rows=1, width=1024,
+        dict(name="norm forward one token", op="norm_forward", type="fp16", rows=1, width=1024,
              skip=True, bias=True, keep_sum=False),
         # a batch of 16 sequences of 512 tokens, post-norm, the previous product's bias folded in
-        dict(name="norm forward, 8192 tokens post-norm", op="norm_forward", type="fp16", rows=8192, width=1024,
+        dict(name="norm forward 8192 tokens post-norm", op="norm_forward", type="fp16", rows=8192, width=1024,
              skip=True, bias=True, keep_sum=False),
         # the residual stream of a wide pre-norm layer: the sum goes on beside the normalised rows
-        dict(name="norm forward, wide pre-norm", op="norm_forward", type="bf16", rows=8192, width=4096,
+        dict(name="norm forward wide pre-norm", op="norm_forward", type="bf16", rows=8192, width=4096,
              skip=True, bias=False, keep_sum=True),
         # a ragged batch at BERT-base's width, master precision
-        dict(name="norm backward, 509 tokens", op="norm_backward", type="fp32", rows=509, width=768,
+        dict(name="norm backward 509 tokens", op="norm_backward", type="fp32", rows=509, width=768,
              skip=False, bias=False, keep_sum=False),
         # a training step's post-norm at BERT-large's width
-        dict(name="norm backward, 8192 tokens post-norm", op="norm_backward", type="bf16", rows=8192, width=1024,
+        dict(name="norm backward 8192 tokens post-norm", op="norm_backward", type="bf16", rows=8192, width=1024,
              skip=True, bias=True, keep_sum=False),
         # the gradient that comes down the residual stream joins in; rows that do not cut into vectors
-        dict(name="norm backward, odd width pre-norm", op="norm_backward", type="fp16", rows=4099, width=1531,
+        dict(name="norm backward odd width pre-norm", op="norm_backward", type="fp16", rows=4099, width=1531,
              skip=False, bias=False, keep_sum=True),
         # one token through the first product of a feed-forward block: a pass over the weights
-        dict(name="linear, one token", op="linear", type="fp16", tokens=1, width=1024, out=4096,
+        dict(name="linear one token", op="linear", type="fp16", tokens=1, width=1024, out=4096,
              act="gelu", bias=True, residual=False, keep_z=False),
         # a short batch through the second product, the residual added on the way out
-        dict(name="linear, 384 tokens with residual", op="linear", type="fp16", tokens=384, width=4096, out=1024,
+        dict(name="linear 384 tokens with residual", op="linear", type="fp16", tokens=384, width=4096, out=1024,
              act="none", bias=True, residual=True, keep_z=False),
         # training: the first product of a feed-forward block, pre-activation kept
-        dict(name="linear, 8192 tokens training", op="linear", type="bf16", tokens=8192, width=1024, out=4096,
+        dict(name="linear 8192 tokens training", op="linear", type="bf16", tokens=8192, width=1024, out=4096,
              act="gelu", bias=True, residual=False, keep_z=True),
         # a head of odd sizes in master precision
-        dict(name="linear, odd sizes fp32", op="linear", type="fp32", tokens=1003, width=1001, out=517,
+        dict(name="linear odd sizes fp32", op="linear", type="fp32", tokens=1003, width=1001, out=517,
              act="relu", bias=True, residual=True, keep_z=False),
         # the gradient of a projection at BERT-base's width, a ragged batch
-        dict(name="linear backward, 771 tokens", op="linear_backward", type="fp16", tokens=771, width=768, out=1011,
+        dict(name="linear backward 771 tokens", op="linear_backward", type="fp16", tokens=771, width=768, out=1011,
              act="none", bias=True),
         # the gradient of the training case above
-        dict(name="linear backward, 8192 tokens", op="linear_backward", type="bf16", tokens=8192, width=1024, out=4096,
+        dict(name="linear backward 8192 tokens", op="linear_backward", type="bf16", tokens=8192, width=1024, out=4096,
              act="gelu", bias=True),
     ]
 
