@@ -1,0 +1,762 @@
+// LayerNorm for training on gfx950: the forward pass that keeps its statistics (and, for pre-norm layers, the
+// sum it normalises) and the backward pass with the column sums of gamma's, beta's and the bias's gradients.
+//
+//   h = x (+ skip) (+ bias),  mean and rstd = 1 / sqrt(var + eps) over a row,  xhat = (h - mean) * rstd
+//   y = gamma * xhat + beta
+//   dh = rstd * (g - mean(g) - xhat * mean(g * xhat)) with g = dy * gamma,  dx = dh (+ dsum)
+//   dgamma = sum over rows of dy * xhat, dbeta = sum of dy, dbias = sum of dh
+//
+// Everything between the loads and the one rounding at the store is fp32.  LPR lanes own a row (a part of a
+// wavefront, a wavefront, or several), 16 bytes per lane and step, NV steps, the row in registers: it is read
+// once, and the next row's loads are in flight while this one is reduced.  Rows that do not divide into 16-byte
+// slices (odd lengths, any element alignment) use the same loads unaligned: the lane that holds the row's end
+// reads the row's LAST slice instead and leaves out the elements its neighbour has.
+//
+// The column sums stay in registers over all rows a workgroup processes, are combined through LDS in a fixed
+// order and leave as one row of partials per workgroup; a second small launch adds those, also in a fixed order:
+// no atomics, results repeat bit for bit.  Rows longer than a workgroup's registers are streamed from cache
+// (ln_*_stream_kernel), their column sums by a kernel that walks rows down each column.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <type_traits>
+
+#include "../common.h"
+#include "device_util.h"
+
+// No implicit multiply-add fusion: every variant of a kernel (with a bias, from a stored sum, any lane layout) rounds
+// the same operations the same way, so every fused operation is written as an explicit fma.
+#pragma clang fp contract(off)
+
+namespace fwdmi {
+namespace {
+
+struct LnTrain {
+  const void* x;
+  const void* skip;  // nullable
+  const void* dsum;  // backward, nullable: gradient that arrives at the sum from elsewhere
+  const void* dy;    // backward
+  const float* gamma;
+  const float* beta;  // forward
+  const float* bias;  // nullable
+  void* out;          // forward: y; backward: dx
+  void* sum;          // forward, nullable: h rounded to T
+  float* mean;        // forward: written; backward: read
+  float* rstd;
+  float* part_gamma;  // backward: row p of partials starts at part_* + p * part_stride
+  float* part_beta;
+  float* part_bias;
+  float* c1;          // streamed backward: mean(g * xhat) and mean(g) per row
+  float* c2;
+  int64_t part_stride;
+  int64_t rows;
+  int32_t ld;
+  float eps;
+};
+
+// VEC elements at any element alignment (one global_load_dwordx4 where the slice is 16 bytes).
+template <typename T, int N>
+__device__ __forceinline__ Pack<T, N> load_slice(const T FWDMI_GLOBAL* p) {
+  Pack<T, N> r;
+  if constexpr (N == 1) {
+    r.v[0] = *p;
+  } else {
+    typedef T V __attribute__((ext_vector_type(N), aligned(sizeof(T))));
+    const V x = *(const V FWDMI_GLOBAL*)p;
+    __builtin_memcpy(&r, &x, sizeof(r));
+  }
+  return r;
+}
+template <typename T, int N>
+__device__ __forceinline__ void store_slice(T FWDMI_GLOBAL* p, const Pack<T, N>& r) {
+  if constexpr (N == 1) {
+    *p = r.v[0];
+  } else {
+    typedef T V __attribute__((ext_vector_type(N), aligned(sizeof(T))));
+    V x;
+    __builtin_memcpy(&x, &r, sizeof(r));
+    *(V FWDMI_GLOBAL*)p = x;
+  }
+}
+
+template <int CTRL>
+__device__ __forceinline__ float dpp_add(float x) {
+  return x + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xf, 0xf, true));
+}
+
+// Sum over aligned groups of G lanes (G = 8 .. 64), the same value in every lane of the group.
+template <int G>
+__device__ __forceinline__ float group_sum(float x) {
+  x = dpp_add<0xB1>(x);              // lane ^ 1
+  x = dpp_add<0x4E>(x);              // lane ^ 2
+  x = dpp_add<0x141>(x);             // the other quad of each 8
+  if (G >= 16) x = dpp_add<0x140>(x);  // the other half of each row of 16
+  if (G >= 32) x += __shfl_xor(x, 16);
+  if (G >= 64) x += __shfl_xor(x, 32);
+  return x;
+}
+
+// Sum over the LPR lanes of a row; `scratch` holds WG / 64 floats per use and phase of the caller's loop.
+template <int WG, int LPR>
+__device__ __forceinline__ float row_sum(float x, float* scratch) {
+  if constexpr (LPR <= 64) {
+    return group_sum<LPR>(x);
+  } else {
+    constexpr int kWaves = LPR / 64;
+    const int wave = threadIdx.x >> 6;
+    x = group_sum<64>(x);
+    if ((threadIdx.x & 63) == 0) scratch[wave] = x;
+    __syncthreads();
+    const int first = wave / kWaves * kWaves;
+    float s = scratch[first];
+#pragma unroll
+    for (int k = 1; k < kWaves; ++k) s += scratch[first + k];
+    return s;
+  }
+}
+
+// Where a lane's slices lie: columns col[j] .. col[j] + VEC, of which the first drop[j] belong to another lane
+// (the row's end) or to nobody (drop == VEC).  FULL: ld == LPR * VEC * NV, every element is the lane's own.
+template <int VEC, int NV, int LPR, bool FULL>
+struct Columns {
+  int col[NV];
+  int drop[NV];
+  __device__ __forceinline__ Columns(int lane_in_row, int ld) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int c = (j * LPR + lane_in_row) * VEC;
+      if (FULL || c + VEC <= ld) {
+        col[j] = c;
+        drop[j] = 0;
+      } else if (c < ld) {
+        col[j] = ld - VEC;
+        drop[j] = VEC - (ld - c);
+      } else {
+        col[j] = 0;
+        drop[j] = VEC;
+      }
+    }
+  }
+  __device__ __forceinline__ bool own(int j, int e) const { return FULL || e >= drop[j]; }
+  // Stores the lane's own elements of slice j (the row's end one by one, at most one lane of the row).
+  template <typename T>
+  __device__ __forceinline__ void store(T FWDMI_GLOBAL* row, int j, const Pack<T, VEC>& o) const {
+    if (FULL || drop[j] == 0) {
+      store_slice<T, VEC>(row + col[j], o);
+    } else if (VEC > 1 && drop[j] < VEC) {
+#pragma unroll
+      for (int e = 1; e < VEC; ++e)
+        if (e >= drop[j]) row[col[j] + e] = o.v[e];
+    }
+  }
+};
+
+template <typename T, int VEC, int NV, int WG, int LPR, bool FULL>
+__global__ __launch_bounds__(WG) void ln_forward_kernel(const LnTrain L) {
+  constexpr int kRows = WG / LPR;
+  __shared__ float s_red[4 * (WG / 64)];
+  const int gl = threadIdx.x % LPR;
+  const int group = threadIdx.x / LPR;
+  const Columns<VEC, NV, LPR, FULL> C(gl, L.ld);
+  const T FWDMI_GLOBAL* const px = gconst<T>(L.x);
+  const T FWDMI_GLOBAL* const ps = gconst<T>(L.skip);
+  const bool has_skip = L.skip != nullptr;
+
+  Pack<T, VEC> x[NV], s[NV];
+  auto fetch = [&](int64_t r) {
+    const int64_t base = min(r, L.rows - 1) * L.ld;  // groups past the last row repeat it and store nothing
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      x[j] = load_slice<T, VEC>(px + base + C.col[j]);
+      if (has_skip) s[j] = load_slice<T, VEC>(ps + base + C.col[j]);
+    }
+  };
+
+  const int64_t step = (int64_t)gridDim.x * kRows;
+  const int64_t first = (int64_t)blockIdx.x * kRows;
+  fetch(first + group);
+  float g[NV][VEC], be[NV][VEC], bi[NV][VEC];
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const Pack<float, VEC> pg = load_slice<float, VEC>(gconst<float>(L.gamma) + C.col[j]);
+    const Pack<float, VEC> pb = load_slice<float, VEC>(gconst<float>(L.beta) + C.col[j]);
+    Pack<float, VEC> pi{};
+    if (L.bias) pi = load_slice<float, VEC>(gconst<float>(L.bias) + C.col[j]);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      g[j][e] = pg.v[e];
+      be[j][e] = pb.v[e];
+      bi[j][e] = pi.v[e];
+    }
+  }
+  const float inv_n = 1.0f / (float)L.ld;
+  int phase = 0;
+  for (int64_t r0 = first; r0 < L.rows; r0 += step, phase ^= 1) {  // the same count for every wave of the workgroup
+    const int64_t r = r0 + group;
+    const bool row_ok = r < L.rows;
+    float h[NV][VEC], sum = 0.0f;
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        float v = (float)x[j].v[e];
+        if (has_skip) v += (float)s[j].v[e];
+        v += bi[j][e];
+        h[j][e] = v;
+        sum += C.own(j, e) ? v : 0.0f;
+      }
+    if (r0 + step < L.rows) fetch(r + step);
+    const float mu = row_sum<WG, LPR>(sum, s_red + phase * 2 * (WG / 64)) * inv_n;
+    float m2 = 0.0f;
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const float d = C.own(j, e) ? h[j][e] - mu : 0.0f;
+        m2 = __builtin_fmaf(d, d, m2);
+      }
+    m2 = row_sum<WG, LPR>(m2, s_red + (phase * 2 + 1) * (WG / 64));
+    const float rs = __builtin_amdgcn_rsqf(__builtin_fmaf(m2, inv_n, L.eps));  // 1 ulp
+    if (row_ok) {
+      if (gl == 0) {
+        gmut<float>(L.mean)[r] = mu;
+        gmut<float>(L.rstd)[r] = rs;
+      }
+      T FWDMI_GLOBAL* const py = gmut<T>(L.out) + r * L.ld;
+      T FWDMI_GLOBAL* const ph = gmut<T>(L.sum) + r * L.ld;
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        Pack<T, VEC> o;
+        if (L.sum) {
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) o.v[e] = (T)h[j][e];
+          C.store(ph, j, o);
+        }
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) o.v[e] = (T)__builtin_fmaf(g[j][e], (h[j][e] - mu) * rs, be[j][e]);
+        C.store(py, j, o);
+      }
+    }
+  }
+}
+
+template <typename T, int VEC, int NV, int WG, int LPR, bool FULL, bool BIAS>
+__global__ __launch_bounds__(WG) void ln_backward_kernel(const LnTrain L) {
+  constexpr int kRows = WG / LPR;
+  constexpr int kSlots = LPR * NV * VEC;  // elements of a row, as the lanes hold them
+  __shared__ float s_red[4 * (WG / 64)];
+  __shared__ float s_col[LPR < WG ? kRows * kSlots : 1];
+  const int gl = threadIdx.x % LPR;
+  const int group = threadIdx.x / LPR;
+  const Columns<VEC, NV, LPR, FULL> C(gl, L.ld);
+  const T FWDMI_GLOBAL* const pdy = gconst<T>(L.dy);
+  const T FWDMI_GLOBAL* const px = gconst<T>(L.x);
+  const T FWDMI_GLOBAL* const ps = gconst<T>(L.skip);
+  const T FWDMI_GLOBAL* const pd = gconst<T>(L.dsum);
+  const bool has_skip = L.skip != nullptr, has_dsum = L.dsum != nullptr;
+
+  Pack<T, VEC> dy[NV], x[NV], s[NV], d[NV];
+  float mu, rs;
+  auto fetch = [&](int64_t r) {
+    r = min(r, L.rows - 1);
+    const int64_t base = r * L.ld;
+    mu = gconst<float>(L.mean)[r];
+    rs = gconst<float>(L.rstd)[r];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      dy[j] = load_slice<T, VEC>(pdy + base + C.col[j]);
+      x[j] = load_slice<T, VEC>(px + base + C.col[j]);
+      if (has_skip) s[j] = load_slice<T, VEC>(ps + base + C.col[j]);
+      if (has_dsum) d[j] = load_slice<T, VEC>(pd + base + C.col[j]);
+    }
+  };
+
+  const int64_t step = (int64_t)gridDim.x * kRows;
+  const int64_t first = (int64_t)blockIdx.x * kRows;
+  fetch(first + group);
+  float g[NV][VEC], bi[NV][VEC], sum_g[NV][VEC], sum_b[NV][VEC], sum_h[NV][VEC];
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const Pack<float, VEC> pg = load_slice<float, VEC>(gconst<float>(L.gamma) + C.col[j]);
+    Pack<float, VEC> pi{};
+    if (BIAS) pi = load_slice<float, VEC>(gconst<float>(L.bias) + C.col[j]);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      g[j][e] = pg.v[e];
+      bi[j][e] = pi.v[e];
+      sum_g[j][e] = sum_b[j][e] = sum_h[j][e] = 0.0f;
+    }
+  }
+  const float inv_n = 1.0f / (float)L.ld;
+  int phase = 0;
+  for (int64_t r0 = first; r0 < L.rows; r0 += step, phase ^= 1) {
+    const int64_t r = r0 + group;
+    const bool row_ok = r < L.rows;
+    const float rstd = rs;
+    float xh[NV][VEC], gy[NV][VEC], add[NV][VEC], a1 = 0.0f, a2 = 0.0f;
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        float h = (float)x[j].v[e];
+        if (has_skip) h += (float)s[j].v[e];
+        if (BIAS) h += bi[j][e];
+        const bool live = row_ok && C.own(j, e);
+        const float w = live ? (float)dy[j].v[e] : 0.0f;
+        xh[j][e] = (h - mu) * rstd;
+        gy[j][e] = w * g[j][e];
+        const float xl = live ? xh[j][e] : 0.0f;  // (a column or row of another lane may hold anything)
+        a1 = __builtin_fmaf(gy[j][e], xl, a1);
+        a2 += gy[j][e];
+        sum_g[j][e] = __builtin_fmaf(w, xl, sum_g[j][e]);
+        sum_b[j][e] += w;
+        add[j][e] = has_dsum ? (float)d[j].v[e] : 0.0f;
+      }
+    if (r0 + step < L.rows) fetch(r + step);
+    float* const red = s_red + phase * 2 * (WG / 64);
+    if constexpr (LPR <= 64) {
+      a1 = group_sum<LPR>(a1);
+      a2 = group_sum<LPR>(a2);
+    } else {  // both sums behind one barrier
+      constexpr int kWaves = LPR / 64;
+      const int wave = threadIdx.x >> 6;
+      a1 = group_sum<64>(a1);
+      a2 = group_sum<64>(a2);
+      if ((threadIdx.x & 63) == 0) {
+        red[wave * 2] = a1;
+        red[wave * 2 + 1] = a2;
+      }
+      __syncthreads();
+      const int w0 = wave / kWaves * kWaves;
+      a1 = red[w0 * 2];
+      a2 = red[w0 * 2 + 1];
+#pragma unroll
+      for (int k = 1; k < kWaves; ++k) {
+        a1 += red[(w0 + k) * 2];
+        a2 += red[(w0 + k) * 2 + 1];
+      }
+    }
+    const float c1 = a1 * inv_n, c2 = a2 * inv_n;
+    T FWDMI_GLOBAL* const po = gmut<T>(L.out) + r * L.ld;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      Pack<T, VEC> o;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const float dh = rstd * __builtin_fmaf(-xh[j][e], c1, gy[j][e] - c2);
+        if (BIAS) sum_h[j][e] += row_ok && C.own(j, e) ? dh : 0.0f;
+        o.v[e] = (T)(dh + add[j][e]);
+      }
+      if (row_ok) C.store(po, j, o);
+    }
+  }
+
+  // One row of partials per workgroup: the groups' sums in group order.
+  auto leave = [&](float (&v)[NV][VEC], float* part) {
+    if constexpr (LPR < WG) {
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) s_col[group * kSlots + (j * LPR + gl) * VEC + e] = v[j][e];
+      __syncthreads();
+      for (int i = threadIdx.x; i < kSlots; i += WG) {
+        float t = s_col[i];
+#pragma unroll
+        for (int k = 1; k < kRows; ++k) t += s_col[k * kSlots + i];
+        // the slice's first column, and the row's last slice where it would pass the row's end
+        const int c0 = i / VEC * VEC, e = i % VEC;
+        if (FULL || c0 + VEC <= L.ld)
+          part[i] = t;
+        else if (c0 < L.ld && e >= VEC - (L.ld - c0))
+          part[L.ld - VEC + e] = t;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e)
+          if (C.own(j, e)) part[C.col[j] + e] = v[j][e];
+    }
+  };
+  const int64_t p = blockIdx.x * L.part_stride;
+  leave(sum_g, L.part_gamma + p);
+  leave(sum_b, L.part_beta + p);
+  if (BIAS) leave(sum_h, L.part_bias + p);
+}
+
+// ---- rows longer than a workgroup's registers ---------------------------------------------------------------
+
+constexpr int kStreamWG = 512;
+
+template <int WG>
+__device__ __forceinline__ float wg_sum(float x, float* scratch) {
+  __syncthreads();  // the scratch of the sum before this one has been read
+  return row_sum<WG, WG>(x, scratch);
+}
+
+template <typename T>
+__device__ __forceinline__ float ln_input(const LnTrain& L, int64_t base, int c) {
+  float v = (float)gconst<T>(L.x)[base + c];
+  if (L.skip) v += (float)gconst<T>(L.skip)[base + c];
+  if (L.bias) v += L.bias[c];
+  return v;
+}
+
+template <typename T>
+__global__ __launch_bounds__(kStreamWG) void ln_forward_stream_kernel(const LnTrain L) {
+  __shared__ float s_red[kStreamWG / 64];
+  const float inv_n = 1.0f / (float)L.ld;
+  for (int64_t r = blockIdx.x; r < L.rows; r += gridDim.x) {
+    const int64_t base = r * L.ld;
+    float a = 0.0f;
+    for (int c = threadIdx.x; c < L.ld; c += kStreamWG) a += ln_input<T>(L, base, c);
+    const float mu = wg_sum<kStreamWG>(a, s_red) * inv_n;
+    a = 0.0f;
+    for (int c = threadIdx.x; c < L.ld; c += kStreamWG) {
+      const float d = ln_input<T>(L, base, c) - mu;
+      a = __builtin_fmaf(d, d, a);
+    }
+    const float rs = __builtin_amdgcn_rsqf(__builtin_fmaf(wg_sum<kStreamWG>(a, s_red), inv_n, L.eps));
+    if (threadIdx.x == 0) {
+      L.mean[r] = mu;
+      L.rstd[r] = rs;
+    }
+    for (int c = threadIdx.x; c < L.ld; c += kStreamWG) {
+      const float h = ln_input<T>(L, base, c);
+      if (L.sum) gmut<T>(L.sum)[base + c] = (T)h;
+      gmut<T>(L.out)[base + c] = (T)__builtin_fmaf(L.gamma[c], (h - mu) * rs, L.beta[c]);
+    }
+  }
+}
+
+template <typename T>
+__global__ __launch_bounds__(kStreamWG) void ln_backward_stream_kernel(const LnTrain L) {
+  __shared__ float s_red[kStreamWG / 64];
+  const float inv_n = 1.0f / (float)L.ld;
+  for (int64_t r = blockIdx.x; r < L.rows; r += gridDim.x) {
+    const int64_t base = r * L.ld;
+    const float mu = L.mean[r], rs = L.rstd[r];
+    float a1 = 0.0f, a2 = 0.0f;
+    for (int c = threadIdx.x; c < L.ld; c += kStreamWG) {
+      const float gy = (float)gconst<T>(L.dy)[base + c] * L.gamma[c];
+      a1 = __builtin_fmaf(gy, (ln_input<T>(L, base, c) - mu) * rs, a1);
+      a2 += gy;
+    }
+    const float c1 = wg_sum<kStreamWG>(a1, s_red) * inv_n;
+    const float c2 = wg_sum<kStreamWG>(a2, s_red) * inv_n;
+    if (threadIdx.x == 0) {
+      L.c1[r] = c1;
+      L.c2[r] = c2;
+    }
+    for (int c = threadIdx.x; c < L.ld; c += kStreamWG) {
+      const float xh = (ln_input<T>(L, base, c) - mu) * rs;
+      float dh = rs * __builtin_fmaf(-xh, c1, (float)gconst<T>(L.dy)[base + c] * L.gamma[c] - c2);
+      if (L.dsum) dh += (float)gconst<T>(L.dsum)[base + c];
+      gmut<T>(L.out)[base + c] = (T)dh;
+    }
+  }
+}
+
+// Column sums of streamed rows: a lane per column, blockIdx.y takes every gridDim.y-th row.
+template <typename T>
+__global__ __launch_bounds__(256) void ln_backward_columns_kernel(const LnTrain L) {
+  const int64_t c64 = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (c64 >= L.ld) return;
+  const int c = (int)c64;
+  float sg = 0.0f, sb = 0.0f, sh = 0.0f;
+  for (int64_t r = blockIdx.y; r < L.rows; r += gridDim.y) {
+    const int64_t base = r * L.ld;
+    const float rs = L.rstd[r];
+    const float w = (float)gconst<T>(L.dy)[base + c];
+    const float xh = (ln_input<T>(L, base, c) - L.mean[r]) * rs;
+    sg = __builtin_fmaf(w, xh, sg);
+    sb += w;
+    if (L.part_bias) sh += rs * __builtin_fmaf(-xh, L.c1[r], w * L.gamma[c] - L.c2[r]);
+  }
+  const int64_t p = blockIdx.y * L.part_stride;
+  L.part_gamma[p + c] = sg;
+  L.part_beta[p + c] = sb;
+  if (L.part_bias) L.part_bias[p + c] = sh;
+}
+
+// Adds `parts` rows of partials: 64 columns per workgroup, its sixteen waves each take every sixteenth row.
+// parts == 0 (no rows) leaves zeros.
+struct ColumnSums {
+  const float* part;  // [parts][kinds * ld]
+  float* out[3];
+  int32_t parts, ld, kinds;
+};
+constexpr int kSumWaves = 16;
+__global__ __launch_bounds__(64 * kSumWaves) void column_sums_kernel(const ColumnSums S) {
+  __shared__ float s_red[kSumWaves][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t width = (int64_t)S.kinds * S.ld;
+  const int64_t c = (int64_t)blockIdx.x * 64 + lane;
+  float a = 0.0f;
+  if (c < width)
+    for (int p = wave; p < S.parts; p += kSumWaves) a += S.part[p * width + c];
+  s_red[wave][lane] = a;
+  __syncthreads();
+  if (wave == 0 && c < width) {
+    for (int k = 1; k < kSumWaves; ++k) a += s_red[k][lane];
+    const int kind = (int)(c / S.ld);
+    float* const out = kind == 0 ? S.out[0] : kind == 1 ? S.out[1] : S.out[2];
+    out[c - (int64_t)kind * S.ld] = a;
+  }
+}
+
+// ---- launch ---------------------------------------------------------------------------------------------------
+
+int device_cus() {
+  int dev = 0, v = 0;
+  if (hipGetDevice(&dev) == hipSuccess &&
+      hipDeviceGetAttribute(&v, hipDeviceAttributeMultiprocessorCount, dev) == hipSuccess && v > 0)
+    return v;
+  (void)hipGetLastError();
+  return 256;
+}
+
+constexpr int kMaxParts = 256;       // rows of partials a backward launch leaves (its workgroups)
+constexpr int kStreamParts = 64;     // the same for streamed rows
+constexpr int kBackwardWG = 512;
+
+// Lanes per row and steps per lane of a row of `ld` elements in slices of VEC; steps == 0: streamed.
+struct Shape {
+  int lpr, nv;
+};
+Shape row_shape(int ld, int vec) {
+  const int64_t slices = ((int64_t)ld + vec - 1) / vec;
+  if (slices <= 8) return {8, 1};
+  if (slices <= 16) return {16, 1};
+  if (slices <= 32) return {32, 1};
+  const int deep = 16 / vec;  // steps that keep 16 elements per lane
+  for (int nv = 1; nv <= deep; nv *= 2)
+    if (slices <= 64 * nv) return {64, nv};
+  for (int nv = 1; nv <= deep; nv *= 2)
+    if (slices <= 256 * nv) return {256, nv};
+  for (int nv = deep; nv <= 2 * deep; nv *= 2)
+    if (slices <= 512 * nv) return {512, nv};
+  return {0, 0};
+}
+
+template <typename T, int VEC, int NV, int LPR>
+int launch_forward(const LnTrain& L, hipStream_t stream) {
+  constexpr int kWG = LPR <= 256 ? 256 : 512;
+  constexpr int kRows = kWG / LPR;
+  const int64_t want = (L.rows + kRows - 1) / kRows;
+  const unsigned grid = (unsigned)std::min<int64_t>(want, (int64_t)device_cus() * (kWG == 256 ? 4 : 2));
+  if (L.ld == LPR * VEC * NV)
+    hipLaunchKernelGGL((ln_forward_kernel<T, VEC, NV, kWG, LPR, true>), dim3(grid), dim3(kWG), 0, stream, L);
+  else
+    hipLaunchKernelGGL((ln_forward_kernel<T, VEC, NV, kWG, LPR, false>), dim3(grid), dim3(kWG), 0, stream, L);
+  FWDMI_HIP_CHECK(hipGetLastError());
+  return FWDMI_OK;
+}
+
+template <typename T, int VEC, int NV, int LPR>
+int launch_backward(const LnTrain& L, unsigned grid, hipStream_t stream) {
+#define FWDMI_LN_LAUNCH(FULL_, BIAS_)                                                                          \
+  hipLaunchKernelGGL((ln_backward_kernel<T, VEC, NV, kBackwardWG, LPR, FULL_, BIAS_>), dim3(grid),             \
+                     dim3(kBackwardWG), 0, stream, L)
+  if (L.ld == LPR * VEC * NV) {
+    if (L.bias)
+      FWDMI_LN_LAUNCH(true, true);
+    else
+      FWDMI_LN_LAUNCH(true, false);
+  } else {
+    if (L.bias)
+      FWDMI_LN_LAUNCH(false, true);
+    else
+      FWDMI_LN_LAUNCH(false, false);
+  }
+#undef FWDMI_LN_LAUNCH
+  FWDMI_HIP_CHECK(hipGetLastError());
+  return FWDMI_OK;
+}
+
+// Calls f.template operator()<VEC, NV, LPR>() for the row's shape; false where rows are streamed.
+template <typename T, typename F>
+bool with_shape(int ld, F&& f) {
+  constexpr int kVec = 16 / sizeof(T);
+  constexpr int kDeep = 16 / kVec;
+  if (ld < kVec) {
+    f(std::integral_constant<int, 1>{}, std::integral_constant<int, 1>{}, std::integral_constant<int, 8>{});
+    return true;
+  }
+  const Shape s = row_shape(ld, kVec);
+  using V = std::integral_constant<int, kVec>;
+#define FWDMI_SHAPE(LPR_, NV_)                                                                       \
+  if (s.lpr == LPR_ && s.nv == NV_) {                                                                \
+    f(V{}, std::integral_constant<int, NV_>{}, std::integral_constant<int, LPR_>{});                 \
+    return true;                                                                                     \
+  }
+  FWDMI_SHAPE(8, 1)
+  FWDMI_SHAPE(16, 1)
+  FWDMI_SHAPE(32, 1)
+  FWDMI_SHAPE(64, 1)
+  FWDMI_SHAPE(64, 2)
+  FWDMI_SHAPE(256, 1)
+  FWDMI_SHAPE(256, 2)
+  if constexpr (kDeep == 4) {
+    FWDMI_SHAPE(64, 4)
+    FWDMI_SHAPE(256, 4)
+  }
+  FWDMI_SHAPE(512, kDeep)
+  FWDMI_SHAPE(512, 2 * kDeep)
+#undef FWDMI_SHAPE
+  return false;
+}
+
+// Rows of partials of a backward launch: its workgroups.
+int64_t backward_parts(int ld, int64_t rows, int dtype) {
+  if (rows == 0) return 0;
+  const int vec = dtype == FWDMI_F32 ? 4 : 8;
+  const Shape s = ld < vec ? Shape{8, 1} : row_shape(ld, vec);
+  if (s.lpr == 0) return std::min<int64_t>(rows, kStreamParts);
+  const int per = kBackwardWG / s.lpr;
+  return std::min<int64_t>((rows + per - 1) / per, kMaxParts);
+}
+
+bool streamed(int ld, int dtype) {
+  const int vec = dtype == FWDMI_F32 ? 4 : 8;
+  return ld >= vec && row_shape(ld, vec).lpr == 0;
+}
+
+template <typename T>
+int forward_typed(const LnTrain& L, hipStream_t stream) {
+  int rc = FWDMI_OK;
+  const bool done = with_shape<T>(L.ld, [&](auto vec, auto nv, auto lpr) {
+    rc = launch_forward<T, decltype(vec)::value, decltype(nv)::value, decltype(lpr)::value>(L, stream);
+  });
+  if (done) return rc;
+  const unsigned grid = (unsigned)std::min<int64_t>(L.rows, (int64_t)device_cus() * 4);
+  hipLaunchKernelGGL((ln_forward_stream_kernel<T>), dim3(grid), dim3(kStreamWG), 0, stream, L);
+  FWDMI_HIP_CHECK(hipGetLastError());
+  return FWDMI_OK;
+}
+
+template <typename T>
+int backward_typed(const LnTrain& L, int64_t parts, hipStream_t stream) {
+  int rc = FWDMI_OK;
+  const bool done = with_shape<T>(L.ld, [&](auto vec, auto nv, auto lpr) {
+    rc = launch_backward<T, decltype(vec)::value, decltype(nv)::value, decltype(lpr)::value>(L, (unsigned)parts, stream);
+  });
+  if (done) return rc;
+  const unsigned grid = (unsigned)std::min<int64_t>(L.rows, (int64_t)device_cus() * 4);
+  hipLaunchKernelGGL((ln_backward_stream_kernel<T>), dim3(grid), dim3(kStreamWG), 0, stream, L);
+  FWDMI_HIP_CHECK(hipGetLastError());
+  const dim3 cgrid((unsigned)(((int64_t)L.ld + 255) / 256), (unsigned)parts);
+  hipLaunchKernelGGL((ln_backward_columns_kernel<T>), cgrid, dim3(256), 0, stream, L);
+  FWDMI_HIP_CHECK(hipGetLastError());
+  return FWDMI_OK;
+}
+
+bool is_train_dtype(int t) { return t == FWDMI_F32 || t == FWDMI_F16 || t == FWDMI_BF16; }
+
+}  // namespace
+}  // namespace fwdmi
+
+extern "C" {
+
+int fwdmi_layer_norm_forward(void* stream, int32_t ld, int64_t n, const void* x, const void* skip, const float* beta,
+                             const float* gamma, const float* bias, void* y, void* sum, float* mean, float* rstd,
+                             int32_t dtype, float eps) {
+  using namespace fwdmi;
+  clear_error();
+  if (!is_train_dtype(dtype)) return set_error(FWDMI_ERR_UNSUPPORTED, "layer norm forward: unsupported dtype %d", dtype);
+  FWDMI_REQUIRE(ld > 0 && n >= 0 && n % ld == 0, "layer norm forward: n=%lld is not a multiple of ld=%d", (long long)n, ld);
+  if (n == 0) return FWDMI_OK;
+  FWDMI_REQUIRE(x && beta && gamma && y && mean && rstd, "layer norm forward: null pointer");
+  LnTrain L{};
+  L.x = x;
+  L.skip = skip;
+  L.gamma = gamma;
+  L.beta = beta;
+  L.bias = bias;
+  L.out = y;
+  L.sum = sum;
+  L.mean = mean;
+  L.rstd = rstd;
+  L.rows = n / ld;
+  L.ld = ld;
+  L.eps = eps;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (dtype == FWDMI_F16) return forward_typed<_Float16>(L, s);
+  if (dtype == FWDMI_BF16) return forward_typed<__bf16>(L, s);
+  return forward_typed<float>(L, s);
+}
+
+size_t fwdmi_layer_norm_backward_workspace(int32_t ld, int64_t n, int32_t dtype) {
+  using namespace fwdmi;
+  if (!is_train_dtype(dtype) || ld <= 0 || n <= 0 || n % ld != 0) return 0;
+  const int64_t rows = n / ld;
+  size_t bytes = (size_t)backward_parts(ld, rows, dtype) * 3 * (size_t)ld * sizeof(float);
+  if (streamed(ld, dtype)) bytes += (size_t)rows * 2 * sizeof(float);
+  return bytes;
+}
+
+int fwdmi_layer_norm_backward(void* stream, int32_t ld, int64_t n, const void* dy, const void* x, const void* skip,
+                              const void* dsum, const float* gamma, const float* bias, const float* mean,
+                              const float* rstd, void* dx, float* dgamma, float* dbeta, float* dbias, void* workspace,
+                              size_t workspace_size, int32_t dtype) {
+  using namespace fwdmi;
+  clear_error();
+  if (!is_train_dtype(dtype)) return set_error(FWDMI_ERR_UNSUPPORTED, "layer norm backward: unsupported dtype %d", dtype);
+  FWDMI_REQUIRE(ld > 0 && n >= 0 && n % ld == 0, "layer norm backward: n=%lld is not a multiple of ld=%d", (long long)n, ld);
+  FWDMI_REQUIRE(dgamma && dbeta && (bias == nullptr) == (dbias == nullptr),
+                "layer norm backward: dgamma and dbeta are written always, dbias exactly where there is a bias");
+  const int64_t rows = n / ld;
+  const int kinds = bias ? 3 : 2;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const int64_t parts = backward_parts(ld, rows, dtype);
+  LnTrain L{};
+  if (rows > 0) {
+    FWDMI_REQUIRE(dy && x && gamma && mean && rstd && dx, "layer norm backward: null pointer");
+    const size_t need = fwdmi_layer_norm_backward_workspace(ld, n, dtype);
+    FWDMI_REQUIRE(workspace && workspace_size >= need && reinterpret_cast<uintptr_t>(workspace) % 4 == 0,
+                  "layer norm backward: workspace of %zu bytes, %zu needed", workspace ? workspace_size : (size_t)0, need);
+    L.dy = dy;
+    L.x = x;
+    L.skip = skip;
+    L.dsum = dsum;
+    L.gamma = gamma;
+    L.bias = bias;
+    L.mean = const_cast<float*>(mean);
+    L.rstd = const_cast<float*>(rstd);
+    L.out = dx;
+    L.rows = rows;
+    L.ld = ld;
+    float* const ws = static_cast<float*>(workspace);
+    L.c1 = ws + parts * 3 * (int64_t)ld;  // read and written by streamed rows only
+    L.c2 = L.c1 + rows;
+    if (parts == 1) {  // one workgroup's sums are the result
+      L.part_gamma = dgamma;
+      L.part_beta = dbeta;
+      L.part_bias = dbias;
+    } else {
+      L.part_gamma = ws;
+      L.part_beta = ws + ld;
+      L.part_bias = bias ? ws + 2 * (int64_t)ld : nullptr;
+      L.part_stride = (int64_t)kinds * ld;
+    }
+    const int rc = dtype == FWDMI_F16    ? backward_typed<_Float16>(L, parts, s)
+                   : dtype == FWDMI_BF16 ? backward_typed<__bf16>(L, parts, s)
+                                         : backward_typed<float>(L, parts, s);
+    if (rc != FWDMI_OK || parts == 1) return rc;
+  }
+  ColumnSums S{};
+  S.part = static_cast<const float*>(workspace);
+  S.out[0] = dgamma;
+  S.out[1] = dbeta;
+  S.out[2] = dbias;
+  S.parts = (int32_t)parts;
+  S.ld = ld;
+  S.kinds = kinds;
+  const unsigned grid = (unsigned)(((int64_t)kinds * ld + 63) / 64);
+  hipLaunchKernelGGL(column_sums_kernel, dim3(grid), dim3(64 * kSumWaves), 0, s, S);
+  FWDMI_HIP_CHECK(hipGetLastError());
+  return FWDMI_OK;
+}
+
+}  // extern "C"

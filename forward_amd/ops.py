@@ -12,6 +12,7 @@ import torch
 from . import lib
 
 _FDT = {torch.float32: lib.F32, torch.float16: lib.F16}
+_TDT = {torch.float32: lib.F32, torch.float16: lib.F16, torch.bfloat16: lib.BF16}   # training and linear launchers
 _IDT = {torch.int32: lib.I32, torch.int64: lib.I64}
 MODES = {"sum": lib.OP_SUM, "mean": lib.OP_MEAN, "max": lib.OP_MAX, "square_sum": lib.OP_SQUARE_SUM}
 
@@ -376,3 +377,114 @@ def emb_layer_norm(input_ids, segment_ids, input_mask, word, pos, tok, gamma, be
                                               C.byref(x)))
     del keep
     return out, mask_idx
+
+
+# ---- training and linear launchers --------------------------------------------------------------
+
+def _place(x, stream, **others):
+    """The device and stream of a call on ``x``: every operand lies on ``x``'s device, the call runs there
+    whatever the current device is, on ``stream`` or that device's current stream."""
+    for name, t in others.items():
+        _require(t is None or t.device == x.device, '%s lies on the device of the first operand' % name)
+    if stream is not None:
+        _require(stream.device == x.device, 'stream belongs to the device of the first operand')
+    return x.device
+
+
+class _On:
+    """Allocations and the launch of one call: on the operands' device, on the call's stream (results and
+    workspaces then belong to the stream that writes them)."""
+
+    def __init__(self, device, stream):
+        self.device, self.stream, self.guard = device, stream, None
+
+    def __enter__(self):
+        if self.stream is not None:
+            self.guard = torch.cuda.stream(self.stream)
+        elif self.device.index != torch.cuda.current_device():
+            self.guard = torch.cuda.device(self.device)
+        if self.guard is not None:
+            self.guard.__enter__()
+        return C.c_void_p(torch.cuda.current_stream().cuda_stream)
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
+def _train_dtype(x, name):
+    if x.dtype not in _TDT:
+        raise TypeError("%s must be float32, float16 or bfloat16, not %s" % (name, x.dtype))
+    return _TDT[x.dtype]
+
+
+def _vector(t, n, name):
+    _require(_dev(t, name).dtype == torch.float32 and t.numel() == n, '%s is float32 with %d elements' % (name, n))
+    return t
+
+
+def _like(t, x, name):
+    _require(_dev(t, name).dtype == x.dtype and t.shape == x.shape, '%s has the shape and dtype of the input' % name)
+    return t
+
+
+def layer_norm_forward(x, gamma, beta, skip=None, bias=None, eps=0.0, want_sum=False, stream=None):
+    """``LN(h)``, ``h = x (+ skip) (+ bias)``, over the last axis for training: ``(y, mean, rstd)``, and with
+    ``want_sum`` ``(y, mean, rstd, h)`` with ``h`` rounded to ``x``'s dtype (the residual stream of a pre-norm layer).
+
+    ``x`` / ``skip``: float32, float16 or bfloat16; gamma / beta / bias: float32 vectors; mean / rstd: float32,
+    ``x.shape[:-1]``.
+    """
+    x = _dev(x, "input")
+    dt = _train_dtype(x, "input")
+    _require(x.dim() >= 1 and x.shape[-1] > 0, 'input has a last axis of at least one element')
+    ld = x.shape[-1]
+    _vector(gamma, ld, "gamma")
+    _vector(beta, ld, "beta")
+    if bias is not None:
+        _vector(bias, ld, "bias")
+    if skip is not None:
+        _like(skip, x, "skip")
+    device = _place(x, stream, gamma=gamma, beta=beta, skip=skip, bias=bias)
+    with _On(device, stream) as s:
+        y = torch.empty_like(x)
+        h = torch.empty_like(x) if want_sum else None
+        mean = torch.empty(x.shape[:-1], dtype=torch.float32, device=device)
+        rstd = torch.empty_like(mean)
+        lib.check(lib.dll.fwdmi_layer_norm_forward(s, ld, x.numel(), _p(x), _p(skip), _p(beta), _p(gamma), _p(bias), _p(y),
+                                                   _p(h), _p(mean), _p(rstd), dt, eps))
+    return (y, mean, rstd, h) if want_sum else (y, mean, rstd)
+
+
+def layer_norm_backward(dy, x, gamma, mean, rstd, skip=None, bias=None, dsum=None, stream=None):
+    """Gradient of ``layer_norm_forward``: ``(dx, dgamma, dbeta)``, with a bias ``(dx, dgamma, dbeta, dbias)``.
+
+    ``x`` / ``skip`` / ``bias`` as the forward call took them, or its sum as ``x`` alone; ``dx`` is the gradient of
+    ``x`` and of ``skip`` alike.  ``dsum``: a gradient that reaches the sum from elsewhere, added to ``dx``.
+    dgamma / dbeta / dbias are float32, summed over the rows in a fixed order.
+    """
+    x = _dev(x, "input")
+    dt = _train_dtype(x, "input")
+    _require(x.dim() >= 1 and x.shape[-1] > 0, 'input has a last axis of at least one element')
+    ld = x.shape[-1]
+    rows = x.numel() // ld
+    _like(dy, x, "dy")
+    _vector(gamma, ld, "gamma")
+    _vector(mean, rows, "mean")
+    _vector(rstd, rows, "rstd")
+    if skip is not None:
+        _like(skip, x, "skip")
+    if bias is not None:
+        _vector(bias, ld, "bias")
+    if dsum is not None:
+        _like(dsum, x, "dsum")
+    device = _place(x, stream, dy=dy, gamma=gamma, mean=mean, rstd=rstd, skip=skip, bias=bias, dsum=dsum)
+    with _On(device, stream) as s:
+        dx = torch.empty_like(x)
+        grads = torch.empty((2 if bias is None else 3, ld), dtype=torch.float32, device=device).unbind(0)
+        size = lib.dll.fwdmi_layer_norm_backward_workspace(ld, x.numel(), dt)
+        ws = torch.empty((size,), dtype=torch.uint8, device=device)
+        lib.check(lib.dll.fwdmi_layer_norm_backward(s, ld, x.numel(), _p(dy), _p(x), _p(skip), _p(dsum), _p(gamma),
+                                                    _p(bias), _p(mean), _p(rstd), _p(dx), _p(grads[0]), _p(grads[1]),
+                                                    _p(grads[2]) if bias is not None else None, _p(ws), size, dt))
+    return (dx,) + tuple(grads)

@@ -38,6 +38,7 @@ extern "C" {
 #define FWDMI_I8 2
 #define FWDMI_I32 3
 #define FWDMI_BOOL 4
+#define FWDMI_BF16 7 /* bfloat16: the training and linear launchers only */
 #define FWDMI_I64 10
 
 /* ---- plugin field types: values follow nvinfer1::PluginFieldType -------------------------- */
@@ -303,6 +304,35 @@ int fwdmi_emb_layer_norm_ex(void* stream, int32_t S, int32_t B, int32_t ld, cons
                             int32_t word_count, int32_t pos_count, int32_t tok_count, void* output,
                             int32_t* mask_idx, int32_t dtype, float eps, int32_t* oob_flag,
                             const fwdmi_emb_ext* ext);
+
+/*
+ * LayerNorm for training: out = LN(h), h = x (+ skip) (+ bias), keeping what the backward pass reads.
+ *   x, skip (may be NULL), y [rows, ld] in `dtype` (FWDMI_F32 | FWDMI_F16 | FWDMI_BF16), rows = n / ld;
+ *   sum (may be NULL) [rows, ld] in `dtype`: h rounded once, for layers whose residual stream goes on unnormalised
+ *   (y is computed from the unrounded h);
+ *   mean, rstd fp32 [rows];  gamma / beta / bias fp32 [ld], bias may be NULL.
+ * Operands need the alignment of their elements only; outputs overlap neither each other nor an input.
+ * (The reference is an inference engine and has no counterpart of this and the next launcher.)
+ */
+int fwdmi_layer_norm_forward(void* stream, int32_t ld, int64_t n, const void* x, const void* skip, const float* beta,
+                             const float* gamma, const float* bias, void* y, void* sum, float* mean, float* rstd,
+                             int32_t dtype, float eps);
+
+/*
+ * Its gradient: dx = dLN(dy) (+ dsum), dgamma, dbeta and, where there is a bias, dbias.
+ *   dx is the gradient of x, of skip and of each row's bias alike (dbias sums it over the rows, without dsum);
+ *   x / skip / bias as given to the forward call, or x = its `sum` with skip = bias = NULL;
+ *   dsum (may be NULL) [rows, ld]: a gradient that reaches the sum from elsewhere;
+ *   dgamma, dbeta, dbias fp32 [ld], overwritten (zeros for n == 0); dbias is NULL exactly where bias is.
+ * `workspace`: device memory of fwdmi_layer_norm_backward_workspace(ld, n, dtype) bytes, 4-byte aligned, used by
+ * this call alone until it has run on `stream` (calls in flight together need one each).
+ * Sums are added in a fixed order: results repeat bit for bit.
+ */
+size_t fwdmi_layer_norm_backward_workspace(int32_t ld, int64_t n, int32_t dtype);
+int fwdmi_layer_norm_backward(void* stream, int32_t ld, int64_t n, const void* dy, const void* x, const void* skip,
+                              const void* dsum, const float* gamma, const float* bias, const float* mean,
+                              const float* rstd, void* dx, float* dgamma, float* dbeta, float* dbias, void* workspace,
+                              size_t workspace_size, int32_t dtype);
 
 /* ========================================================================================= *
  *  2. Plugin objects (opaque handles over the C++ classes in fwdmi_plugin.h)
