@@ -1,0 +1,84 @@
+// Slices of a few elements at any element alignment, and the sum of partial rows: shared by the training and linear
+// kernels.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include "../common.h"
+#include "device_util.h"
+
+namespace fwdmi {
+namespace {
+
+// N elements at any element alignment (one global_load_dwordx4 where the slice is 16 bytes).
+template <typename T, int N>
+__device__ __forceinline__ Pack<T, N> load_slice(const T FWDMI_GLOBAL* p) {
+  Pack<T, N> r;
+  if constexpr (N == 1) {
+    r.v[0] = *p;
+  } else {
+    typedef T V __attribute__((ext_vector_type(N), aligned(sizeof(T))));
+    const V x = *(const V FWDMI_GLOBAL*)p;
+    __builtin_memcpy(&r, &x, sizeof(r));
+  }
+  return r;
+}
+template <typename T, int N>
+__device__ __forceinline__ void store_slice(T FWDMI_GLOBAL* p, const Pack<T, N>& r) {
+  if constexpr (N == 1) {
+    *p = r.v[0];
+  } else {
+    typedef T V __attribute__((ext_vector_type(N), aligned(sizeof(T))));
+    V x;
+    __builtin_memcpy(&x, &r, sizeof(r));
+    *(V FWDMI_GLOBAL*)p = x;
+  }
+}
+
+// Adds `parts` rows of partials in a fixed order: 64 columns per workgroup, its sixteen waves each take every
+// sixteenth row.  parts == 0 leaves zeros.
+struct ColumnSums {
+  const float* part;  // [parts][kinds * ld]
+  float* out[3];      // [ld] each
+  int32_t parts, ld, kinds;
+};
+constexpr int kSumWaves = 16;
+__global__ __launch_bounds__(64 * kSumWaves) void column_sums_kernel(const ColumnSums S) {
+  __shared__ float s_red[kSumWaves][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t width = (int64_t)S.kinds * S.ld;
+  const int64_t c = (int64_t)blockIdx.x * 64 + lane;
+  float a = 0.0f;
+  if (c < width)
+    for (int p = wave; p < S.parts; p += kSumWaves) a += gconst<float>(S.part)[p * width + c];
+  s_red[wave][lane] = a;
+  __syncthreads();
+  if (wave == 0 && c < width) {
+    for (int k = 1; k < kSumWaves; ++k) a += s_red[k][lane];
+    const int kind = (int)(c / S.ld);
+    float* const out = kind == 0 ? S.out[0] : kind == 1 ? S.out[1] : S.out[2];
+    gmut<float>(out)[c - (int64_t)kind * S.ld] = a;
+  }
+}
+
+inline int launch_column_sums(const ColumnSums& S, hipStream_t stream) {
+  const unsigned grid = (unsigned)(((int64_t)S.kinds * S.ld + 63) / 64);
+  hipLaunchKernelGGL(column_sums_kernel, dim3(grid), dim3(64 * kSumWaves), 0, stream, S);
+  FWDMI_HIP_CHECK(hipGetLastError());
+  return FWDMI_OK;
+}
+
+inline int device_cus() {
+  int dev = 0, v = 0;
+  if (hipGetDevice(&dev) == hipSuccess &&
+      hipDeviceGetAttribute(&v, hipDeviceAttributeMultiprocessorCount, dev) == hipSuccess && v > 0)
+    return v;
+  (void)hipGetLastError();
+  return 256;
+}
+
+// Types of the training and linear launchers.
+inline bool is_train_dtype(int t) { return t == FWDMI_F32 || t == FWDMI_F16 || t == FWDMI_BF16; }
+
+}  // namespace
+}  // namespace fwdmi

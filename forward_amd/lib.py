@@ -22,6 +22,7 @@ OK, ERR_UNSUPPORTED, ERR_BAD_ARG, ERR_HIP, ERR_NOT_CONFIGURED, ERR_TRUNCATED = 0
 F32, F16, I8, I32, BOOL, BF16, I64 = 0, 1, 2, 3, 4, 7, 10
 FIELD_F16, FIELD_F32, FIELD_F64, FIELD_I8, FIELD_I16, FIELD_I32, FIELD_CHAR, FIELD_DIMS, FIELD_UNKNOWN = range(9)
 FORMAT_LINEAR = 0
+ACT_NONE, ACT_RELU, ACT_GELU, ACT_GELU_TANH, ACT_SILU = range(5)
 OP_SUM, OP_MEAN, OP_MAX, OP_SQUARE_SUM, OP_GATHER = 0, 1, 2, 3, 999
 BAG_XCD_TABLE_AFFINITY = 1
 BAG_TABLE_WEIGHTS = 2
@@ -106,6 +107,10 @@ SIGNATURES = {
     "fwdmi_layer_norm_backward_workspace": (_sz, [_i32, _i64, _i32]),
     "fwdmi_layer_norm_backward": (C.c_int, [_vp, _i32, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
                                             _vp, _sz, _i32]),
+    "fwdmi_linear_workspace": (_sz, [_i64, _i64, _i64, _i32]),
+    "fwdmi_linear": (C.c_int, [_vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _vp, _sz]),
+    "fwdmi_linear_backward_workspace": (_sz, [_i64, _i64, _i64, _i32, _i32]),
+    "fwdmi_linear_backward": (C.c_int, [_vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _vp, _sz]),
     "fwdmi_get_plugin_creator": (_vp, [_cp, _cp]),
     "fwdmi_registry_size": (C.c_int, []),
     "fwdmi_registry_at": (_vp, [C.c_int]),

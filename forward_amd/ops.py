@@ -14,6 +14,8 @@ from . import lib
 _FDT = {torch.float32: lib.F32, torch.float16: lib.F16}
 _TDT = {torch.float32: lib.F32, torch.float16: lib.F16, torch.bfloat16: lib.BF16}   # training and linear launchers
 _IDT = {torch.int32: lib.I32, torch.int64: lib.I64}
+ACTIVATIONS = {"none": lib.ACT_NONE, "relu": lib.ACT_RELU, "gelu": lib.ACT_GELU, "gelu_tanh": lib.ACT_GELU_TANH,
+               "silu": lib.ACT_SILU}
 MODES = {"sum": lib.OP_SUM, "mean": lib.OP_MEAN, "max": lib.OP_MAX, "square_sum": lib.OP_SQUARE_SUM}
 
 
@@ -488,3 +490,76 @@ def layer_norm_backward(dy, x, gamma, mean, rstd, skip=None, bias=None, dsum=Non
                                                     _p(bias), _p(mean), _p(rstd), _p(dx), _p(grads[0]), _p(grads[1]),
                                                     _p(grads[2]) if bias is not None else None, _p(ws), size, dt))
     return (dx,) + tuple(grads)
+
+
+def _act(activation):
+    _require(activation in ACTIVATIONS, 'activation is one of %s' % ", ".join(ACTIVATIONS))
+    return ACTIVATIONS[activation]
+
+
+def _weight(weight, x):
+    _require(_dev(weight, "weight").dim() == 2 and weight.dtype == x.dtype, 'weight is [out, in] of the input dtype')
+    _require(x.dim() >= 1 and x.shape[-1] == weight.shape[1], 'the last axis of the input is as long as a row of weight')
+    return weight.shape
+
+
+def linear(x, weight, bias=None, activation="none", residual=None, want_preact=False, stream=None):
+    """``act(x weight^T (+ bias)) (+ residual)`` over the last axis, one rounding at the end.
+
+    ``x`` ``[..., in]``, ``weight`` ``[out, in]``, ``residual`` ``[..., out]``: float32, float16 or bfloat16 alike;
+    ``bias``: a float32 vector; ``activation``: a key of ``ACTIVATIONS``.  With ``want_preact`` returns
+    ``(y, z)``, ``z`` the value in front of the activation, which ``linear_backward`` reads.
+    """
+    x = _dev(x, "input")
+    dt = _train_dtype(x, "input")
+    act = _act(activation)
+    n, k = _weight(weight, x)
+    shape = x.shape[:-1] + (n,)
+    m = 1
+    for v in x.shape[:-1]:
+        m *= v
+    if bias is not None:
+        _vector(bias, n, "bias")
+    if residual is not None:
+        _require(_dev(residual, "residual").dtype == x.dtype and residual.shape == shape,
+                 'residual has the shape of the result and the dtype of the input')
+    device = _place(x, stream, weight=weight, bias=bias, residual=residual)
+    with _On(device, stream) as s:
+        y = torch.empty(shape, dtype=x.dtype, device=device)
+        z = torch.empty_like(y) if want_preact else None
+        size = lib.dll.fwdmi_linear_workspace(m, n, k, dt)
+        ws = torch.empty((size,), dtype=torch.uint8, device=device) if size else None
+        lib.check(lib.dll.fwdmi_linear(s, m, n, k, _p(x), _p(weight), _p(bias), _p(residual), _p(y), _p(z), act, dt, _p(ws),
+                                       size))
+    return (y, z) if want_preact else y
+
+
+def linear_backward(dy, x, weight, preact=None, activation="none", want_dx=True, want_dweight=True, want_dbias=True,
+                    stream=None):
+    """Gradient of ``linear``: ``(dx, dweight, dbias)``, without those not wanted (the residual's is ``dy`` itself).
+
+    ``preact``: what ``linear`` returned for ``want_preact``, needed with an activation.  ``dx`` and ``dweight`` have the
+    input's dtype, ``dbias`` is float32.
+    """
+    x = _dev(x, "input")
+    dt = _train_dtype(x, "input")
+    act = _act(activation)
+    n, k = _weight(weight, x)
+    shape = x.shape[:-1] + (n,)
+    m = 1
+    for v in x.shape[:-1]:
+        m *= v
+    _require(_dev(dy, "dy").dtype == x.dtype and dy.shape == shape, 'dy has the shape of the result and the dtype of the input')
+    if act != lib.ACT_NONE:
+        _require(preact is not None and _dev(preact, "preact").dtype == x.dtype and preact.shape == shape,
+                 'an activation needs preact, with the shape of the result and the dtype of the input')
+    device = _place(x, stream, dy=dy, weight=weight, preact=preact)
+    with _On(device, stream) as s:
+        dx = torch.empty_like(x) if want_dx else None
+        dw = torch.empty_like(weight) if want_dweight else None
+        db = torch.empty((n,), dtype=torch.float32, device=device) if want_dbias else None
+        size = lib.dll.fwdmi_linear_backward_workspace(m, n, k, act, dt)
+        ws = torch.empty((size,), dtype=torch.uint8, device=device) if size else None
+        lib.check(lib.dll.fwdmi_linear_backward(s, m, n, k, _p(dy), _p(x), _p(weight), _p(preact), _p(dx), _p(dw), _p(db),
+                                                act, dt, _p(ws), size))
+    return tuple(t for t in (dx, dw, db) if t is not None)

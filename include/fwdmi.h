@@ -55,6 +55,13 @@ extern "C" {
 /* ---- tensor format: nvinfer1::TensorFormat::kLINEAR ---------------------------------------- */
 #define FWDMI_FORMAT_LINEAR 0
 
+/* ---- activations of the linear launchers -------------------------------------------------- */
+#define FWDMI_ACT_NONE 0
+#define FWDMI_ACT_RELU 1
+#define FWDMI_ACT_GELU 2      /* z Phi(z), Phi the normal distribution function */
+#define FWDMI_ACT_GELU_TANH 3 /* z (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))) / 2 */
+#define FWDMI_ACT_SILU 4      /* z / (1 + exp(-z)) */
+
 /* ---- bag reduction codes: ReduceOperation, embedding_bag_plugin.h:39 ----------------------- */
 #define FWDMI_OP_SUM 0
 #define FWDMI_OP_MEAN 1
@@ -333,6 +340,34 @@ int fwdmi_layer_norm_backward(void* stream, int32_t ld, int64_t n, const void* d
                               const void* dsum, const float* gamma, const float* bias, const float* mean,
                               const float* rstd, void* dx, float* dgamma, float* dbeta, float* dbias, void* workspace,
                               size_t workspace_size, int32_t dtype);
+
+/*
+ * Linear layer: y = act(z) (+ residual), z = x w^T (+ bias): the product in front of a SkipLayerNorm.
+ *   x [m, k], w [n, k], residual [m, n] (may be NULL), y [m, n] in `dtype` (FWDMI_F32 | FWDMI_F16 | FWDMI_BF16),
+ *   packed rows; bias fp32 [n] or NULL; preact (may be NULL) [m, n]: z rounded to `dtype`, what the backward pass
+ *   reads; act: FWDMI_ACT_*.  Sums, activation and residual are fp32, rounded once.
+ * Any sizes up to 2^30 each and any element alignment; operands of whole 16-byte lines (k a multiple of 8, fp32 4,
+ * and pointers of 16) are the fast ones.  Outputs overlap neither each other nor an input.
+ * `workspace`: fwdmi_linear_workspace(m, n, k, dtype) bytes (often 0) on a 16-byte boundary, used by this call alone
+ * until it has run on `stream` (calls in flight together need one each).
+ * (In the reference a fully connected layer is TensorRT's own, followed by activation and element-wise layers.)
+ */
+size_t fwdmi_linear_workspace(int64_t m, int64_t n, int64_t k, int32_t dtype);
+int fwdmi_linear(void* stream, int64_t m, int64_t n, int64_t k, const void* x, const void* w, const float* bias,
+                 const void* residual, void* y, void* preact, int32_t act, int32_t dtype, void* workspace,
+                 size_t workspace_size);
+
+/*
+ * Its gradient: dz = dy act'(preact), dx = dz w, dw = dz^T x, dbias = sum of dz over the rows (the residual's
+ * gradient is dy itself).  dx [m, k], dw [n, k] in `dtype`, dbias fp32 [n]: each may be NULL when not wanted, the
+ * others are overwritten.  preact is not read with FWDMI_ACT_NONE.  dz is rounded to `dtype` before the products (as
+ * the operand of a matrix instruction has to be); dbias sums it unrounded.  relu's slope at 0 is 0.
+ * Sums run in a fixed order: results repeat bit for bit.  `workspace` as above.
+ */
+size_t fwdmi_linear_backward_workspace(int64_t m, int64_t n, int64_t k, int32_t act, int32_t dtype);
+int fwdmi_linear_backward(void* stream, int64_t m, int64_t n, int64_t k, const void* dy, const void* x, const void* w,
+                          const void* preact, void* dx, void* dw, float* dbias, int32_t act, int32_t dtype,
+                          void* workspace, size_t workspace_size);
 
 /* ========================================================================================= *
  *  2. Plugin objects (opaque handles over the C++ classes in fwdmi_plugin.h)

@@ -67,3 +67,57 @@ def test_layer_norm_workspace_sizes():
     assert f(16, 0, lib.F32) == 0 and f(0, 16, lib.F32) == 0 and f(16, 17, lib.F32) == 0 and f(16, 16, lib.I8) == 0
     assert f(1024, 8192 * 1024, lib.F16) >= 3 * 1024 * 4
     assert f(100000, 5 * 100000, lib.F32) >= 5 * 8 + 3 * 100000 * 4
+
+
+def test_linear_refuses():
+    good = dict(x=z(4, 16), weight=z(8, 16))
+    for change in (dict(weight=z(8, 15)), dict(weight=z(8, 16, dtype=torch.float16)), dict(weight=z(8, 16, 1)), dict(bias=z(16)),
+                   dict(bias=z(8, dtype=torch.float16)), dict(residual=z(4, 16)), dict(residual=z(4, 8, dtype=torch.float16)),
+                   dict(activation="tanh"), dict(weight=z(16, 8).t())):
+        with pytest.raises(ValueError):
+            ops.linear(**{**good, **change})
+    with pytest.raises(TypeError):
+        ops.linear(z(4, 16, dtype=torch.float64), z(8, 16, dtype=torch.float64))
+
+
+def test_linear_backward_refuses():
+    good = dict(dy=z(4, 8), x=z(4, 16), weight=z(8, 16), preact=z(4, 8), activation="gelu")
+    for change in (dict(dy=z(4, 16)), dict(dy=z(4, 8, dtype=torch.float16)), dict(preact=None), dict(preact=z(4, 16)),
+                   dict(preact=z(4, 8, dtype=torch.bfloat16)), dict(weight=z(8, 8)), dict(activation="")):
+        with pytest.raises(ValueError):
+            ops.linear_backward(**{**good, **change})
+
+
+def test_linear_launchers_refuse():
+    d = lib.dll
+    none6 = [None] * 6
+    assert d.fwdmi_linear(None, 4, 8, 16, *none6, lib.ACT_NONE, lib.I8, None, 0) == lib.ERR_UNSUPPORTED
+    assert d.fwdmi_linear(None, 4, 8, 16, *none6, 9, lib.F16, None, 0) == lib.ERR_BAD_ARG
+    assert d.fwdmi_linear(None, 4, 8, 16, *none6, -1, lib.F16, None, 0) == lib.ERR_BAD_ARG
+    assert d.fwdmi_linear(None, -4, 8, 16, *none6, 0, lib.F16, None, 0) == lib.ERR_BAD_ARG
+    assert d.fwdmi_linear(None, 4, 8, 1 << 40, *none6, 0, lib.F16, None, 0) == lib.ERR_BAD_ARG
+    assert d.fwdmi_linear(None, 4, 8, 16, *none6, 0, lib.F16, None, 0) == lib.ERR_BAD_ARG            # null pointers
+    assert d.fwdmi_linear(None, 0, 8, 16, *none6, 0, lib.F16, None, 0) == lib.OK                     # nothing to do
+    need = d.fwdmi_linear_workspace(16, 64, 1 << 16, lib.F16)
+    assert need > 0                                                                                # a long sum is split
+    some = [64, 64, None, None, 64, None]
+    assert d.fwdmi_linear(None, 16, 64, 1 << 16, *some, 0, lib.F16, 64, need - 1) == lib.ERR_BAD_ARG
+    assert "workspace" in lib.last_error()
+    assert d.fwdmi_linear(None, 16, 64, 1 << 16, *some, 0, lib.F16, 72, need) == lib.ERR_BAD_ARG     # off its boundary
+    none7 = [None] * 7
+    assert d.fwdmi_linear_backward(None, 4, 8, 16, *none7, 0, lib.BOOL, None, 0) == lib.ERR_UNSUPPORTED
+    assert d.fwdmi_linear_backward(None, 4, 8, 16, *none7, 0, lib.F16, None, 0) == lib.ERR_BAD_ARG
+    args = [64, 64, 64, None, 64, 64, 64]
+    assert d.fwdmi_linear_backward(None, 4, 8, 16, *args, lib.ACT_GELU, lib.F16, 64, 1 << 20) == lib.ERR_BAD_ARG
+    assert "pre-activation" in lib.last_error()
+    assert d.fwdmi_linear_backward(None, 4, 8, 16, *args, lib.ACT_NONE, lib.F16, None, 0) == lib.ERR_BAD_ARG
+    assert "workspace" in lib.last_error()
+
+
+def test_linear_workspace_sizes():
+    d = lib.dll
+    assert d.fwdmi_linear_workspace(0, 8, 8, lib.F16) == 0 and d.fwdmi_linear_workspace(8, 8, -1, lib.F16) == 0
+    assert d.fwdmi_linear_workspace(8, 8, 8, lib.I32) == 0
+    # dz and the column sums' partials at least
+    assert d.fwdmi_linear_backward_workspace(100, 64, 64, lib.ACT_GELU, lib.F16) >= 100 * 64 * 2 + 64 * 4
+    assert d.fwdmi_linear_backward_workspace(0, 64, 64, lib.ACT_GELU, lib.F16) == 0
