@@ -8,44 +8,80 @@
 namespace fwdmi {
 namespace {
 
-// The tile whose launch fills the CUs best, and how many splits of t it takes to do so when the tiles are few.
-Plan make_plan(int ni, int nj, int nt, int elem, bool direct) {
+// What bounds a product's operands: the layouts (0 both along t, 1 a along and b across, 2 both across), whether they
+// may be loaded directly and, if so, whether rows across t end inside a chunk.
+struct Operands {
+  int layouts, elem;
+  bool direct, ragged;
+};
+
+// The tile and the number of splits of t with the shortest estimated time.  A CU works off its workgroups' steps, each
+// as long as its loads (direct ones reach 90 KB/us per CU, those through registers 40) or its matrix instructions take
+// (kRate: flop/us per CU that the steps of each tile sustain, bf16; fp32 instructions bound all tiles alike), plus what a
+// round of tiles spends outside its steps and, with splits, the second launch and the partial products' way through
+// the caches.  Measured: 8192 x 4096 x 1024 64 us with 256 x 256, 74 with 256 x 128, 84 with 128 x 128;
+// 8192 x 1024 x 4096 66 us with 256 x 128, 67 with 128 x 128; 384 x 1024 x 4096 12 us with 64 x 32, 15 with 64 x 64,
+// 20 and more with 128 x 128.
+Plan make_plan(int ni, int nj, int nt, const Operands& o) {
+  static const double kRate[kTileKinds] = {6.0e6, 4.6e6, 4.4e6, 3.5e6, 3.0e6};
+  static const double kRound[kTileKinds] = {9.0, 4.0, 3.0, 1.5, 1.0};
   const int cus = device_cus();
-  const int all = ceil_div(nt, kStepBytes / elem);
-  Plan p{kSmall, 64, 64, 1, all};
-  if (elem == 2 && direct && (int64_t)ceil_div(ni, 256) * ceil_div(nj, 256) >= cus * 3 / 4)
-    p = Plan{kBig, 256, 256, 1, all};
-  else if ((int64_t)ceil_div(ni, 128) * ceil_div(nj, 128) >= cus * 3 / 4)
-    p = Plan{kMid, 128, 128, 1, all};
-  const int64_t tiles = (int64_t)ceil_div(ni, p.ti) * ceil_div(nj, p.tj);
-  if (tiles < cus && all > 1) {
-    // at least four steps each, so that a split is worth its partial tile
-    int splits = (int)std::min<int64_t>((2 * cus + tiles - 1) / tiles, std::max(1, all / 4));
-    p.steps_per_split = ceil_div(all, splits);
-    p.splits = ceil_div(all, p.steps_per_split);
+  Plan best{};
+  double best_us = 1e30;
+  for (int kind = o.elem == 2 && o.direct ? k256x256 : k128x128; kind < kTileKinds; ++kind) {
+    const TileShape t = kTiles[kind];
+    Plan p{(TileKind)kind, 1, 0, 0, 0};
+    tail_of(nt, t.step_bytes / o.elem, o.direct && o.ragged, p.whole_steps, p.tail);
+    const int all = p.whole_steps + (p.tail > 0);
+    const int64_t tiles = (int64_t)ceil_div(ni, t.ti) * ceil_div(nj, t.tj);
+    const double load = (t.ti + t.tj) * t.step_bytes / ((o.direct ? 90.0 : 40.0) * 1024);
+    const double flops = 2.0 * t.ti * t.tj * (t.step_bytes / o.elem) / (o.elem == 2 ? kRate[kind] : 0.55e6);
+    const double step = std::max(load, flops);
+    for (int target = 0; target <= 2; ++target) {  // one workgroup per tile, or splits for one or two per CU
+      const int64_t want = target == 0 ? 1 : target * (int64_t)cus / tiles;
+      if (target > 0 && want < 2) continue;
+      const int splits = (int)std::min<int64_t>(want, std::max(1, all / 2));
+      p.steps_per_split = std::max(1, ceil_div(all, splits));
+      p.splits = std::max(1, ceil_div(all, p.steps_per_split));
+      double us = 2.0 + ceil_div(tiles * p.splits, cus) * (kRound[kind] + p.steps_per_split * step);
+      if (p.splits > 1) us += 4.0 + 8.0 * p.splits * ni * nj / 4.0e6;
+      if (us < best_us) {
+        best_us = us;
+        best = p;
+      }
+    }
   }
-  return p;
+  return best;
 }
 
 size_t partial_bytes(const Plan& p, int ni, int nj) {
   return p.splits > 1 ? (size_t)p.splits * ni * nj * sizeof(float) : 0;
 }
 
+bool ragged_rows(int layouts, int ni, int nj, int elem) {
+  const int chunk = 16 / elem;
+  return (layouts == 2 && ni % chunk != 0) || (layouts >= 1 && nj % chunk != 0);
+}
+
 int run(Product& P, int layouts, int dtype, void* workspace, hipStream_t stream) {
   const int elem = dtype == FWDMI_F32 ? 4 : 2;
-  const bool direct = direct_ok(P.a, P.lda, elem, layouts == 2 ? P.ni : P.nt) &&
-                      direct_ok(P.b, P.ldb, elem, layouts == 0 ? P.nt : P.nj);
-  const Plan plan = make_plan(P.ni, P.nj, P.nt, elem, direct);
+  const Operands o{layouts, elem, direct_ok(P.a, P.lda, elem) && direct_ok(P.b, P.ldb, elem),
+                   ragged_rows(layouts, P.ni, P.nj, elem)};
+  const Plan plan = make_plan(P.ni, P.nj, P.nt, o);
   P.partial = plan.splits > 1 ? static_cast<float*>(workspace) : nullptr;
-  return dtype == FWDMI_F16    ? run_product_f16(P, layouts, plan, direct, stream)
-         : dtype == FWDMI_BF16 ? run_product_bf16(P, layouts, plan, direct, stream)
-                               : run_product_f32(P, layouts, plan, direct, stream);
+  return dtype == FWDMI_F16    ? run_product_f16(P, layouts, plan, o.direct, stream)
+         : dtype == FWDMI_BF16 ? run_product_bf16(P, layouts, plan, o.direct, stream)
+                               : run_product_f32(P, layouts, plan, o.direct, stream);
 }
 
 // Partial products of either plan (which of the two runs depends on the operands' alignment).
-size_t product_bytes(int64_t ni, int64_t nj, int64_t nt, int elem) {
-  return std::max(partial_bytes(make_plan((int)ni, (int)nj, (int)nt, elem, true), (int)ni, (int)nj),
-                  partial_bytes(make_plan((int)ni, (int)nj, (int)nt, elem, false), (int)ni, (int)nj));
+size_t product_bytes(int layouts, int64_t ni, int64_t nj, int64_t nt, int elem) {
+  size_t bytes = 0;
+  for (int direct = 0; direct < 2; ++direct) {
+    const Operands o{layouts, elem, direct != 0, ragged_rows(layouts, (int)ni, (int)nj, elem)};
+    bytes = std::max(bytes, partial_bytes(make_plan((int)ni, (int)nj, (int)nt, o), (int)ni, (int)nj));
+  }
+  return bytes;
 }
 
 int elem_size(int dtype) { return dtype == FWDMI_F32 ? 4 : 2; }
@@ -74,7 +110,7 @@ BackwardSpace backward_space(int64_t m, int64_t n, int64_t k, int act, int dtype
   if (act != FWDMI_ACT_NONE) s.dz = align256((size_t)m * n * elem);
   s.part = align256((size_t)slope_parts(m, n) * n * sizeof(float));
   if (k > 0)
-    s.product = std::max(product_bytes(m, k, n, elem), product_bytes(n, k, m, elem));
+    s.product = std::max(product_bytes(1, m, k, n, elem), product_bytes(2, n, k, m, elem));
   return s;
 }
 
@@ -86,7 +122,7 @@ extern "C" {
 size_t fwdmi_linear_workspace(int64_t m, int64_t n, int64_t k, int32_t dtype) {
   using namespace fwdmi;
   if (!is_train_dtype(dtype) || !dims_ok(m, n, k) || m == 0 || n == 0) return 0;
-  return product_bytes(m, n, k, elem_size(dtype));
+  return product_bytes(0, m, n, k, elem_size(dtype));
 }
 
 int fwdmi_linear(void* stream, int64_t m, int64_t n, int64_t k, const void* x, const void* w, const float* bias,

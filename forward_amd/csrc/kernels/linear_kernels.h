@@ -21,6 +21,7 @@
 
 #include <algorithm>
 #include <type_traits>
+#include <utility>
 
 #include "linear_plan.h"
 #include "slice.h"
@@ -89,31 +90,40 @@ __device__ __forceinline__ void with_act(int act, F&& f) {
   }
 }
 
-// y = act(z) + residual, z = acc + bias, of eight neighbours of one row (columns j .. j + 7, those below nj exist).
-template <typename T, int ACT>
-__device__ __forceinline__ void finish(const Product& P, int64_t i, int j, const float (&acc)[8]) {
-  const int64_t at = i * P.nj + j;
-  const int live = min(P.nj - j, 8);
-  Pack<T, 8> y, z, r{};
-  float b[8] = {};
-  if (live == 8) {
-    if (P.bias) {
-      const Pack<float, 4> lo = load_slice<float, 4>(gconst<float>(P.bias) + j);
-      const Pack<float, 4> hi = load_slice<float, 4>(gconst<float>(P.bias) + j + 4);
+__device__ __forceinline__ void load_bias(const Product& P, int j, float (&b)[8]) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        b[e] = lo.v[e];
-        b[e + 4] = hi.v[e];
-      }
+  for (int e = 0; e < 8; ++e) b[e] = 0.0f;
+  if (!P.bias) return;
+  if (j + 8 <= P.nj) {
+    const Pack<float, 4> lo = load_slice<float, 4>(gconst<float>(P.bias) + j);
+    const Pack<float, 4> hi = load_slice<float, 4>(gconst<float>(P.bias) + j + 4);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      b[e] = lo.v[e];
+      b[e + 4] = hi.v[e];
     }
-    if (P.residual) r = load_slice<T, 8>(gconst<T>(P.residual) + at);
   } else {
 #pragma unroll
     for (int e = 0; e < 8; ++e)
-      if (e < live) {
-        if (P.bias) b[e] = gconst<float>(P.bias)[j + e];
-        if (P.residual) r.v[e] = gconst<T>(P.residual)[at + e];
-      }
+      if (j + e < P.nj) b[e] = gconst<float>(P.bias)[j + e];
+  }
+}
+
+// y = act(z) + residual, z = acc + bias, of eight neighbours of one row: columns j .. j + 7, all of them (WHOLE) or
+// those below nj.
+template <typename T, int ACT, bool WHOLE>
+__device__ __forceinline__ void finish(const Product& P, int64_t i, int j, const float (&acc)[8], const float (&b)[8]) {
+  const int64_t at = i * P.nj + j;
+  const int live = WHOLE ? 8 : min(P.nj - j, 8);
+  Pack<T, 8> y, z, r{};
+  if (P.residual) {
+    if (live == 8) {
+      r = load_slice<T, 8>(gconst<T>(P.residual) + at);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (e < live) r.v[e] = gconst<T>(P.residual)[at + e];
+    }
   }
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
@@ -137,17 +147,18 @@ __device__ __forceinline__ void finish(const Product& P, int64_t i, int j, const
 // ---- tiles --------------------------------------------------------------------------------------------------------
 
 template <typename T>
-constexpr int kStep = kStepBytes / (int)sizeof(T);  // elements of t a step covers
-template <typename T>
 constexpr int kChunk = 16 / (int)sizeof(T);
 
-// Position of a tile's chunks: ROWS * 8 of them, in the order they lie in LDS.
-template <typename T, int ROWS, int LAYOUT>
+// Position of a tile's chunks in LDS: ROWS rows by STEP bytes of t.
+template <typename T, int ROWS, int LAYOUT, int STEP>
 struct Tile {
-  static constexpr int kBytes = ROWS * kStepBytes;
-  static constexpr int kLine = LAYOUT == kAlong ? kStepBytes : ROWS * (int)sizeof(T);  // bytes of an LDS line
-  static constexpr int kUnit = sizeof(T) == 2 ? 2 : 4;                                 // chunks of a kAcross unit
+  static constexpr int kBytes = ROWS * STEP;
+  static constexpr int kT = STEP / (int)sizeof(T);                            // elements of t
+  static constexpr int kLine = LAYOUT == kAlong ? STEP : ROWS * (int)sizeof(T);  // bytes of an LDS line
+  static constexpr int kUnit = sizeof(T) == 2 ? 2 : 4;                        // chunks of a kAcross unit
   static constexpr int kUnits = kLine / (16 * kUnit);
+  // what XOR permutes the chunks of row r by: eight neighbouring rows of one chunk fill 128 bytes
+  __device__ static __forceinline__ int along(int r) { return STEP >= 128 ? r & 7 : (r >> 1) & 3; }
   // what XOR permutes the units of line t by; fragments read 16 lines at a time: the bits that differ among them
   __device__ static __forceinline__ int across(int t) {
     const int f = sizeof(T) == 2 ? (t & 3) | ((t >> 1) & 4) : (t >> 2) & 3;
@@ -159,80 +170,108 @@ struct Tile {
     line = p / per;
     const int c = p % per;
     if (LAYOUT == kAlong)
-      chunk = c ^ (line & 7);
+      chunk = c ^ along(line);
     else
       chunk = ((c / kUnit) ^ across(line)) * kUnit + c % kUnit;
   }
 };
 
-// Loads of one operand's tile: ROWS rows from row `row0`, steps from `step0` on, by NT threads.
-template <typename T, int ROWS, int LAYOUT, int NT, bool DIRECT>
+// Loads of one operand's tile by NT threads: ROWS rows from row `row0` on, steps of t from `step0` on.
+// DIRECT: memory to LDS, whole steps only (`count` of them, then nothing); else through registers, two sets of them.
+template <typename T, int ROWS, int LAYOUT, int STEP, int NT, bool DIRECT>
 struct Loader {
-  using Tl = Tile<T, ROWS, LAYOUT>;
-  static constexpr int kLoads = ROWS * 8 / NT;
-  static_assert(ROWS * 8 % NT == 0, "whole loads");
-  const T FWDMI_GLOBAL* base;  // the tile's first element at step0
+  using Tl = Tile<T, ROWS, LAYOUT, STEP>;
+  static constexpr int kLoads = Tl::kBytes / 16 / NT;
+  static_assert(Tl::kBytes % (16 * NT) == 0, "whole loads");
+  const T FWDMI_GLOBAL* base;  // the tile's first element in the present step
   int64_t ld, step_elems;
-  int rows, t_left;  // rows of the tile that exist; elements of t from the present step on
+  int rows, left;  // rows of the tile that exist; DIRECT: whole steps left, else elements of t left
   int line[kLoads], chunk[kLoads];
-  uint32_t offset[kLoads];
-  Pack<T, kChunk<T>> held[DIRECT ? 1 : kLoads];
+  uint32_t offset[DIRECT ? kLoads : 1];
+  Pack<T, kChunk<T>> held[DIRECT ? 1 : 2][DIRECT ? 1 : kLoads];
 
-  __device__ __forceinline__ Loader(const void* p, int64_t ld_, int row0, int n_rows, int nt, int step0) {
+  __device__ __forceinline__ Loader(const void* p, int64_t ld_, int row0, int n_rows, int step0, int left_) {
     ld = ld_;
     rows = min(n_rows - row0, ROWS);
-    t_left = nt - step0 * kStep<T>;
-    const int64_t t0 = (int64_t)step0 * kStep<T>;
+    left = left_;
+    const int64_t t0 = (int64_t)step0 * Tl::kT;
     base = gconst<T>(p) + (LAYOUT == kAlong ? row0 * ld + t0 : t0 * ld + row0);
-    step_elems = LAYOUT == kAlong ? kStep<T> : kStep<T> * ld;
+    step_elems = LAYOUT == kAlong ? Tl::kT : Tl::kT * ld;
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
       Tl::locate(i * NT + (int)threadIdx.x, line[i], chunk[i]);
-      offset[i] = (uint32_t)(line[i] * (uint32_t)(ld * sizeof(T)) + chunk[i] * 16);
+      if (DIRECT) offset[i] = (uint32_t)(line[i] * (uint32_t)(ld * sizeof(T)) + chunk[i] * 16);
     }
   }
 
-  // DIRECT: issues the loads of the present step into `lds`; otherwise into registers (`drop` stores them).
+  // ---- DIRECT
   __device__ __forceinline__ void load(char* lds) {
-    if constexpr (DIRECT) {
-      // bytes from `base` to the end of what the tile may read; past it buffer loads give zeros
-      const uint32_t lines = LAYOUT == kAlong ? rows : min(t_left, kStep<T>);
-      const uint32_t last = LAYOUT == kAlong ? t_left : rows;
-      const uint32_t bytes = ((lines - 1) * (uint32_t)ld + last) * (uint32_t)sizeof(T);
-      const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, (int)bytes, 0x00020000);
-      const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    load_part<0, kLoads>(lds);
+    advance();
+  }
+  __device__ __forceinline__ void advance() {
+    base += step_elems;
+    --left;
+  }
+  template <int FIRST, int COUNT>
+  __device__ __forceinline__ void load_part(char* lds) {
+    // Bytes from `base` to the end of what the step may read; past it buffer loads give zeros and touch nothing.
+    // (kAcross: the last chunk of a line may reach into the next line, which exists: see `tail_of`.)
+    const uint32_t lines = LAYOUT == kAlong ? rows : Tl::kT;
+    const uint32_t last = LAYOUT == kAlong ? Tl::kT : (rows + kChunk<T> - 1) / kChunk<T> * kChunk<T>;
+    const uint32_t bytes = left > 0 ? ((lines - 1) * (uint32_t)ld + last) * (uint32_t)sizeof(T) : 0;
+    const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, (int)bytes, 0x00020000);
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+#pragma unroll
+    for (int i = FIRST; i < FIRST + COUNT; ++i)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (FWDMI_LDS void*)(lds + (i * NT + wave * 64) * 16), 16,
+                                               (int)offset[i], 0, 0, 0);
+  }
+
+  // ---- through registers
+  // Chunk i of a step that has `t_left` elements of t, element by element, zeros where nothing exists.
+  __device__ __forceinline__ Pack<T, kChunk<T>> some(int i, int t_left) const {
+    const int r = LAYOUT == kAlong ? line[i] : chunk[i] * kChunk<T>;
+    const int t = LAYOUT == kAlong ? chunk[i] * kChunk<T> : line[i];
+    const int n = r < rows && t < t_left ? (LAYOUT == kAlong ? t_left - t : rows - r) : 0;
+    const T FWDMI_GLOBAL* const at = base + (n > 0 ? (int64_t)line[i] * ld + chunk[i] * kChunk<T> : 0);
+    Pack<T, kChunk<T>> v;
+#pragma unroll
+    for (int e = 0; e < kChunk<T>; ++e) v.v[e] = e < n ? at[e] : (T)0.0f;
+    return v;
+  }
+  __device__ __forceinline__ void put(char* lds, int i, const Pack<T, kChunk<T>>& v) const {
+    *reinterpret_cast<Pack<T, kChunk<T>>*>(lds + (i * NT + (int)threadIdx.x) * 16) = v;
+  }
+  template <int SET>
+  __device__ __forceinline__ void fetch() {
+    // A step whose loads all lie inside the matrix takes them whole: rows past the tile's last repeat one (nobody
+    // reads their products), a line's last chunk may reach up to a chunk less one element into the lines behind it.
+    const bool whole = left >= Tl::kT && (LAYOUT == kAlong || rows % kChunk<T> == 0 ||
+                                          (int64_t)(left - Tl::kT) * ld >= kChunk<T> - 1);
+    if (whole) {
+      const int most = LAYOUT == kAlong ? rows - 1 : (rows + kChunk<T> - 1) / kChunk<T> - 1;
 #pragma unroll
       for (int i = 0; i < kLoads; ++i) {
-        uint32_t at = offset[i];
-        // a chunk of a row past the end of t would be the next row's beginning
-        if (LAYOUT == kAlong && chunk[i] * kChunk<T> >= t_left) at = 0x80000000u;
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (FWDMI_LDS void*)(lds + (i * NT + wave * 64) * 16), 16, (int)at, 0,
-                                                 0, 0);
+        const int l = LAYOUT == kAlong ? min(line[i], most) : line[i], c = LAYOUT == kAlong ? chunk[i] : min(chunk[i], most);
+        held[SET][i] = load_slice<T, kChunk<T>>(base + (int64_t)l * ld + c * kChunk<T>);
       }
-    } else {
+    } else if (left > 0) {
 #pragma unroll
-      for (int i = 0; i < kLoads; ++i) {
-        const int r = LAYOUT == kAlong ? line[i] : chunk[i] * kChunk<T>;
-        const int t = LAYOUT == kAlong ? chunk[i] * kChunk<T> : line[i];
-        const T FWDMI_GLOBAL* const at = base + (int64_t)line[i] * ld + chunk[i] * kChunk<T>;
-        const int n = r < rows && t < t_left ? (LAYOUT == kAlong ? t_left - t : rows - r) : 0;  // elements that exist
-        if (n >= kChunk<T>) {
-          held[i] = load_slice<T, kChunk<T>>(at);
-        } else {
-#pragma unroll
-          for (int e = 0; e < kChunk<T>; ++e) held[i].v[e] = e < n ? at[e] : (T)0.0f;
-        }
-      }
+      for (int i = 0; i < kLoads; ++i) held[SET][i] = some(i, left);
     }
     base += step_elems;
-    t_left -= kStep<T>;
+    left -= Tl::kT;
   }
-  __device__ __forceinline__ void drop(char* lds) {
-    if constexpr (!DIRECT) {
+  template <int SET>
+  __device__ __forceinline__ void drop(char* lds) const {
 #pragma unroll
-      for (int i = 0; i < kLoads; ++i)
-        *reinterpret_cast<Pack<T, kChunk<T>>*>(lds + (i * NT + (int)threadIdx.x) * 16) = held[i];
-    }
+    for (int i = 0; i < kLoads; ++i) put(lds, i, held[SET][i]);
+  }
+  // The last, partial step of DIRECT loads.
+  __device__ __forceinline__ void tail(char* lds, int t_left) const {
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) put(lds, i, some(i, t_left));
   }
 };
 
@@ -243,17 +282,17 @@ struct Frag {
 };
 
 // Reads the fragments of FR blocks of 16 rows from `row0` (a multiple of 16) on.
-template <typename T, int ROWS, int LAYOUT, int FR>
+template <typename T, int ROWS, int LAYOUT, int STEP, int FR>
 struct Reader {
-  using Tl = Tile<T, ROWS, LAYOUT>;
+  using Tl = Tile<T, ROWS, LAYOUT, STEP>;
   int at[LAYOUT == kAlong ? 1 : FR];
   int half;
   __device__ __forceinline__ explicit Reader(int row0) {
     const int lane = threadIdx.x & 63, g = lane >> 4, j = lane & 15;
     half = 0;
     if constexpr (LAYOUT == kAlong) {
-      at[0] = (row0 + j) * kStepBytes + ((g ^ (j & 7)) << 4);  // (row & 7 == j & 7); the second half flips bit 2
-      half = ((g ^ (j & 7)) & 4) ? -64 : 64;
+      at[0] = (row0 + j) * STEP + ((g ^ Tl::along(j)) << 4);  // (row0 is a multiple of 16)
+      half = (g ^ Tl::along(j)) & 4;  // a half of 64 bytes more flips bit 2 of the chunk and carries into bit 3
     } else if constexpr (sizeof(T) == 2) {
       const int t = g * 8 + (j >> 2);
 #pragma unroll
@@ -263,14 +302,16 @@ struct Reader {
       for (int f = 0; f < FR; ++f) at[f] = g * 4 * Tl::kLine + ((row0 / 16 + f) ^ Tl::across(g * 4)) * 64 + j * 4;
     }
   }
-  // half h (of 64 bytes of t) of the step
-  __device__ __forceinline__ void read(const char* lds, int h, Frag<T> (&out)[FR]) const {
+  // blocks FIRST .. FIRST + COUNT - 1 of half h (64 bytes of t) of the step
+  template <int FIRST = 0, int COUNT = FR>
+  __device__ __forceinline__ void read(const char* lds, int h, Frag<T> (&out)[COUNT]) const {
 #pragma unroll
-    for (int f = 0; f < FR; ++f) {
+    for (int f = 0; f < COUNT; ++f) {
       if constexpr (LAYOUT == kAlong) {
-        out[f].v = *reinterpret_cast<const Pack<T, kChunk<T>>*>(lds + at[0] + h * half + f * 16 * kStepBytes);
+        out[f].v = *reinterpret_cast<const Pack<T, kChunk<T>>*>(lds + at[0] + (h & 1 ? 64 - 32 * half : 0) + (h >> 1) * 128 +
+                                                                    (FIRST + f) * 16 * STEP);
       } else if constexpr (sizeof(T) == 2) {
-        const char* const p = lds + at[f] + h * 32 * Tl::kLine;
+        const char* const p = lds + at[FIRST + f] + h * 32 * Tl::kLine;
         const S4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((FWDMI_LDS S4*)(p));
         const S4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((FWDMI_LDS S4*)(p + 4 * Tl::kLine));
         __builtin_memcpy(&out[f].v.v[0], &lo, 8);
@@ -278,7 +319,7 @@ struct Reader {
       } else {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          out[f].v.v[e] = *reinterpret_cast<const T*>(lds + at[f] + (h * 16 + e) * Tl::kLine);
+          out[f].v.v[e] = *reinterpret_cast<const T*>(lds + at[FIRST + f] + (h * 16 + e) * Tl::kLine);
       }
     }
   }
@@ -307,71 +348,52 @@ __device__ __forceinline__ F4 multiply(const Frag<T>& b, const Frag<T>& a, F4 ac
   }
 }
 
-template <typename T, int LA, int LB, int TI, int TJ, int WI, int WJ, bool DIRECT>
-__global__ __launch_bounds__(64 * WI * WJ) void product_kernel(const Product P) {
-  constexpr int kNT = 64 * WI * WJ;
-  constexpr int kFI = TI / WI / 16, kFJ = TJ / WJ / 16;
-  using TileA = Tile<T, TI, LA>;
-  using TileB = Tile<T, TJ, LB>;
-  constexpr int kBuffer = TileA::kBytes + TileB::kBytes;  // one step of both operands
-  __shared__ __attribute__((aligned(1024))) char s_tile[2 * kBuffer];
-  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+// The steps of t that this workgroup's split walks: whole ones from `first` on, and `tail` elements of a last one.
+struct Steps {
+  int first, whole, tail;
+};
+__device__ __forceinline__ Steps split_steps(const Product& P) {
+  const int first = (int)blockIdx.y * P.steps_per_split, end = first + P.steps_per_split;
+  const int whole = max(min(end, P.whole_steps) - first, 0);
+  return Steps{first, whole, first <= P.whole_steps && end > P.whole_steps ? P.tail : 0};
+}
+
+// The immediate of s_waitcnt that waits until at most n vector memory operations are in flight (and for nothing else).
+constexpr int wait_loads(int n) { return (n & 15) | (n >> 4) << 14 | 0x0f70; }
+
+// The tile of this workgroup.  Workgroups go to the XCDs in turn, so the numbers are dealt out in eight runs of
+// neighbours, one per XCD, and a run walks columns of at most eight tiles: the tiles an XCD works on at a time share
+// their lines of A and B in its L2.
+template <int TI, int TJ>
+__device__ __forceinline__ void locate_tile(const Product& P, int& i0, int& j0) {
+  const int total = P.tiles_i * P.tiles_j, b = (int)blockIdx.x;
+  const int xcd = b & 7, per = total >> 3, more = total & 7;
+  const int n = xcd * per + min(xcd, more) + (b >> 3);
+  constexpr int kGroup = 8;
+  const int group = n / (kGroup * P.tiles_j), first = group * kGroup;
+  const int height = min(P.tiles_i - first, kGroup), in = n - group * kGroup * P.tiles_j;
+  i0 = (first + in % height) * TI;
+  j0 = in / height * TJ;
+}
+
+// The tile leaves through LDS, as much of it at a time as the buffers hold, so that every row is read back and stored
+// in whole 16-byte slices by neighbouring lanes.  16-byte chunk c of row r lies at c ^ (r & 15).
+template <typename T, int TI, int TJ, int WI, int WJ, int WK, int ROOM, bool EPILOGUE, int FI, int FJ>
+__device__ __forceinline__ void leave_tile(const Product& P, const F4 (&acc)[FJ][FI], char* s_tile, int i0, int j0) {
+  constexpr int kNT = 64 * WI * WJ * WK;
+  constexpr int kAllBytes = TI * TJ * 4 * WK;
+  constexpr int kPhases = kAllBytes <= ROOM ? 1 : kAllBytes <= 2 * ROOM ? 2 : 4;
+  static_assert(kAllBytes / kPhases <= ROOM && FI % kPhases == 0, "a part of the tile fits the buffers");
   const int lane = threadIdx.x & 63;
-  const int ti = (int)(blockIdx.x % P.tiles_i), tj = (int)(blockIdx.x / P.tiles_i);
-  const int i0 = ti * TI, j0 = tj * TJ;
-  const int wi = wave % WI * (TI / WI), wj = wave / WI * (TJ / WJ);
-
-  const int all = (P.nt + kStep<T> - 1) / kStep<T>;
-  const int step0 = (int)blockIdx.y * P.steps_per_split;
-  const int steps = min(all - step0, P.steps_per_split);
-
-  F4 acc[kFJ][kFI];
-#pragma unroll
-  for (int j = 0; j < kFJ; ++j)
-#pragma unroll
-    for (int i = 0; i < kFI; ++i) acc[j][i] = F4{0.0f, 0.0f, 0.0f, 0.0f};
-
-  if (steps > 0) {
-    Loader<T, TI, LA, kNT, DIRECT> la(P.a, P.lda, i0, P.ni, P.nt, step0);
-    Loader<T, TJ, LB, kNT, DIRECT> lb(P.b, P.ldb, j0, P.nj, P.nt, step0);
-    const Reader<T, TI, LA, kFI> ra(wi);
-    const Reader<T, TJ, LB, kFJ> rb(wj);
-    la.load(s_tile);
-    lb.load(s_tile + TileA::kBytes);
-    la.drop(s_tile);
-    lb.drop(s_tile + TileA::kBytes);
-    for (int s = 0; s < steps; ++s) {
-      char* const now = s_tile + (s & 1) * kBuffer;
-      char* const next = s_tile + (~s & 1) * kBuffer;
-      __syncthreads();  // this step's tiles are in LDS, and the other buffers have been read
-      if (s + 1 < steps) {
-        la.load(next);
-        lb.load(next + TileA::kBytes);
-      }
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        Frag<T> fa[kFI], fb[kFJ];
-        ra.read(now, h, fa);
-        rb.read(now + TileA::kBytes, h, fb);
-#pragma unroll
-        for (int j = 0; j < kFJ; ++j)
-#pragma unroll
-          for (int i = 0; i < kFI; ++i) acc[j][i] = multiply<T>(fb[j], fa[i], acc[j][i]);
-      }
-      if (s + 1 < steps) {
-        la.drop(next);
-        lb.drop(next + TileA::kBytes);
-      }
-    }
-  }
-
-  // The tile leaves through LDS, as much of it at a time as the buffers hold, so that every row is read back and
-  // stored in whole 16-byte slices by neighbouring lanes.  16-byte chunk c of row r lies at c ^ (r & 15).
-  constexpr int kPhases = std::max(1, TI * TJ * 4 / (2 * kBuffer));
-  constexpr int kFP = kFI / kPhases;                // fragments of i a wave leaves per phase
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int wj = wave / WI % WJ * (TJ / WJ);
+  constexpr int kFP = FI / kPhases;                // fragments of i a wave leaves per phase
   constexpr int kRowsPhase = TI / kPhases;          // rows of all waves per phase
   constexpr int kRowsWave = kRowsPhase / WI;
+  constexpr int kMix = (TJ / 4 < 16 ? TJ / 4 : 16) - 1;
+  constexpr int kSlab = kRowsPhase * TJ;            // elements of a wave group's part of the sum over t
   float* const s_out = reinterpret_cast<float*>(s_tile);
+  float* const s_mine = s_out + wave / (WI * WJ) * kSlab;
   const int r_lane = wave % WI * kRowsWave + (lane & 15);
   for (int phase = 0; phase < kPhases; ++phase) {
     __syncthreads();
@@ -381,9 +403,9 @@ __global__ __launch_bounds__(64 * WI * WJ) void product_kernel(const Product P) 
 #pragma unroll
         for (int i = 0; i < kFP; ++i)
 #pragma unroll
-          for (int j = 0; j < kFJ; ++j) {
-            const int chunk = ((wj + j * 16) / 4 + (lane >> 4)) ^ (lane & 15);
-            *reinterpret_cast<F4*>(s_out + (r_lane + i * 16) * TJ + chunk * 4) = acc[j][p * kFP + i];
+          for (int j = 0; j < FJ; ++j) {
+            const int chunk = ((wj + j * 16) / 4 + (lane >> 4)) ^ (lane & kMix);
+            *reinterpret_cast<F4*>(s_mine + (r_lane + i * 16) * TJ + chunk * 4) = acc[j][p * kFP + i];
           }
       }
     __syncthreads();
@@ -393,8 +415,12 @@ __global__ __launch_bounds__(64 * WI * WJ) void product_kernel(const Product P) 
         const int row = q / (TJ / 8), c = q % (TJ / 8);
         const int i = i0 + row / kRowsWave * (TI / WI) + phase * kRowsWave + row % kRowsWave, j = j0 + c * 8;
         if (i >= P.ni || j >= P.nj) continue;
-        const F4 lo = *reinterpret_cast<const F4*>(s_out + row * TJ + ((2 * c) ^ (row & 15)) * 4);
-        const F4 hi = *reinterpret_cast<const F4*>(s_out + row * TJ + ((2 * c + 1) ^ (row & 15)) * 4);
+        F4 lo{0.0f, 0.0f, 0.0f, 0.0f}, hi = lo;
+#pragma unroll
+        for (int k = 0; k < WK; ++k) {
+          lo += *reinterpret_cast<const F4*>(s_out + k * kSlab + row * TJ + ((2 * c) ^ (row & kMix)) * 4);
+          hi += *reinterpret_cast<const F4*>(s_out + k * kSlab + row * TJ + ((2 * c + 1) ^ (row & kMix)) * 4);
+        }
         const float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
         f((int64_t)i, j, v);
       }
@@ -412,14 +438,285 @@ __global__ __launch_bounds__(64 * WI * WJ) void product_kernel(const Product P) 
             if (j + e < P.nj) p[e] = v[e];
         }
       });
-    } else if constexpr (LA == kAlong && LB == kAlong) {
+    } else if constexpr (EPILOGUE) {
       with_act(P.act, [&](auto act) {
-        leave([&](int64_t i, int j, const float (&v)[8]) { finish<T, decltype(act)::value>(P, i, j, v); });
+        leave([&](int64_t i, int j, const float (&v)[8]) {
+          float b[8];
+          load_bias(P, j, b);
+          finish<T, decltype(act)::value, false>(P, i, j, v, b);
+        });
       });
     } else {  // the gradient's products have no epilogue
-      leave([&](int64_t i, int j, const float (&v)[8]) { finish<T, FWDMI_ACT_NONE>(P, i, j, v); });
+      leave([&](int64_t i, int j, const float (&v)[8]) {
+        const float b[8] = {};
+        finish<T, FWDMI_ACT_NONE, false>(P, i, j, v, b);
+      });
     }
   }
+}
+
+// A tile whose columns all exist leaves straight from the accumulators.  A lane holds four neighbouring columns of
+// blocks 2 p and 2 p + 1; exchanges between the lane rows (16 lanes each) give it eight neighbouring columns of one
+// block, so that a store instruction writes 64 contiguous bytes of each of its 16 rows: no LDS, no barrier, and the two
+// waves of a SIMD overlap each other's arithmetic and stores.
+template <typename T, int TI, int TJ, int WI, int WJ, bool EPILOGUE, int FI, int FJ>
+__device__ __forceinline__ void leave_registers(const Product& P, const F4 (&acc)[FJ][FI], int i0, int j0) {
+  const int lane = threadIdx.x & 63, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int i_lane = i0 + wave % WI * (TI / WI) + (lane & 15);
+  const int j_lane = j0 + wave / WI * (TJ / WJ) + (g & 1) * 8 + (g >> 1) * 16;
+  if (P.partial) {  // four fp32 neighbours are 16 bytes as they lie
+    float FWDMI_GLOBAL* const out = gmut<float>(P.partial) + (int64_t)blockIdx.y * P.ni * P.nj;
+    const int j4 = j0 + wave / WI * (TJ / WJ) + g * 4;
+#pragma unroll
+    for (int i = 0; i < FI; ++i)
+      if (i_lane + i * 16 < P.ni)
+#pragma unroll
+        for (int j = 0; j < FJ; ++j) {
+          Pack<float, 4> v;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v.v[e] = acc[j][i][e];
+          store_slice<float, 4>(out + (int64_t)(i_lane + i * 16) * P.nj + j4 + j * 16, v);
+        }
+    return;
+  }
+  auto eight = [&](int p, int i, float (&v)[8]) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      // lane rows of the two blocks: 0 1 2 3 and 4 5 6 7 -> 0 1 4 5 and 2 3 6 7 -> 0 2 4 6 and 1 3 5 7
+      auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(acc[2 * p][i][e]), __float_as_uint(acc[2 * p + 1][i][e]),
+                                                false, false);
+      auto b = __builtin_amdgcn_permlane16_swap(a[0], a[1], false, false);
+      v[e] = __uint_as_float(b[0]);
+      v[e + 4] = __uint_as_float(b[1]);
+    }
+  };
+  with_act(EPILOGUE ? P.act : FWDMI_ACT_NONE, [&](auto act) {
+    if (!EPILOGUE && decltype(act)::value != FWDMI_ACT_NONE) return;
+#pragma unroll
+    for (int p = 0; p < FJ / 2; ++p) {
+      const int j = j_lane + p * 32;
+      float b[8] = {};
+      if (EPILOGUE) load_bias(P, j, b);
+#pragma unroll
+      for (int i = 0; i < FI; ++i) {
+        float v[8];
+        eight(p, i, v);
+        if (i_lane + i * 16 < P.ni) finish<T, decltype(act)::value, true>(P, i_lane + i * 16, j, v, b);
+      }
+    }
+  });
+}
+
+template <typename T, int LA, int LB, int TI, int TJ, int WI, int WJ, int WK, int STEP, int STAGES, bool DIRECT>
+__global__ __launch_bounds__(64 * WI * WJ * WK) void product_kernel(const Product P) {
+  constexpr int kNT = 64 * WI * WJ * WK;
+  constexpr int kFI = TI / WI / 16, kFJ = TJ / WJ / 16, kHalves = STEP / 64 / WK;
+  using TileA = Tile<T, TI, LA, STEP>;
+  using TileB = Tile<T, TJ, LB, STEP>;
+  using LoadA = Loader<T, TI, LA, STEP, kNT, DIRECT>;
+  using LoadB = Loader<T, TJ, LB, STEP, kNT, DIRECT>;
+  static_assert(DIRECT || STAGES == 2, "registers hold one step");
+  constexpr int kBuffer = TileA::kBytes + TileB::kBytes;  // one step of both operands
+  __shared__ __attribute__((aligned(1024))) char s_tile[STAGES * kBuffer];
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  int i0, j0;
+  locate_tile<TI, TJ>(P, i0, j0);
+  const int wi = wave % WI * (TI / WI), wj = wave / WI % WJ * (TJ / WJ), wk = wave / (WI * WJ);
+
+  const Steps steps = split_steps(P);
+
+  F4 acc[kFJ][kFI];
+#pragma unroll
+  for (int j = 0; j < kFJ; ++j)
+#pragma unroll
+    for (int i = 0; i < kFI; ++i) acc[j][i] = F4{0.0f, 0.0f, 0.0f, 0.0f};
+
+  const Reader<T, TI, LA, STEP, kFI> ra(wi);
+  const Reader<T, TJ, LB, STEP, kFJ> rb(wj);
+  auto multiply_step = [&](const char* now) {
+#pragma unroll
+    for (int h = 0; h < kHalves; ++h) {
+      Frag<T> fa[kFI], fb[kFJ];
+      ra.read(now, wk * kHalves + h, fa);
+      rb.read(now + TileA::kBytes, wk * kHalves + h, fb);
+#pragma unroll
+      for (int j = 0; j < kFJ; ++j)
+#pragma unroll
+        for (int i = 0; i < kFI; ++i) acc[j][i] = multiply<T>(fb[j], fa[i], acc[j][i]);
+    }
+  };
+  if constexpr (DIRECT) {
+    LoadA la(P.a, P.lda, i0, P.ni, steps.first, steps.whole);
+    LoadB lb(P.b, P.ldb, j0, P.nj, steps.first, steps.whole);
+    // STAGES - 1 steps of loads are in flight; steps past the end load nothing (every lane out of range) so that the
+    // number in flight is always the same
+    constexpr int kAhead = (STAGES - 2) * (LoadA::kLoads + LoadB::kLoads);
+    static_assert(kAhead < 64, "what the counter of loads in flight holds");
+#pragma unroll
+    for (int k = 0; k < STAGES - 1; ++k) {
+      la.load(s_tile + k * kBuffer);
+      lb.load(s_tile + k * kBuffer + TileA::kBytes);
+    }
+    int now = 0, next = (STAGES - 1) * kBuffer;
+    for (int s = 0; s < steps.whole; ++s) {
+      __builtin_amdgcn_sched_barrier(0);
+      __builtin_amdgcn_s_waitcnt(wait_loads(kAhead));  // this step's are in
+      __builtin_amdgcn_s_barrier();                    // ... of every wave, and the buffer of the step before has been read
+      __builtin_amdgcn_sched_barrier(0);
+      la.load(s_tile + next);
+      lb.load(s_tile + next + TileA::kBytes);
+      multiply_step(s_tile + now);
+      now = now + kBuffer == STAGES * kBuffer ? 0 : now + kBuffer;
+      next = next + kBuffer == STAGES * kBuffer ? 0 : next + kBuffer;
+    }
+    __builtin_amdgcn_s_waitcnt(wait_loads(0));  // loads past the end write zeros: before the buffers are used again
+    if (steps.tail > 0) {
+      // (`base` has run ahead of the tail by the steps in flight)
+      __syncthreads();
+      la.base -= (STAGES - 1) * la.step_elems;
+      lb.base -= (STAGES - 1) * lb.step_elems;
+      la.tail(s_tile, steps.tail);
+      lb.tail(s_tile + TileA::kBytes, steps.tail);
+      __syncthreads();
+      multiply_step(s_tile);
+    }
+  } else if (const int n = steps.whole + (steps.tail > 0 ? 1 : 0); n > 0) {
+    const int t = steps.whole * TileA::kT + steps.tail;
+    LoadA la(P.a, P.lda, i0, P.ni, steps.first, t);
+    LoadB lb(P.b, P.ldb, j0, P.nj, steps.first, t);
+    // registers hold the two steps after the one being multiplied
+    la.template fetch<0>();
+    lb.template fetch<0>();
+    la.template drop<0>(s_tile);
+    lb.template drop<0>(s_tile + TileA::kBytes);
+    la.template fetch<1>();
+    lb.template fetch<1>();
+    auto step = [&](auto set, int s) {
+      constexpr int kSet = decltype(set)::value;  // s & 1
+      char* const next = s_tile + (kSet ^ 1) * kBuffer;
+      __syncthreads();  // this step's tiles are in LDS, and the other buffers have been read
+      la.template fetch<kSet>();
+      lb.template fetch<kSet>();
+      multiply_step(s_tile + kSet * kBuffer);
+      if (s + 1 < n) {
+        la.template drop<kSet ^ 1>(next);
+        lb.template drop<kSet ^ 1>(next + TileA::kBytes);
+      }
+    };
+    for (int s = 0; s < n; s += 2) {
+      step(std::integral_constant<int, 0>{}, s);
+      if (s + 1 < n) step(std::integral_constant<int, 1>{}, s + 1);
+    }
+  }
+  leave_tile<T, TI, TJ, WI, WJ, WK, STAGES * kBuffer, LA == kAlong && LB == kAlong>(P, acc, s_tile, i0, j0);
+}
+
+template <int... I, typename F>
+__device__ __forceinline__ void unrolled(std::integer_sequence<int, I...>, F&& f) {
+  (f(std::integral_constant<int, I>{}), ...);
+}
+
+// Large products of 16-bit operands: eight waves, two on every SIMD of the CU, take turns.  While one multiplies (16
+// matrix instructions, 256 cycles of its SIMD), the other reads the fragments of its next 16 from LDS, and both change
+// over at a barrier.  Waves 4 .. 7 run half a phase behind 0 .. 3, by one barrier more in front and one fewer behind.
+//
+// A step of 64 t has a phase for each half of t and each 64 rows of the wave.  With two buffers (256 x 256 tiles, 128 KB)
+// the next step's loads go into the buffer of the step before this one: they start in phase 1, when the late waves
+// have read that buffer's last fragments (those reads are waited for in front of the multiplications they feed), and every
+// wave waits for its own in the last phase, in front of the barrier behind which the first waves read them.  With
+// three buffers (256 x 128, 144 KB) the loads of the step after next go out in phase 1 and have a whole step more.
+template <typename T, int LA, int LB, int TI, int TJ, int WI, int WJ, int STAGES>
+__global__ __launch_bounds__(512) void product_turns_kernel(const Product P) {
+  constexpr int kNT = 512, STEP = 128;
+  constexpr int kFI = TI / WI / 16, kFJ = TJ / WJ / 16, kQ = kFI / 4, kPhases = 2 * kQ;
+  static_assert(WI * WJ == 8 && kFI % 4 == 0 && kFJ == 4 && (STAGES == 3 || kPhases == 4), "shape of the phases");
+  using TileA = Tile<T, TI, LA, STEP>;
+  using TileB = Tile<T, TJ, LB, STEP>;
+  using LoadA = Loader<T, TI, LA, STEP, kNT, true>;
+  using LoadB = Loader<T, TJ, LB, STEP, kNT, true>;
+  constexpr int kBuffer = TileA::kBytes + TileB::kBytes;
+  constexpr int kAhead = (STAGES - 2) * (LoadA::kLoads + LoadB::kLoads);  // loads that stay in flight over a step's end
+  __shared__ __attribute__((aligned(1024))) char s_tile[STAGES * kBuffer];
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  int i0, j0;
+  locate_tile<TI, TJ>(P, i0, j0);
+  const int wi = wave % WI * (TI / WI), wj = wave / WI * (TJ / WJ);
+  const Steps steps = split_steps(P);
+
+  F4 acc[kFJ][kFI];
+#pragma unroll
+  for (int j = 0; j < kFJ; ++j)
+#pragma unroll
+    for (int i = 0; i < kFI; ++i) acc[j][i] = F4{0.0f, 0.0f, 0.0f, 0.0f};
+
+  LoadA la(P.a, P.lda, i0, P.ni, steps.first, steps.whole);
+  LoadB lb(P.b, P.ldb, j0, P.nj, steps.first, steps.whole);
+  const Reader<T, TI, LA, STEP, kFI> ra(wi);
+  const Reader<T, TJ, LB, STEP, kFJ> rb(wj);
+  // (steps past the end load nothing, every lane out of range, so that the number in flight is always the same)
+#pragma unroll
+  for (int k = 0; k < STAGES - 1; ++k) {
+    la.load(s_tile + k * kBuffer);
+    lb.load(s_tile + k * kBuffer + TileA::kBytes);
+  }
+  __builtin_amdgcn_s_waitcnt(wait_loads(kAhead));
+  __builtin_amdgcn_s_barrier();
+  if (wave >= 4) __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_sched_barrier(0);
+  Frag<T> fa[4], fb[kFJ];
+  auto change = [&] {
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  auto multiply_block = [&](auto first) {
+    constexpr int kFirst = decltype(first)::value;
+#pragma unroll
+    for (int j = 0; j < kFJ; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[j][kFirst + i] = multiply<T>(fb[j], fa[i], acc[j][kFirst + i]);
+  };
+  int now_at = 0, next_at = (STAGES - 1) * kBuffer;
+  for (int s = 0; s < steps.whole; ++s) {
+    const char* const now = s_tile + now_at;
+    char* const next = s_tile + next_at;
+    unrolled(std::make_integer_sequence<int, kPhases>{}, [&](auto phase) {
+      constexpr int ph = decltype(phase)::value, h = ph / kQ, q = ph % kQ;
+      if constexpr (q == 0) rb.read(now + TileA::kBytes, h, fb);
+      ra.template read<q * 4, 4>(now, h, fa);
+      if constexpr (ph == 1) la.load(next);
+      if constexpr (ph == (STAGES == 2 ? 2 : 1)) lb.load(next + TileA::kBytes);
+      if constexpr (ph == kPhases - 1) __builtin_amdgcn_s_waitcnt(wait_loads(kAhead));
+      change();
+      __builtin_amdgcn_s_setprio(1);
+      multiply_block(std::integral_constant<int, q * 4>{});
+      __builtin_amdgcn_s_setprio(0);
+      change();
+    });
+    now_at = now_at + kBuffer == STAGES * kBuffer ? 0 : now_at + kBuffer;
+    next_at = next_at + kBuffer == STAGES * kBuffer ? 0 : next_at + kBuffer;
+  }
+  if (wave < 4) __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_s_waitcnt(wait_loads(0));  // loads past the end write zeros: before the buffers are used again
+  if (steps.tail > 0) {
+    __syncthreads();
+    la.base -= (STAGES - 1) * la.step_elems;
+    lb.base -= (STAGES - 1) * lb.step_elems;
+    la.tail(s_tile, steps.tail);
+    lb.tail(s_tile + TileA::kBytes, steps.tail);
+    __syncthreads();
+    unrolled(std::make_integer_sequence<int, kPhases>{}, [&](auto phase) {
+      constexpr int ph = decltype(phase)::value, h = ph / kQ, q = ph % kQ;
+      if constexpr (q == 0) rb.read(s_tile + TileA::kBytes, h, fb);
+      ra.template read<q * 4, 4>(s_tile, h, fa);
+      multiply_block(std::integral_constant<int, q * 4>{});
+    });
+  }
+  if (j0 + TJ <= P.nj)
+    leave_registers<T, TI, TJ, WI, WJ, LA == kAlong && LB == kAlong>(P, acc, i0, j0);
+  else
+    leave_tile<T, TI, TJ, WI, WJ, 1, STAGES * kBuffer, LA == kAlong && LB == kAlong>(P, acc, s_tile, i0, j0);
 }
 
 // Adds the splits' partial products in split order and finishes them; eight neighbours of a row per lane.
@@ -448,7 +745,9 @@ __global__ __launch_bounds__(256) void finish_kernel(const Product P, int splits
         if (e < live) acc[e] += p[e];
     }
   }
-  with_act(P.act, [&](auto act) { finish<T, decltype(act)::value>(P, i, j, acc); });
+  float b[8];
+  load_bias(P, j, b);
+  with_act(P.act, [&](auto act) { finish<T, decltype(act)::value, false>(P, i, j, acc, b); });
 }
 
 // ---- dz = dy * act'(z) and its column sums -----------------------------------------------------------------------
@@ -509,15 +808,26 @@ __global__ __launch_bounds__(256) void slope_kernel(const Slope S) {
 
 template <typename T, int LA, int LB, bool DIRECT>
 int launch_product(Product& P, const Plan& plan, hipStream_t stream) {
-  P.tiles_i = ceil_div(P.ni, plan.ti);
-  P.tiles_j = ceil_div(P.nj, plan.tj);
+  const TileShape tile = kTiles[plan.tile];
+  P.tiles_i = ceil_div(P.ni, tile.ti);
+  P.tiles_j = ceil_div(P.nj, tile.tj);
+  P.whole_steps = plan.whole_steps;
+  P.tail = plan.tail;
   P.steps_per_split = plan.steps_per_split;
   const dim3 grid((unsigned)(P.tiles_i * P.tiles_j), (unsigned)plan.splits);
   if constexpr (sizeof(T) == 2 && DIRECT) {
-    if (plan.tile == kBig) hipLaunchKernelGGL((product_kernel<T, LA, LB, 256, 256, 2, 4, true>), grid, dim3(512), 0, stream, P);
+    if (plan.tile == k256x256)
+      hipLaunchKernelGGL((product_turns_kernel<T, LA, LB, 256, 256, 2, 4, 2>), grid, dim3(512), 0, stream, P);
+    if (plan.tile == k256x128)
+      hipLaunchKernelGGL((product_turns_kernel<T, LA, LB, 256, 128, 4, 2, 3>), grid, dim3(512), 0, stream, P);
   }
-  if (plan.tile == kMid) hipLaunchKernelGGL((product_kernel<T, LA, LB, 128, 128, 2, 2, DIRECT>), grid, dim3(256), 0, stream, P);
-  if (plan.tile == kSmall) hipLaunchKernelGGL((product_kernel<T, LA, LB, 64, 64, 2, 2, DIRECT>), grid, dim3(256), 0, stream, P);
+  if (plan.tile == k128x128)
+    hipLaunchKernelGGL((product_kernel<T, LA, LB, 128, 128, 2, 2, 1, 128, 2, DIRECT>), grid, dim3(256), 0, stream, P);
+  if (plan.tile == k64x64)
+    hipLaunchKernelGGL((product_kernel<T, LA, LB, 64, 64, 2, 1, 4, 256, 2, DIRECT>), grid, dim3(512), 0, stream, P);
+  if (plan.tile == k64x32)
+    hipLaunchKernelGGL((product_kernel<T, LA, LB, 64, 32, 2, 1, 4, 256, DIRECT ? 4 : 2, DIRECT>), grid, dim3(512), 0, stream,
+                       P);
   FWDMI_HIP_CHECK(hipGetLastError());
   if (plan.splits > 1) {
     const int64_t octets = (int64_t)P.ni * ((P.nj + 7) / 8);

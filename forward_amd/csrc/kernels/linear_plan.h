@@ -18,7 +18,8 @@ struct Product {
   const void* b;
   int64_t lda, ldb;
   int32_t ni, nj, nt;
-  int32_t steps_per_split;  // steps of 128 bytes that one of gridDim.y splits walks
+  int32_t whole_steps, tail;  // t as steps of a tile's depth and the elements that are left (`tail_of`)
+  int32_t steps_per_split;    // of whole_steps (+ 1 for the tail) that one of gridDim.y splits walks
   float* partial;           // not null: C goes there unfinished, [split][ni][nj]
   void* c;                  // [ni, nj]
   void* preact;             // nullable
@@ -39,22 +40,35 @@ struct Slope {
   int32_t act;
 };
 
-constexpr int kStepBytes = 128;  // of t that a step covers
+// The tiles there are.  The first two are the eight-wave kernel of 16-bit operands (product_turns_kernel).
+enum TileKind { k256x256, k256x128, k128x128, k64x64, k64x32, kTileKinds };
+struct TileShape {
+  int ti, tj, step_bytes;
+};
+constexpr TileShape kTiles[kTileKinds] = {{256, 256, 128}, {256, 128, 128}, {128, 128, 128}, {64, 64, 256}, {64, 32, 256}};
 
-enum TileKind { kBig = 0, kMid = 1, kSmall = 2 };
 struct Plan {
   TileKind tile;
-  int ti, tj;
-  int splits, steps_per_split;
+  int splits, whole_steps, tail, steps_per_split;
 };
 
 inline int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
-// Lines that are whole 16-byte chunks from a 16-byte boundary on, within a buffer load's 31-bit offsets.
-inline bool direct_ok(const void* p, int64_t ld, int elem, int extent_along) {
-  const int chunk = 16 / elem;
-  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % chunk == 0 && extent_along % chunk == 0 &&
-         ld * elem <= (int64_t)1 << 22;
+// Operands that go from memory straight to LDS: 16-byte loads need 4-byte aligned lines, offsets are 31 bits.
+inline bool direct_ok(const void* p, int64_t ld, int elem) {
+  return reinterpret_cast<uintptr_t>(p) % 4 == 0 && ld * elem % 4 == 0 && ld >= 8 && ld * elem <= (int64_t)1 << 22;
+}
+
+// t as whole steps of `depth` elements and a tail that is loaded element by element.  Direct loads of lines across t
+// take whole chunks, of which a line's last may reach into the next line: where rows do not fill their chunks (`ragged`)
+// the matrix's last line has to be in the tail, so that a line is behind every one that is loaded whole.
+inline void tail_of(int nt, int depth, bool ragged, int& whole, int& tail) {
+  whole = nt / depth;
+  tail = nt % depth;
+  if (ragged && tail == 0 && whole > 0) {
+    --whole;
+    tail = depth;
+  }
 }
 
 // Run P as planned (with the finishing launch where t is split) / dz and its column sums, in elements of one type.

@@ -4,6 +4,8 @@
 
 #include <hip/hip_runtime.h>
 
+#include <atomic>
+
 #include "../common.h"
 #include "device_util.h"
 
@@ -68,11 +70,18 @@ inline int launch_column_sums(const ColumnSums& S, hipStream_t stream) {
   return FWDMI_OK;
 }
 
+// Compute units of the current device (asked once per device).
 inline int device_cus() {
+  static std::atomic<int> known[64];
   int dev = 0, v = 0;
-  if (hipGetDevice(&dev) == hipSuccess &&
-      hipDeviceGetAttribute(&v, hipDeviceAttributeMultiprocessorCount, dev) == hipSuccess && v > 0)
-    return v;
+  if (hipGetDevice(&dev) == hipSuccess) {
+    const bool keep = dev >= 0 && dev < 64;
+    if (keep && (v = known[dev].load(std::memory_order_relaxed)) > 0) return v;
+    if (hipDeviceGetAttribute(&v, hipDeviceAttributeMultiprocessorCount, dev) == hipSuccess && v > 0) {
+      if (keep) known[dev].store(v, std::memory_order_relaxed);
+      return v;
+    }
+  }
   (void)hipGetLastError();
   return 256;
 }

@@ -382,52 +382,57 @@ def emb_layer_norm(input_ids, segment_ids, input_mask, word, pos, tok, gamma, be
 
 
 # ---- training and linear launchers --------------------------------------------------------------
-
-def _place(x, stream, **others):
-    """The device and stream of a call on ``x``: every operand lies on ``x``'s device, the call runs there
-    whatever the current device is, on ``stream`` or that device's current stream."""
-    for name, t in others.items():
-        _require(t is None or t.device == x.device, '%s lies on the device of the first operand' % name)
-    if stream is not None:
-        _require(stream.device == x.device, 'stream belongs to the device of the first operand')
-    return x.device
-
+# These are short launches that a step issues by the hundred: pointers go to ctypes as plain integers, the stream
+# handle comes without a Stream object around it, and nothing is allocated that the result does not need.
 
 class _On:
-    """Allocations and the launch of one call: on the operands' device, on the call's stream (results and
-    workspaces then belong to the stream that writes them)."""
+    """Allocations and the launch of one call: on the operands' device whatever the current one is, on the call's stream
+    or that device's current one (results and workspaces then belong to the stream that writes them)."""
 
-    def __init__(self, device, stream):
-        self.device, self.stream, self.guard = device, stream, None
+    def __init__(self, operands, stream):
+        first = operands[0].device
+        for t in operands:
+            _require(t is None or t.device == first, 'all operands lie on one device')
+        _require(stream is None or stream.device == first, 'stream belongs to the device of the operands')
+        self.device, self.guard = first, None
+        if stream is not None:
+            self.guard = torch.cuda.stream(stream)
+        elif first.index != torch.cuda.current_device():
+            self.guard = torch.cuda.device(first)
 
     def __enter__(self):
-        if self.stream is not None:
-            self.guard = torch.cuda.stream(self.stream)
-        elif self.device.index != torch.cuda.current_device():
-            self.guard = torch.cuda.device(self.device)
         if self.guard is not None:
             self.guard.__enter__()
-        return C.c_void_p(torch.cuda.current_stream().cuda_stream)
+        return torch._C._cuda_getCurrentRawStream(self.device.index)
 
     def __exit__(self, *exc):
         if self.guard is not None:
             self.guard.__exit__(*exc)
 
 
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
 def _train_dtype(x, name):
-    if x.dtype not in _TDT:
+    dt = _TDT.get(x.dtype)
+    if dt is None:
         raise TypeError("%s must be float32, float16 or bfloat16, not %s" % (name, x.dtype))
-    return _TDT[x.dtype]
+    return dt
 
 
 def _vector(t, n, name):
-    _require(_dev(t, name).dtype == torch.float32 and t.numel() == n, '%s is float32 with %d elements' % (name, n))
-    return t
+    if t is not None and (_dev(t, name).dtype != torch.float32 or t.numel() != n):
+        _require(False, '%s is float32 with %d elements' % (name, n))
 
 
-def _like(t, x, name):
-    _require(_dev(t, name).dtype == x.dtype and t.shape == x.shape, '%s has the shape and dtype of the input' % name)
-    return t
+def _like(t, shape, dtype, name):
+    if t is not None and (_dev(t, name).dtype != dtype or t.shape != shape):
+        _require(False, '%s has shape %s and dtype %s' % (name, tuple(shape), dtype))
+
+
+def _space(size, device):
+    return torch.empty((size,), dtype=torch.uint8, device=device) if size else None
 
 
 def layer_norm_forward(x, gamma, beta, skip=None, bias=None, eps=0.0, want_sum=False, stream=None):
@@ -437,24 +442,22 @@ def layer_norm_forward(x, gamma, beta, skip=None, bias=None, eps=0.0, want_sum=F
     ``x`` / ``skip``: float32, float16 or bfloat16; gamma / beta / bias: float32 vectors; mean / rstd: float32,
     ``x.shape[:-1]``.
     """
-    x = _dev(x, "input")
-    dt = _train_dtype(x, "input")
-    _require(x.dim() >= 1 and x.shape[-1] > 0, 'input has a last axis of at least one element')
-    ld = x.shape[-1]
-    _vector(gamma, ld, "gamma")
-    _vector(beta, ld, "beta")
-    if bias is not None:
-        _vector(bias, ld, "bias")
-    if skip is not None:
-        _like(skip, x, "skip")
-    device = _place(x, stream, gamma=gamma, beta=beta, skip=skip, bias=bias)
-    with _On(device, stream) as s:
+    dt = _train_dtype(_dev(x, "input"), "input")
+    shape = x.shape
+    ld = shape[-1] if shape else 0
+    _require(ld > 0, 'input has a last axis of at least one element')
+    _vector(_dev(gamma, "gamma"), ld, "gamma")
+    _vector(_dev(beta, "beta"), ld, "beta")
+    _vector(bias, ld, "bias")
+    _like(skip, shape, x.dtype, "skip")
+    with _On((x, gamma, beta, skip, bias), stream) as s:
         y = torch.empty_like(x)
         h = torch.empty_like(x) if want_sum else None
-        mean = torch.empty(x.shape[:-1], dtype=torch.float32, device=device)
+        mean = x.new_empty(shape[:-1], dtype=torch.float32)
         rstd = torch.empty_like(mean)
-        lib.check(lib.dll.fwdmi_layer_norm_forward(s, ld, x.numel(), _p(x), _p(skip), _p(beta), _p(gamma), _p(bias), _p(y),
-                                                   _p(h), _p(mean), _p(rstd), dt, eps))
+        lib.check(lib.dll.fwdmi_layer_norm_forward(s, ld, x.numel(), x.data_ptr(), _ptr(skip), beta.data_ptr(),
+                                                   gamma.data_ptr(), _ptr(bias), y.data_ptr(), _ptr(h), mean.data_ptr(),
+                                                   rstd.data_ptr(), dt, eps))
     return (y, mean, rstd, h) if want_sum else (y, mean, rstd)
 
 
@@ -465,31 +468,28 @@ def layer_norm_backward(dy, x, gamma, mean, rstd, skip=None, bias=None, dsum=Non
     ``x`` and of ``skip`` alike.  ``dsum``: a gradient that reaches the sum from elsewhere, added to ``dx``.
     dgamma / dbeta / dbias are float32, summed over the rows in a fixed order.
     """
-    x = _dev(x, "input")
-    dt = _train_dtype(x, "input")
-    _require(x.dim() >= 1 and x.shape[-1] > 0, 'input has a last axis of at least one element')
-    ld = x.shape[-1]
-    rows = x.numel() // ld
-    _like(dy, x, "dy")
-    _vector(gamma, ld, "gamma")
-    _vector(mean, rows, "mean")
-    _vector(rstd, rows, "rstd")
-    if skip is not None:
-        _like(skip, x, "skip")
-    if bias is not None:
-        _vector(bias, ld, "bias")
-    if dsum is not None:
-        _like(dsum, x, "dsum")
-    device = _place(x, stream, dy=dy, gamma=gamma, mean=mean, rstd=rstd, skip=skip, bias=bias, dsum=dsum)
-    with _On(device, stream) as s:
+    dt = _train_dtype(_dev(x, "input"), "input")
+    shape, n = x.shape, x.numel()
+    ld = shape[-1] if shape else 0
+    _require(ld > 0, 'input has a last axis of at least one element')
+    _like(_dev(dy, "dy"), shape, x.dtype, "dy")
+    _vector(_dev(gamma, "gamma"), ld, "gamma")
+    _vector(_dev(mean, "mean"), n // ld, "mean")
+    _vector(_dev(rstd, "rstd"), n // ld, "rstd")
+    _vector(bias, ld, "bias")
+    _like(skip, shape, x.dtype, "skip")
+    _like(dsum, shape, x.dtype, "dsum")
+    with _On((x, dy, gamma, mean, rstd, skip, bias, dsum), stream) as s:
         dx = torch.empty_like(x)
-        grads = torch.empty((2 if bias is None else 3, ld), dtype=torch.float32, device=device).unbind(0)
-        size = lib.dll.fwdmi_layer_norm_backward_workspace(ld, x.numel(), dt)
-        ws = torch.empty((size,), dtype=torch.uint8, device=device)
-        lib.check(lib.dll.fwdmi_layer_norm_backward(s, ld, x.numel(), _p(dy), _p(x), _p(skip), _p(dsum), _p(gamma),
-                                                    _p(bias), _p(mean), _p(rstd), _p(dx), _p(grads[0]), _p(grads[1]),
-                                                    _p(grads[2]) if bias is not None else None, _p(ws), size, dt))
-    return (dx,) + tuple(grads)
+        dgamma, dbeta = torch.empty_like(gamma), torch.empty_like(gamma)
+        dbias = None if bias is None else torch.empty_like(gamma)
+        size = lib.dll.fwdmi_layer_norm_backward_workspace(ld, n, dt)
+        ws = _space(size, x.device)
+        lib.check(lib.dll.fwdmi_layer_norm_backward(s, ld, n, dy.data_ptr(), x.data_ptr(), _ptr(skip), _ptr(dsum),
+                                                    gamma.data_ptr(), _ptr(bias), mean.data_ptr(), rstd.data_ptr(),
+                                                    dx.data_ptr(), dgamma.data_ptr(), dbeta.data_ptr(), _ptr(dbias),
+                                                    _ptr(ws), size, dt))
+    return (dx, dgamma, dbeta) if bias is None else (dx, dgamma, dbeta, dbias)
 
 
 def _act(activation):
@@ -497,10 +497,14 @@ def _act(activation):
     return ACTIVATIONS[activation]
 
 
-def _weight(weight, x):
+def _linear_sizes(x, weight):
+    """(m, n, k) and the result's shape of a product of ``x`` [..., k] and ``weight`` [n, k]."""
     _require(_dev(weight, "weight").dim() == 2 and weight.dtype == x.dtype, 'weight is [out, in] of the input dtype')
-    _require(x.dim() >= 1 and x.shape[-1] == weight.shape[1], 'the last axis of the input is as long as a row of weight')
-    return weight.shape
+    n, k = weight.shape
+    shape = x.shape
+    _require(len(shape) >= 1 and shape[-1] == k, 'the last axis of the input is as long as a row of weight')
+    m = x.numel() // k if k else shape[:-1].numel()
+    return m, n, k, shape[:-1] + (n,)
 
 
 def linear(x, weight, bias=None, activation="none", residual=None, want_preact=False, stream=None):
@@ -510,27 +514,18 @@ def linear(x, weight, bias=None, activation="none", residual=None, want_preact=F
     ``bias``: a float32 vector; ``activation``: a key of ``ACTIVATIONS``.  With ``want_preact`` returns
     ``(y, z)``, ``z`` the value in front of the activation, which ``linear_backward`` reads.
     """
-    x = _dev(x, "input")
-    dt = _train_dtype(x, "input")
+    dt = _train_dtype(_dev(x, "input"), "input")
     act = _act(activation)
-    n, k = _weight(weight, x)
-    shape = x.shape[:-1] + (n,)
-    m = 1
-    for v in x.shape[:-1]:
-        m *= v
-    if bias is not None:
-        _vector(bias, n, "bias")
-    if residual is not None:
-        _require(_dev(residual, "residual").dtype == x.dtype and residual.shape == shape,
-                 'residual has the shape of the result and the dtype of the input')
-    device = _place(x, stream, weight=weight, bias=bias, residual=residual)
-    with _On(device, stream) as s:
-        y = torch.empty(shape, dtype=x.dtype, device=device)
+    m, n, k, shape = _linear_sizes(x, weight)
+    _vector(bias, n, "bias")
+    _like(residual, shape, x.dtype, "residual")
+    with _On((x, weight, bias, residual), stream) as s:
+        y = x.new_empty(shape)
         z = torch.empty_like(y) if want_preact else None
         size = lib.dll.fwdmi_linear_workspace(m, n, k, dt)
-        ws = torch.empty((size,), dtype=torch.uint8, device=device) if size else None
-        lib.check(lib.dll.fwdmi_linear(s, m, n, k, _p(x), _p(weight), _p(bias), _p(residual), _p(y), _p(z), act, dt, _p(ws),
-                                       size))
+        ws = _space(size, x.device)
+        lib.check(lib.dll.fwdmi_linear(s, m, n, k, x.data_ptr(), weight.data_ptr(), _ptr(bias), _ptr(residual),
+                                       y.data_ptr(), _ptr(z), act, dt, _ptr(ws), size))
     return (y, z) if want_preact else y
 
 
@@ -541,25 +536,18 @@ def linear_backward(dy, x, weight, preact=None, activation="none", want_dx=True,
     ``preact``: what ``linear`` returned for ``want_preact``, needed with an activation.  ``dx`` and ``dweight`` have the
     input's dtype, ``dbias`` is float32.
     """
-    x = _dev(x, "input")
-    dt = _train_dtype(x, "input")
+    dt = _train_dtype(_dev(x, "input"), "input")
     act = _act(activation)
-    n, k = _weight(weight, x)
-    shape = x.shape[:-1] + (n,)
-    m = 1
-    for v in x.shape[:-1]:
-        m *= v
-    _require(_dev(dy, "dy").dtype == x.dtype and dy.shape == shape, 'dy has the shape of the result and the dtype of the input')
-    if act != lib.ACT_NONE:
-        _require(preact is not None and _dev(preact, "preact").dtype == x.dtype and preact.shape == shape,
-                 'an activation needs preact, with the shape of the result and the dtype of the input')
-    device = _place(x, stream, dy=dy, weight=weight, preact=preact)
-    with _On(device, stream) as s:
+    m, n, k, shape = _linear_sizes(x, weight)
+    _like(_dev(dy, "dy"), shape, x.dtype, "dy")
+    _require(act == lib.ACT_NONE or preact is not None, 'an activation needs preact')
+    _like(preact, shape, x.dtype, "preact")
+    with _On((x, dy, weight, preact), stream) as s:
         dx = torch.empty_like(x) if want_dx else None
         dw = torch.empty_like(weight) if want_dweight else None
-        db = torch.empty((n,), dtype=torch.float32, device=device) if want_dbias else None
+        db = x.new_empty((n,), dtype=torch.float32) if want_dbias else None
         size = lib.dll.fwdmi_linear_backward_workspace(m, n, k, act, dt)
-        ws = torch.empty((size,), dtype=torch.uint8, device=device) if size else None
-        lib.check(lib.dll.fwdmi_linear_backward(s, m, n, k, _p(dy), _p(x), _p(weight), _p(preact), _p(dx), _p(dw), _p(db),
-                                                act, dt, _p(ws), size))
+        ws = _space(size, x.device)
+        lib.check(lib.dll.fwdmi_linear_backward(s, m, n, k, dy.data_ptr(), x.data_ptr(), weight.data_ptr(), _ptr(preact),
+                                                _ptr(dx), _ptr(dw), _ptr(db), act, dt, _ptr(ws), size))
     return tuple(t for t in (dx, dw, db) if t is not None)
