@@ -17,14 +17,16 @@ struct Operands {
 
 // The tile and the number of splits of t with the shortest estimated time.  A CU works off its workgroups' steps, each
 // as long as its loads (direct ones reach 90 KB/us per CU, those through registers 40) or its matrix instructions take
-// (kRate: flop/us per CU that the steps of each tile sustain, bf16; fp32 instructions bound all tiles alike), plus what a
-// round of tiles spends outside its steps and, with splits, the second launch and the partial products' way through
-// the caches.  Measured: 8192 x 4096 x 1024 64 us with 256 x 256, 74 with 256 x 128, 84 with 128 x 128;
-// 8192 x 1024 x 4096 66 us with 256 x 128, 67 with 128 x 128; 384 x 1024 x 4096 12 us with 64 x 32, 15 with 64 x 64,
+// (kRate: flop/us per CU that the steps of each tile sustain in bf16, for operands along t or only b across, and both
+// across; fp32 instructions bound all tiles alike), plus what a round of tiles spends outside its steps and, with splits,
+// the second launch and the partial products' way through the caches.  Measured: 8192 x 4096 x 1024 64 us with 256 x 256, 74 with 256 x 128, 84 with 128 x 128;
+// 8192 x 1024 x 4096 (b across) 66 us with 256 x 128, 81 with 128 x 128;
+// 4096 x 1024 x 8192 (both across) 63 us and 15 to add four splits with 256 x 256, 72 and 9 with 256 x 128 and two; 384 x 1024 x 4096 12 us with 64 x 32, 15 with 64 x 64,
 // 20 and more with 128 x 128.
 Plan make_plan(int ni, int nj, int nt, const Operands& o) {
-  static const double kRate[kTileKinds] = {6.0e6, 4.6e6, 4.4e6, 3.5e6, 3.0e6};
+  static const double kRate[2][kTileKinds] = {{6.0e6, 4.6e6, 4.0e6, 3.5e6, 3.0e6}, {6.0e6, 4.3e6, 2.2e6, 3.5e6, 3.0e6}};
   static const double kRound[kTileKinds] = {9.0, 4.0, 3.0, 1.5, 1.0};
+  if (o.layouts == 0 && ni <= kFewRows) return Plan{kFew, 1, 0, 0, 0};
   const int cus = device_cus();
   Plan best{};
   double best_us = 1e30;
@@ -35,7 +37,7 @@ Plan make_plan(int ni, int nj, int nt, const Operands& o) {
     const int all = p.whole_steps + (p.tail > 0);
     const int64_t tiles = (int64_t)ceil_div(ni, t.ti) * ceil_div(nj, t.tj);
     const double load = (t.ti + t.tj) * t.step_bytes / ((o.direct ? 90.0 : 40.0) * 1024);
-    const double flops = 2.0 * t.ti * t.tj * (t.step_bytes / o.elem) / (o.elem == 2 ? kRate[kind] : 0.55e6);
+    const double flops = 2.0 * t.ti * t.tj * (t.step_bytes / o.elem) / (o.elem == 2 ? kRate[o.layouts == 2][kind] : 0.47e6);
     const double step = std::max(load, flops);
     for (int target = 0; target <= 2; ++target) {  // one workgroup per tile, or splits for one or two per CU
       const int64_t want = target == 0 ? 1 : target * (int64_t)cus / tiles;
@@ -44,7 +46,7 @@ Plan make_plan(int ni, int nj, int nt, const Operands& o) {
       p.steps_per_split = std::max(1, ceil_div(all, splits));
       p.splits = std::max(1, ceil_div(all, p.steps_per_split));
       double us = 2.0 + ceil_div(tiles * p.splits, cus) * (kRound[kind] + p.steps_per_split * step);
-      if (p.splits > 1) us += 4.0 + 8.0 * p.splits * ni * nj / 4.0e6;
+      if (p.splits > 1) us += 3.0 + 6.0 * p.splits * ni * nj / 5.0e6;
       if (us < best_us) {
         best_us = us;
         best = p;

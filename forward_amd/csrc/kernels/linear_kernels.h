@@ -90,53 +90,53 @@ __device__ __forceinline__ void with_act(int act, F&& f) {
   }
 }
 
-__device__ __forceinline__ void load_bias(const Product& P, int j, float (&b)[8]) {
+template <int N>
+__device__ __forceinline__ void load_bias(const Product& P, int j, float (&b)[N]) {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) b[e] = 0.0f;
+  for (int e = 0; e < N; ++e) b[e] = 0.0f;
   if (!P.bias) return;
-  if (j + 8 <= P.nj) {
-    const Pack<float, 4> lo = load_slice<float, 4>(gconst<float>(P.bias) + j);
-    const Pack<float, 4> hi = load_slice<float, 4>(gconst<float>(P.bias) + j + 4);
+  if (j + N <= P.nj) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      b[e] = lo.v[e];
-      b[e + 4] = hi.v[e];
+    for (int q = 0; q < N / 4; ++q) {
+      const Pack<float, 4> v = load_slice<float, 4>(gconst<float>(P.bias) + j + q * 4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) b[q * 4 + e] = v.v[e];
     }
   } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
+    for (int e = 0; e < N; ++e)
       if (j + e < P.nj) b[e] = gconst<float>(P.bias)[j + e];
   }
 }
 
-// y = act(z) + residual, z = acc + bias, of eight neighbours of one row: columns j .. j + 7, all of them (WHOLE) or
+// y = act(z) + residual, z = acc + bias, of N neighbours of one row: columns j .. j + N - 1, all of them (WHOLE) or
 // those below nj.
-template <typename T, int ACT, bool WHOLE>
-__device__ __forceinline__ void finish(const Product& P, int64_t i, int j, const float (&acc)[8], const float (&b)[8]) {
+template <typename T, int ACT, bool WHOLE, int N>
+__device__ __forceinline__ void finish(const Product& P, int64_t i, int j, const float (&acc)[N], const float (&b)[N]) {
   const int64_t at = i * P.nj + j;
-  const int live = WHOLE ? 8 : min(P.nj - j, 8);
-  Pack<T, 8> y, z, r{};
+  const int live = WHOLE ? N : min(P.nj - j, N);
+  Pack<T, N> y, z, r{};
   if (P.residual) {
-    if (live == 8) {
-      r = load_slice<T, 8>(gconst<T>(P.residual) + at);
+    if (live == N) {
+      r = load_slice<T, N>(gconst<T>(P.residual) + at);
     } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
+      for (int e = 0; e < N; ++e)
         if (e < live) r.v[e] = gconst<T>(P.residual)[at + e];
     }
   }
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
+  for (int e = 0; e < N; ++e) {
     const float s = acc[e] + b[e];
     z.v[e] = (T)s;
     y.v[e] = (T)(activate<ACT, sizeof(T) == 4>(s) + (float)r.v[e]);
   }
-  if (live == 8) {
-    store_slice<T, 8>(gmut<T>(P.c) + at, y);
-    if (P.preact) store_slice<T, 8>(gmut<T>(P.preact) + at, z);
+  if (live == N) {
+    store_slice<T, N>(gmut<T>(P.c) + at, y);
+    if (P.preact) store_slice<T, N>(gmut<T>(P.preact) + at, z);
   } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
+    for (int e = 0; e < N; ++e)
       if (e < live) {
         gmut<T>(P.c)[at + e] = y.v[e];
         if (P.preact) gmut<T>(P.preact)[at + e] = z.v[e];
@@ -348,12 +348,12 @@ __device__ __forceinline__ F4 multiply(const Frag<T>& b, const Frag<T>& a, F4 ac
   }
 }
 
-// The steps of t that this workgroup's split walks: whole ones from `first` on, and `tail` elements of a last one.
+// The steps of t that a split walks: whole ones from `first` on, and `tail` elements of a last one.
 struct Steps {
   int first, whole, tail;
 };
-__device__ __forceinline__ Steps split_steps(const Product& P) {
-  const int first = (int)blockIdx.y * P.steps_per_split, end = first + P.steps_per_split;
+__device__ __forceinline__ Steps split_steps(const Product& P, int split) {
+  const int first = split * P.steps_per_split, end = first + P.steps_per_split;
   const int whole = max(min(end, P.whole_steps) - first, 0);
   return Steps{first, whole, first <= P.whole_steps && end > P.whole_steps ? P.tail : 0};
 }
@@ -361,25 +361,28 @@ __device__ __forceinline__ Steps split_steps(const Product& P) {
 // The immediate of s_waitcnt that waits until at most n vector memory operations are in flight (and for nothing else).
 constexpr int wait_loads(int n) { return (n & 15) | (n >> 4) << 14 | 0x0f70; }
 
-// The tile of this workgroup.  Workgroups go to the XCDs in turn, so the numbers are dealt out in eight runs of
-// neighbours, one per XCD, and a run walks columns of at most eight tiles: the tiles an XCD works on at a time share
-// their lines of A and B in its L2.
+// The tile and split of this workgroup.  Workgroups go to the XCDs in turn, so the numbers are dealt out in eight runs
+// of neighbours, one per XCD; a run stays in one split as long as it can and walks columns of at most kGroup tiles, so
+// that the tiles an XCD works on at a time share their lines of A and B in its L2.
 template <int TI, int TJ>
-__device__ __forceinline__ void locate_tile(const Product& P, int& i0, int& j0) {
-  const int total = P.tiles_i * P.tiles_j, b = (int)blockIdx.x;
+__device__ __forceinline__ int locate_tile(const Product& P, int& i0, int& j0) {
+  const int tiles = P.tiles_i * P.tiles_j, total = (int)gridDim.x, b = (int)blockIdx.x;
   const int xcd = b & 7, per = total >> 3, more = total & 7;
   const int n = xcd * per + min(xcd, more) + (b >> 3);
-  constexpr int kGroup = 8;
-  const int group = n / (kGroup * P.tiles_j), first = group * kGroup;
-  const int height = min(P.tiles_i - first, kGroup), in = n - group * kGroup * P.tiles_j;
+  const int split = n / tiles, m = n - split * tiles;
+  constexpr int kGroup = TI > TJ ? 4 : 8;
+  const int group = m / (kGroup * P.tiles_j), first = group * kGroup;
+  const int height = min(P.tiles_i - first, kGroup), in = m - group * kGroup * P.tiles_j;
   i0 = (first + in % height) * TI;
   j0 = in / height * TJ;
+  return split;
 }
 
 // The tile leaves through LDS, as much of it at a time as the buffers hold, so that every row is read back and stored
 // in whole 16-byte slices by neighbouring lanes.  16-byte chunk c of row r lies at c ^ (r & 15).
 template <typename T, int TI, int TJ, int WI, int WJ, int WK, int ROOM, bool EPILOGUE, int FI, int FJ>
-__device__ __forceinline__ void leave_tile(const Product& P, const F4 (&acc)[FJ][FI], char* s_tile, int i0, int j0) {
+__device__ __forceinline__ void leave_tile(const Product& P, const F4 (&acc)[FJ][FI], char* s_tile, int i0, int j0,
+                                           int split) {
   constexpr int kNT = 64 * WI * WJ * WK;
   constexpr int kAllBytes = TI * TJ * 4 * WK;
   constexpr int kPhases = kAllBytes <= ROOM ? 1 : kAllBytes <= 2 * ROOM ? 2 : 4;
@@ -426,7 +429,7 @@ __device__ __forceinline__ void leave_tile(const Product& P, const F4 (&acc)[FJ]
       }
     };
     if (P.partial) {
-      float FWDMI_GLOBAL* const out = gmut<float>(P.partial) + (int64_t)blockIdx.y * P.ni * P.nj;
+      float FWDMI_GLOBAL* const out = gmut<float>(P.partial) + (int64_t)split * P.ni * P.nj;
       leave([&](int64_t i, int j, const float (&v)[8]) {
         float FWDMI_GLOBAL* const p = out + i * P.nj + j;
         if (j + 8 <= P.nj) {
@@ -460,13 +463,13 @@ __device__ __forceinline__ void leave_tile(const Product& P, const F4 (&acc)[FJ]
 // block, so that a store instruction writes 64 contiguous bytes of each of its 16 rows: no LDS, no barrier, and the two
 // waves of a SIMD overlap each other's arithmetic and stores.
 template <typename T, int TI, int TJ, int WI, int WJ, bool EPILOGUE, int FI, int FJ>
-__device__ __forceinline__ void leave_registers(const Product& P, const F4 (&acc)[FJ][FI], int i0, int j0) {
+__device__ __forceinline__ void leave_registers(const Product& P, const F4 (&acc)[FJ][FI], int i0, int j0, int split) {
   const int lane = threadIdx.x & 63, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int i_lane = i0 + wave % WI * (TI / WI) + (lane & 15);
   const int j_lane = j0 + wave / WI * (TJ / WJ) + (g & 1) * 8 + (g >> 1) * 16;
   if (P.partial) {  // four fp32 neighbours are 16 bytes as they lie
-    float FWDMI_GLOBAL* const out = gmut<float>(P.partial) + (int64_t)blockIdx.y * P.ni * P.nj;
+    float FWDMI_GLOBAL* const out = gmut<float>(P.partial) + (int64_t)split * P.ni * P.nj;
     const int j4 = j0 + wave / WI * (TJ / WJ) + g * 4;
 #pragma unroll
     for (int i = 0; i < FI; ++i)
@@ -521,10 +524,10 @@ __global__ __launch_bounds__(64 * WI * WJ * WK) void product_kernel(const Produc
   __shared__ __attribute__((aligned(1024))) char s_tile[STAGES * kBuffer];
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   int i0, j0;
-  locate_tile<TI, TJ>(P, i0, j0);
+  const int split = locate_tile<TI, TJ>(P, i0, j0);
   const int wi = wave % WI * (TI / WI), wj = wave / WI % WJ * (TJ / WJ), wk = wave / (WI * WJ);
 
-  const Steps steps = split_steps(P);
+  const Steps steps = split_steps(P, split);
 
   F4 acc[kFJ][kFI];
 #pragma unroll
@@ -609,7 +612,7 @@ __global__ __launch_bounds__(64 * WI * WJ * WK) void product_kernel(const Produc
       if (s + 1 < n) step(std::integral_constant<int, 1>{}, s + 1);
     }
   }
-  leave_tile<T, TI, TJ, WI, WJ, WK, STAGES * kBuffer, LA == kAlong && LB == kAlong>(P, acc, s_tile, i0, j0);
+  leave_tile<T, TI, TJ, WI, WJ, WK, STAGES * kBuffer, LA == kAlong && LB == kAlong>(P, acc, s_tile, i0, j0, split);
 }
 
 template <int... I, typename F>
@@ -640,9 +643,9 @@ __global__ __launch_bounds__(512) void product_turns_kernel(const Product P) {
   __shared__ __attribute__((aligned(1024))) char s_tile[STAGES * kBuffer];
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   int i0, j0;
-  locate_tile<TI, TJ>(P, i0, j0);
+  const int split = locate_tile<TI, TJ>(P, i0, j0);
   const int wi = wave % WI * (TI / WI), wj = wave / WI * (TJ / WJ);
-  const Steps steps = split_steps(P);
+  const Steps steps = split_steps(P, split);
 
   F4 acc[kFJ][kFI];
 #pragma unroll
@@ -714,9 +717,86 @@ __global__ __launch_bounds__(512) void product_turns_kernel(const Product P) {
     });
   }
   if (j0 + TJ <= P.nj)
-    leave_registers<T, TI, TJ, WI, WJ, LA == kAlong && LB == kAlong>(P, acc, i0, j0);
+    leave_registers<T, TI, TJ, WI, WJ, LA == kAlong && LB == kAlong>(P, acc, i0, j0, split);
   else
-    leave_tile<T, TI, TJ, WI, WJ, 1, STAGES * kBuffer, LA == kAlong && LB == kAlong>(P, acc, s_tile, i0, j0);
+    leave_tile<T, TI, TJ, WI, WJ, 1, STAGES * kBuffer, LA == kAlong && LB == kAlong>(P, acc, s_tile, i0, j0, split);
+}
+
+// A few rows (at most 16 MB tokens) through a matrix of weights: one pass over w.  A workgroup takes 16 rows of w and
+// all of x; its waves take 128-byte pieces of t in turn, straight from memory to the matrix instructions (a piece is
+// read by one wave alone, LDS would only add a stop), two pieces in flight, and their sums meet in LDS in wave order.
+// Rows past the last repeat it, their products are dropped.
+template <typename T, int MB>
+__global__ __launch_bounds__(1024) void product_few_kernel(const Product P) {
+  extern __shared__ __attribute__((aligned(16))) F4 s_sum[];  // [waves][MB][64]
+  constexpr int kPiece = 128 / (int)sizeof(T), kHalf = kPiece / 2;
+  const int lane = threadIdx.x & 63, g = lane >> 4, r = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), waves = (int)blockDim.x >> 6;
+  const int j0 = (int)blockIdx.x * 16;
+  const T FWDMI_GLOBAL* const pw = gconst<T>(P.b) + (int64_t)min(j0 + r, P.nj - 1) * P.ldb + g * kChunk<T>;
+  const T FWDMI_GLOBAL* px[MB];
+#pragma unroll
+  for (int b = 0; b < MB; ++b) px[b] = gconst<T>(P.a) + (int64_t)min(b * 16 + r, P.ni - 1) * P.lda + g * kChunk<T>;
+  F4 acc[MB];
+#pragma unroll
+  for (int b = 0; b < MB; ++b) acc[b] = F4{0.0f, 0.0f, 0.0f, 0.0f};
+
+  const int pieces = P.nt / kPiece;
+  constexpr int kBatch = 2;
+  auto batch = [&](int piece, auto count) {
+    constexpr int kN = decltype(count)::value;
+    Frag<T> w[kN][2], x[kN][2][MB];
+#pragma unroll
+    for (int k = 0; k < kN; ++k)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int64_t t = (int64_t)(piece + k * waves) * kPiece + h * kHalf;
+        w[k][h].v = load_slice<T, kChunk<T>>(pw + t);
+#pragma unroll
+        for (int b = 0; b < MB; ++b) x[k][h][b].v = load_slice<T, kChunk<T>>(px[b] + t);
+      }
+#pragma unroll
+    for (int k = 0; k < kN; ++k)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int b = 0; b < MB; ++b) acc[b] = multiply<T>(w[k][h], x[k][h][b], acc[b]);
+  };
+  int piece = wave;
+  for (; piece + (kBatch - 1) * waves < pieces; piece += kBatch * waves) batch(piece, std::integral_constant<int, kBatch>{});
+  for (; piece < pieces; piece += waves) batch(piece, std::integral_constant<int, 1>{});
+  if (piece == pieces && P.nt % kPiece != 0) {  // the wave whose turn it is takes what is left, element by element
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int t = pieces * kPiece + h * kHalf, n = P.nt - t - g * kChunk<T>;
+      auto some = [&](const T FWDMI_GLOBAL* p) {
+        Frag<T> f;
+#pragma unroll
+        for (int e = 0; e < kChunk<T>; ++e) f.v.v[e] = e < n ? p[t + e] : (T)0.0f;
+        return f;
+      };
+      const Frag<T> w = some(pw);
+#pragma unroll
+      for (int b = 0; b < MB; ++b) acc[b] = multiply<T>(w, some(px[b]), acc[b]);
+    }
+  }
+#pragma unroll
+  for (int b = 0; b < MB; ++b) s_sum[(wave * MB + b) * 64 + lane] = acc[b];
+  __syncthreads();
+  if (wave < MB) {
+    float v[4] = {};
+    for (int k = 0; k < waves; ++k) {
+      const F4 part = s_sum[(k * MB + wave) * 64 + lane];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] += part[e];
+    }
+    const int i = wave * 16 + r, j = j0 + g * 4;
+    if (i < P.ni && j < P.nj) {
+      float b[4];
+      load_bias(P, j, b);
+      with_act(P.act, [&](auto act) { finish<T, decltype(act)::value, false>(P, i, j, v, b); });
+    }
+  }
 }
 
 // Adds the splits' partial products in split order and finishes them; eight neighbours of a row per lane.
@@ -731,19 +811,30 @@ __global__ __launch_bounds__(256) void finish_kernel(const Product P, int splits
   const float FWDMI_GLOBAL* p = gconst<float>(P.partial) + i * P.nj + j;
   const int live = min(P.nj - j, 8);
   float acc[8] = {};
-  for (int s = 0; s < splits; ++s, p += plane) {
-    if (live == 8) {
-      const Pack<float, 4> lo = load_slice<float, 4>(p), hi = load_slice<float, 4>(p + 4);
+  if (live == 8) {
+    constexpr int kBatch = 4;  // splits in flight
+    for (int s = 0; s < splits; s += kBatch) {
+      Pack<float, 4> lo[kBatch], hi[kBatch];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        acc[e] += lo.v[e];
-        acc[e + 4] += hi.v[e];
+      for (int k = 0; k < kBatch; ++k) {
+        const float FWDMI_GLOBAL* const q = p + min(s + k, splits - 1) * plane;
+        lo[k] = load_slice<float, 4>(q);
+        hi[k] = load_slice<float, 4>(q + 4);
       }
-    } else {
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k)
+        if (s + k < splits)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            acc[e] += lo[k].v[e];
+            acc[e + 4] += hi[k].v[e];
+          }
+    }
+  } else {
+    for (int s = 0; s < splits; ++s, p += plane)
 #pragma unroll
       for (int e = 0; e < 8; ++e)
         if (e < live) acc[e] += p[e];
-    }
   }
   float b[8];
   load_bias(P, j, b);
@@ -808,13 +899,26 @@ __global__ __launch_bounds__(256) void slope_kernel(const Slope S) {
 
 template <typename T, int LA, int LB, bool DIRECT>
 int launch_product(Product& P, const Plan& plan, hipStream_t stream) {
+  if constexpr (LA == kAlong && LB == kAlong) {
+    if (plan.tile == kFew) {
+      const int pieces = P.nt / (128 / (int)sizeof(T));
+      const int waves = pieces >= 32 ? 16 : pieces >= 16 ? 8 : 4;
+      const dim3 grid((unsigned)ceil_div(P.nj, 16)), block(64 * waves);
+      if (P.ni <= 16)
+        hipLaunchKernelGGL((product_few_kernel<T, 1>), grid, block, waves * 1024, stream, P);
+      else
+        hipLaunchKernelGGL((product_few_kernel<T, 2>), grid, block, waves * 2048, stream, P);
+      FWDMI_HIP_CHECK(hipGetLastError());
+      return FWDMI_OK;
+    }
+  }
   const TileShape tile = kTiles[plan.tile];
   P.tiles_i = ceil_div(P.ni, tile.ti);
   P.tiles_j = ceil_div(P.nj, tile.tj);
   P.whole_steps = plan.whole_steps;
   P.tail = plan.tail;
   P.steps_per_split = plan.steps_per_split;
-  const dim3 grid((unsigned)(P.tiles_i * P.tiles_j), (unsigned)plan.splits);
+  const dim3 grid((unsigned)(P.tiles_i * P.tiles_j * plan.splits));
   if constexpr (sizeof(T) == 2 && DIRECT) {
     if (plan.tile == k256x256)
       hipLaunchKernelGGL((product_turns_kernel<T, LA, LB, 256, 256, 2, 4, 2>), grid, dim3(512), 0, stream, P);

@@ -41,7 +41,9 @@ struct Slope {
 };
 
 // The tiles there are.  The first two are the eight-wave kernel of 16-bit operands (product_turns_kernel).
-enum TileKind { k256x256, k256x128, k128x128, k64x64, k64x32, kTileKinds };
+// kFew: product_few_kernel, at most kFewRows rows of x.
+enum TileKind { k256x256, k256x128, k128x128, k64x64, k64x32, kTileKinds, kFew = kTileKinds };
+constexpr int kFewRows = 32;
 struct TileShape {
   int ti, tj, step_bytes;
 };

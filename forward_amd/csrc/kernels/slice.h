@@ -51,8 +51,18 @@ __global__ __launch_bounds__(64 * kSumWaves) void column_sums_kernel(const Colum
   const int64_t width = (int64_t)S.kinds * S.ld;
   const int64_t c = (int64_t)blockIdx.x * 64 + lane;
   float a = 0.0f;
-  if (c < width)
-    for (int p = wave; p < S.parts; p += kSumWaves) a += gconst<float>(S.part)[p * width + c];
+  if (c < width) {
+    const float FWDMI_GLOBAL* at = gconst<float>(S.part) + wave * width + c;
+    int left = (S.parts - wave + kSumWaves - 1) / kSumWaves;  // rows of this wave
+    for (; left >= 8; left -= 8, at += 8 * kSumWaves * width) {  // eight in flight, added in row order
+      float v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = at[k * kSumWaves * width];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) a += v[k];
+    }
+    for (; left > 0; --left, at += kSumWaves * width) a += *at;
+  }
   s_red[wave][lane] = a;
   __syncthreads();
   if (wave == 0 && c < width) {
