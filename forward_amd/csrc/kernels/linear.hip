@@ -9,10 +9,11 @@ namespace fwdmi {
 namespace {
 
 // What bounds a product's operands: the layouts (0 both along t, 1 a along and b across, 2 both across), whether they
-// may be loaded directly and, if so, whether rows across t end inside a chunk.
+// may be loaded directly and, if so, how the end of t is (through registers: kTail).
 struct Operands {
   int layouts, elem;
-  bool direct, ragged;
+  bool direct;
+  End end;
 };
 
 // The tile and the number of splits of t with the shortest estimated time.  A CU works off its workgroups' steps, each
@@ -26,14 +27,14 @@ struct Operands {
 Plan make_plan(int ni, int nj, int nt, const Operands& o) {
   static const double kRate[2][kTileKinds] = {{6.0e6, 4.6e6, 4.0e6, 3.5e6, 3.0e6}, {6.0e6, 4.3e6, 2.2e6, 3.5e6, 3.0e6}};
   static const double kRound[kTileKinds] = {9.0, 4.0, 3.0, 1.5, 1.0};
-  if (o.layouts == 0 && ni <= kFewRows) return Plan{kFew, 1, 0, 0, 0};
+  if (o.layouts == 0 && ni <= kFewRows) return Plan{kFew, 1, 0, 0, 0, 0.0};
   const int cus = device_cus();
   Plan best{};
   double best_us = 1e30;
   for (int kind = o.elem == 2 && o.direct ? k256x256 : k128x128; kind < kTileKinds; ++kind) {
     const TileShape t = kTiles[kind];
-    Plan p{(TileKind)kind, 1, 0, 0, 0};
-    tail_of(nt, t.step_bytes / o.elem, o.direct && o.ragged, p.whole_steps, p.tail);
+    Plan p{(TileKind)kind, 1, 0, 0, 0, 0.0};
+    tail_of(nt, t.step_bytes / o.elem, o.end, p.whole_steps, p.tail);
     const int all = p.whole_steps + (p.tail > 0);
     const int64_t tiles = (int64_t)ceil_div(ni, t.ti) * ceil_div(nj, t.tj);
     const double load = (t.ti + t.tj) * t.step_bytes / ((o.direct ? 90.0 : 40.0) * 1024);
@@ -50,6 +51,7 @@ Plan make_plan(int ni, int nj, int nt, const Operands& o) {
       if (us < best_us) {
         best_us = us;
         best = p;
+        best.us = us;
       }
     }
   }
@@ -60,27 +62,31 @@ size_t partial_bytes(const Plan& p, int ni, int nj) {
   return p.splits > 1 ? (size_t)p.splits * ni * nj * sizeof(float) : 0;
 }
 
-bool ragged_rows(int layouts, int ni, int nj, int elem) {
+End end_of(int layouts, int ni, int nj, int nt, int64_t lda, int64_t ldb, int elem) {
   const int chunk = 16 / elem;
-  return (layouts == 2 && ni % chunk != 0) || (layouts >= 1 && nj % chunk != 0);
+  // (lines longer than their contents are copies made here, with zeros behind)
+  auto part = [&](int n, int64_t ld) { return n % chunk != 0 && ld < (int64_t)ceil_div(n, chunk) * chunk; };
+  if ((layouts == 2 && part(ni, lda)) || (layouts >= 1 && part(nj, ldb))) return kTailLine;
+  return (layouts <= 1 && part(nt, lda)) || (layouts == 0 && part(nt, ldb)) ? kTail : kWhole;
 }
 
 int run(Product& P, int layouts, int dtype, void* workspace, hipStream_t stream) {
   const int elem = dtype == FWDMI_F32 ? 4 : 2;
-  const Operands o{layouts, elem, direct_ok(P.a, P.lda, elem) && direct_ok(P.b, P.ldb, elem),
-                   ragged_rows(layouts, P.ni, P.nj, elem)};
+  const bool direct = direct_ok(P.a, P.lda, elem) && direct_ok(P.b, P.ldb, elem);
+  const Operands o{layouts, elem, direct, direct ? end_of(layouts, P.ni, P.nj, P.nt, P.lda, P.ldb, elem) : kTail};
   const Plan plan = make_plan(P.ni, P.nj, P.nt, o);
   P.partial = plan.splits > 1 ? static_cast<float*>(workspace) : nullptr;
-  return dtype == FWDMI_F16    ? run_product_f16(P, layouts, plan, o.direct, stream)
-         : dtype == FWDMI_BF16 ? run_product_bf16(P, layouts, plan, o.direct, stream)
-                               : run_product_f32(P, layouts, plan, o.direct, stream);
+  return dtype == FWDMI_F16    ? run_product_f16(P, layouts, plan, direct, stream)
+         : dtype == FWDMI_BF16 ? run_product_bf16(P, layouts, plan, direct, stream)
+                               : run_product_f32(P, layouts, plan, direct, stream);
 }
 
-// Partial products of either plan (which of the two runs depends on the operands' alignment).
+// Partial products of any plan that `run` may choose for these sizes (that depends on the operands' alignment too).
 size_t product_bytes(int layouts, int64_t ni, int64_t nj, int64_t nt, int elem) {
   size_t bytes = 0;
-  for (int direct = 0; direct < 2; ++direct) {
-    const Operands o{layouts, elem, direct != 0, ragged_rows(layouts, (int)ni, (int)nj, elem)};
+  for (const Operands& o : {Operands{layouts, elem, true, kWhole}, Operands{layouts, elem, true, kTail},
+                            Operands{layouts, elem, true, kTailLine}, Operands{layouts, elem, false, kTail}}) {
+    if (o.end == kTailLine && layouts == 0) continue;
     bytes = std::max(bytes, partial_bytes(make_plan((int)ni, (int)nj, (int)nt, o), (int)ni, (int)nj));
   }
   return bytes;
@@ -88,10 +94,34 @@ size_t product_bytes(int layouts, int64_t ni, int64_t nj, int64_t nt, int elem) 
 
 int elem_size(int dtype) { return dtype == FWDMI_F32 ? 4 : 2; }
 size_t align256(size_t v) { return (v + 255) / 256 * 256; }
+int64_t widened(int64_t ld) { return (ld + 7) / 8 * 8; }
 
-constexpr int64_t kMaxDim = (int64_t)1 << 30;  // of each of m, n, k: tile numbers and row ends stay in 31 bits
+// Lines of an odd number of 16-bit elements cannot be loaded directly.  Where copies with whole lines cost less than
+// direct loads gain (an estimate from the sizes alone, so that the workspace's size follows from them too), operands are
+// copied first.  `us`: what the products are estimated to take through registers and directly.
+bool widening_pays(int64_t ld, int elem, double lines, double registers_us, double direct_us) {
+  if (elem != 2 || ld % 2 == 0) return false;
+  return direct_us + 4.0 + lines * (double)ld * 2 * elem / 4.0e6 < registers_us;
+}
+bool widen_forward(int64_t m, int64_t n, int64_t k, int elem) {
+  if (m <= kFewRows || elem != 2 || k % 2 == 0) return false;
+  return widening_pays(k, elem, (double)(m + n), make_plan((int)m, (int)n, (int)k, Operands{0, elem, false, kTail}).us,
+                       make_plan((int)m, (int)n, (int)k, Operands{0, elem, true, kWhole}).us);
+}
+bool widen_backward(int64_t m, int64_t n, int64_t k, int elem) {
+  if (elem != 2 || k % 2 == 0) return false;
+  auto both = [&](bool direct) {
+    return make_plan((int)m, (int)k, (int)n, Operands{1, elem, direct, direct ? kWhole : kTail}).us +
+           make_plan((int)n, (int)k, (int)m, Operands{2, elem, direct, direct ? kWhole : kTail}).us;
+  };
+  return widening_pays(k, elem, (double)(m + n), both(false), both(true));
+}
+
+constexpr int64_t kMaxDim = (int64_t)1 << 30;   // of each of m, n, k, and of their products in pairs: tile numbers and
+constexpr double kMaxPlane = 1099511627776.0;   // launch sizes stay in 31 bits
 bool dims_ok(int64_t m, int64_t n, int64_t k) {
-  return m >= 0 && n >= 0 && k >= 0 && m <= kMaxDim && n <= kMaxDim && k <= kMaxDim;
+  return m >= 0 && n >= 0 && k >= 0 && m <= kMaxDim && n <= kMaxDim && k <= kMaxDim && (double)m * n <= kMaxPlane &&
+         (double)m * k <= kMaxPlane && (double)n * k <= kMaxPlane;
 }
 
 int slope_parts(int64_t m, int64_t n) {
@@ -100,19 +130,44 @@ int slope_parts(int64_t m, int64_t n) {
   return (int)std::max<int64_t>(1, std::min<int64_t>((m + 3) / 4, std::min<int64_t>(want, 256)));
 }
 
-// Workspace of the backward pass: dz, its column sums' partials, then the larger of the two products' partials.
+// Workspace of the forward pass: copies of x and w with whole lines, then the partial products.
+struct ForwardSpace {
+  size_t x, w, product;
+  size_t total() const { return x + w + product; }
+};
+ForwardSpace forward_space(int64_t m, int64_t n, int64_t k, int dtype) {
+  const int elem = elem_size(dtype);
+  ForwardSpace s{0, 0, 0};
+  if (m == 0 || n == 0) return s;
+  if (widen_forward(m, n, k, elem)) {
+    s.x = align256((size_t)m * widened(k) * elem);
+    s.w = align256((size_t)n * widened(k) * elem);
+  }
+  s.product = product_bytes(0, m, n, k, elem);
+  return s;
+}
+
+// Workspace of the backward pass: dz (with an activation, or where dy's lines are odd), its column sums' partials, copies
+// of x and w with whole lines, then the larger of the two products' partials.
 struct BackwardSpace {
-  size_t dz, part, product;
-  size_t total() const { return dz + part + product; }
+  size_t dz, part, x, w, product;
+  int64_t ld_dz;
+  size_t total() const { return dz + part + x + w + product; }
 };
 BackwardSpace backward_space(int64_t m, int64_t n, int64_t k, int act, int dtype) {
   const int elem = elem_size(dtype);
-  BackwardSpace s{0, 0, 0};
+  BackwardSpace s{0, 0, 0, 0, 0, n};
   if (m == 0 || n == 0) return s;
-  if (act != FWDMI_ACT_NONE) s.dz = align256((size_t)m * n * elem);
+  if (elem == 2 && n % 2 != 0) s.ld_dz = widened(n);
+  if (act != FWDMI_ACT_NONE || s.ld_dz != n) s.dz = align256((size_t)m * s.ld_dz * elem);
   s.part = align256((size_t)slope_parts(m, n) * n * sizeof(float));
-  if (k > 0)
+  if (k > 0) {
+    if (widen_backward(m, n, k, elem)) {
+      s.x = align256((size_t)m * widened(k) * elem);
+      s.w = align256((size_t)n * widened(k) * elem);
+    }
     s.product = std::max(product_bytes(1, m, k, n, elem), product_bytes(2, n, k, m, elem));
+  }
   return s;
 }
 
@@ -124,7 +179,7 @@ extern "C" {
 size_t fwdmi_linear_workspace(int64_t m, int64_t n, int64_t k, int32_t dtype) {
   using namespace fwdmi;
   if (!is_train_dtype(dtype) || !dims_ok(m, n, k) || m == 0 || n == 0) return 0;
-  return product_bytes(0, m, n, k, elem_size(dtype));
+  return forward_space(m, n, k, dtype).total();
 }
 
 int fwdmi_linear(void* stream, int64_t m, int64_t n, int64_t k, const void* x, const void* w, const float* bias,
@@ -137,13 +192,23 @@ int fwdmi_linear(void* stream, int64_t m, int64_t n, int64_t k, const void* x, c
   FWDMI_REQUIRE(dims_ok(m, n, k), "linear: m=%lld n=%lld k=%lld", (long long)m, (long long)n, (long long)k);
   if (m == 0 || n == 0) return FWDMI_OK;
   FWDMI_REQUIRE(y && (k == 0 || (x && w)), "linear: null pointer");
-  const size_t need = fwdmi_linear_workspace(m, n, k, dtype);
-  FWDMI_REQUIRE(need == 0 || (workspace && workspace_size >= need && reinterpret_cast<uintptr_t>(workspace) % 16 == 0),
-                "linear: workspace of %zu bytes, %zu needed", workspace ? workspace_size : (size_t)0, need);
+  const ForwardSpace space = forward_space(m, n, k, dtype);
+  FWDMI_REQUIRE(space.total() == 0 || (workspace && workspace_size >= space.total() &&
+                                       reinterpret_cast<uintptr_t>(workspace) % 16 == 0),
+                "linear: workspace of %zu bytes, %zu needed", workspace ? workspace_size : (size_t)0, space.total());
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  char* const ws = static_cast<char*>(workspace);
   Product P{};
   P.a = x;
   P.b = w;
   P.lda = P.ldb = k;
+  if (space.x) {
+    const int rc = run_widen(Widen{{x, w}, {ws, ws + space.x}, {m, n}, (int)k, (int)widened(k)}, s);
+    if (rc != FWDMI_OK) return rc;
+    P.a = ws;
+    P.b = ws + space.x;
+    P.lda = P.ldb = widened(k);
+  }
   P.ni = (int)m;
   P.nj = (int)n;
   P.nt = (int)k;
@@ -152,7 +217,7 @@ int fwdmi_linear(void* stream, int64_t m, int64_t n, int64_t k, const void* x, c
   P.bias = bias;
   P.residual = residual;
   P.act = act;
-  return run(P, 0, dtype, workspace, static_cast<hipStream_t>(stream));
+  return run(P, 0, dtype, ws + space.x + space.w, s);
 }
 
 size_t fwdmi_linear_backward_workspace(int64_t m, int64_t n, int64_t k, int32_t act, int32_t dtype) {
@@ -183,14 +248,16 @@ int fwdmi_linear_backward(void* stream, int64_t m, int64_t n, int64_t k, const v
   const int parts = any ? slope_parts(m, n) : 0;
   const void* dz = dy;
   int rc = FWDMI_OK;
-  if (any && (act != FWDMI_ACT_NONE || dbias)) {
+  const bool products = k > 0 && (dx || dw);
+  if (any && ((space.dz && products) || dbias)) {
     Slope S{};
     S.dy = dy;
-    if (act != FWDMI_ACT_NONE) {
-      S.z = preact;
+    if (act != FWDMI_ACT_NONE) S.z = preact;
+    if (space.dz && products) {
       S.dz = ws;
       dz = ws;
     }
+    S.ld_dz = (int)space.ld_dz;
     S.part = dbias ? reinterpret_cast<float*>(ws + space.dz) : nullptr;
     S.m = m;
     S.n = (int)n;
@@ -210,11 +277,21 @@ int fwdmi_linear_backward(void* stream, int64_t m, int64_t n, int64_t k, const v
     rc = launch_column_sums(C, s);
     if (rc != FWDMI_OK) return rc;
   }
-  void* const partial = ws + space.dz + space.part;
+  char* const wide = ws + space.dz + space.part;
+  void* const partial = wide + space.x + space.w;
   Product P{};
   P.a = dz;
-  P.lda = n;
+  P.lda = space.ld_dz;
   P.ldb = k;
+  if (space.x && products) {
+    rc = dx && dw ? run_widen(Widen{{x, w}, {wide, wide + space.x}, {m, n}, (int)k, (int)widened(k)}, s)
+         : dw     ? run_widen(Widen{{x, nullptr}, {wide, nullptr}, {m, 0}, (int)k, (int)widened(k)}, s)
+                  : run_widen(Widen{{w, nullptr}, {wide + space.x, nullptr}, {n, 0}, (int)k, (int)widened(k)}, s);
+    if (rc != FWDMI_OK) return rc;
+    x = wide;
+    w = wide + space.x;
+    P.ldb = widened(k);
+  }
   P.nj = (int)k;
   if (dx && m > 0 && k > 0) {  // (n == 0: an empty sum, zeros)
     P.b = w;

@@ -177,7 +177,7 @@ struct Tile {
 };
 
 // Loads of one operand's tile by NT threads: ROWS rows from row `row0` on, steps of t from `step0` on.
-// DIRECT: memory to LDS, whole steps only (`count` of them, then nothing); else through registers, two sets of them.
+// DIRECT: memory to LDS, `left` steps and then nothing; else through registers, two sets of them.
 template <typename T, int ROWS, int LAYOUT, int STEP, int NT, bool DIRECT>
 struct Loader {
   using Tl = Tile<T, ROWS, LAYOUT, STEP>;
@@ -185,15 +185,19 @@ struct Loader {
   static_assert(Tl::kBytes % (16 * NT) == 0, "whole loads");
   const T FWDMI_GLOBAL* base;  // the tile's first element in the present step
   int64_t ld, step_elems;
-  int rows, left;  // rows of the tile that exist; DIRECT: whole steps left, else elements of t left
+  int rows, left;  // rows of the tile that exist; steps left
+  int t_left;      // elements of t left (of the whole matrix, DIRECT, or of the split)
+  int partial;     // DIRECT: the value of `left` at which a step is the matrix's last and partial, 0 for never
+  uint32_t bytes;  // DIRECT: from `base` to the end of what a step may read
   int line[kLoads], chunk[kLoads];
   uint32_t offset[DIRECT ? kLoads : 1];
   Pack<T, kChunk<T>> held[DIRECT ? 1 : 2][DIRECT ? 1 : kLoads];
 
-  __device__ __forceinline__ Loader(const void* p, int64_t ld_, int row0, int n_rows, int step0, int left_) {
+  __device__ __forceinline__ Loader(const void* p, int64_t ld_, int row0, int n_rows, int step0, int left_, int t_left_) {
     ld = ld_;
     rows = min(n_rows - row0, ROWS);
     left = left_;
+    t_left = t_left_;
     const int64_t t0 = (int64_t)step0 * Tl::kT;
     base = gconst<T>(p) + (LAYOUT == kAlong ? row0 * ld + t0 : t0 * ld + row0);
     step_elems = LAYOUT == kAlong ? Tl::kT : Tl::kT * ld;
@@ -202,24 +206,39 @@ struct Loader {
       Tl::locate(i * NT + (int)threadIdx.x, line[i], chunk[i]);
       if (DIRECT) offset[i] = (uint32_t)(line[i] * (uint32_t)(ld * sizeof(T)) + chunk[i] * 16);
     }
+    if (DIRECT) {
+      bytes = readable(Tl::kT);
+      partial = left * Tl::kT > t_left ? 1 : 0;
+    }
   }
 
   // ---- DIRECT
+  // Bytes from `base` to the end of what a step with t elements of t may read; past it buffer loads give zeros and touch
+  // nothing.  (The last chunk of a line may reach past the rows or past t: into zeros, or into the next line, `tail_of`.)
+  __device__ __forceinline__ uint32_t readable(int t) const {
+    constexpr int kC = kChunk<T>;
+    const uint32_t lines = LAYOUT == kAlong ? rows : t, last = ((LAYOUT == kAlong ? t : rows) + kC - 1) / kC * kC;
+    return ((lines - 1) * (uint32_t)ld + last) * (uint32_t)sizeof(T);
+  }
   __device__ __forceinline__ void load(char* lds) {
     load_part<0, kLoads>(lds);
     advance();
   }
   __device__ __forceinline__ void advance() {
     base += step_elems;
+    t_left -= Tl::kT;
     --left;
   }
   template <int FIRST, int COUNT>
   __device__ __forceinline__ void load_part(char* lds) {
-    // Bytes from `base` to the end of what the step may read; past it buffer loads give zeros and touch nothing.
-    // (kAcross: the last chunk of a line may reach into the next line, which exists: see `tail_of`.)
-    const uint32_t lines = LAYOUT == kAlong ? rows : Tl::kT;
-    const uint32_t last = LAYOUT == kAlong ? Tl::kT : (rows + kChunk<T> - 1) / kChunk<T> * kChunk<T>;
-    const uint32_t bytes = left > 0 ? ((lines - 1) * (uint32_t)ld + last) * (uint32_t)sizeof(T) : 0;
+    // Few scalar instructions: a wave's loads wait for them at the head of every step.
+    if (left == partial) {  // also past the end, where there is nothing to read
+      bytes = left > 0 ? readable(t_left) : 0;
+      if (LAYOUT == kAlong)  // a chunk past the end of t would be the next row's beginning
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) offset[i] = chunk[i] * kChunk<T> < t_left ? offset[i] : 0x80000000u;
+      partial = 0;
+    }
     const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, (int)bytes, 0x00020000);
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
 #pragma unroll
@@ -229,15 +248,19 @@ struct Loader {
   }
 
   // ---- through registers
-  // Chunk i of a step that has `t_left` elements of t, element by element, zeros where nothing exists.
+  // Chunk i of a step that has `t_left` elements of t, zeros where nothing exists.
   __device__ __forceinline__ Pack<T, kChunk<T>> some(int i, int t_left) const {
     const int r = LAYOUT == kAlong ? line[i] : chunk[i] * kChunk<T>;
     const int t = LAYOUT == kAlong ? chunk[i] * kChunk<T> : line[i];
     const int n = r < rows && t < t_left ? (LAYOUT == kAlong ? t_left - t : rows - r) : 0;
     const T FWDMI_GLOBAL* const at = base + (n > 0 ? (int64_t)line[i] * ld + chunk[i] * kChunk<T> : 0);
     Pack<T, kChunk<T>> v;
+    if (n >= kChunk<T>) {
+      v = load_slice<T, kChunk<T>>(at);
+    } else {
 #pragma unroll
-    for (int e = 0; e < kChunk<T>; ++e) v.v[e] = e < n ? at[e] : (T)0.0f;
+      for (int e = 0; e < kChunk<T>; ++e) v.v[e] = e < n ? at[e] : (T)0.0f;
+    }
     return v;
   }
   __device__ __forceinline__ void put(char* lds, int i, const Pack<T, kChunk<T>>& v) const {
@@ -247,8 +270,8 @@ struct Loader {
   __device__ __forceinline__ void fetch() {
     // A step whose loads all lie inside the matrix takes them whole: rows past the tile's last repeat one (nobody
     // reads their products), a line's last chunk may reach up to a chunk less one element into the lines behind it.
-    const bool whole = left >= Tl::kT && (LAYOUT == kAlong || rows % kChunk<T> == 0 ||
-                                          (int64_t)(left - Tl::kT) * ld >= kChunk<T> - 1);
+    const bool whole = t_left >= Tl::kT && (LAYOUT == kAlong || rows % kChunk<T> == 0 ||
+                                            (int64_t)(t_left - Tl::kT) * ld >= kChunk<T> - 1);
     if (whole) {
       const int most = LAYOUT == kAlong ? rows - 1 : (rows + kChunk<T> - 1) / kChunk<T> - 1;
 #pragma unroll
@@ -256,12 +279,12 @@ struct Loader {
         const int l = LAYOUT == kAlong ? min(line[i], most) : line[i], c = LAYOUT == kAlong ? chunk[i] : min(chunk[i], most);
         held[SET][i] = load_slice<T, kChunk<T>>(base + (int64_t)l * ld + c * kChunk<T>);
       }
-    } else if (left > 0) {
+    } else if (t_left > 0) {
 #pragma unroll
-      for (int i = 0; i < kLoads; ++i) held[SET][i] = some(i, left);
+      for (int i = 0; i < kLoads; ++i) held[SET][i] = some(i, t_left);
     }
     base += step_elems;
-    left -= Tl::kT;
+    t_left -= Tl::kT;
   }
   template <int SET>
   __device__ __forceinline__ void drop(char* lds) const {
@@ -550,8 +573,8 @@ __global__ __launch_bounds__(64 * WI * WJ * WK) void product_kernel(const Produc
     }
   };
   if constexpr (DIRECT) {
-    LoadA la(P.a, P.lda, i0, P.ni, steps.first, steps.whole);
-    LoadB lb(P.b, P.ldb, j0, P.nj, steps.first, steps.whole);
+    LoadA la(P.a, P.lda, i0, P.ni, steps.first, steps.whole, P.nt - steps.first * TileA::kT);
+    LoadB lb(P.b, P.ldb, j0, P.nj, steps.first, steps.whole, P.nt - steps.first * TileB::kT);
     // STAGES - 1 steps of loads are in flight; steps past the end load nothing (every lane out of range) so that the
     // number in flight is always the same
     constexpr int kAhead = (STAGES - 2) * (LoadA::kLoads + LoadB::kLoads);
@@ -586,8 +609,8 @@ __global__ __launch_bounds__(64 * WI * WJ * WK) void product_kernel(const Produc
     }
   } else if (const int n = steps.whole + (steps.tail > 0 ? 1 : 0); n > 0) {
     const int t = steps.whole * TileA::kT + steps.tail;
-    LoadA la(P.a, P.lda, i0, P.ni, steps.first, t);
-    LoadB lb(P.b, P.ldb, j0, P.nj, steps.first, t);
+    LoadA la(P.a, P.lda, i0, P.ni, steps.first, n, t);
+    LoadB lb(P.b, P.ldb, j0, P.nj, steps.first, n, t);
     // registers hold the two steps after the one being multiplied
     la.template fetch<0>();
     lb.template fetch<0>();
@@ -653,8 +676,8 @@ __global__ __launch_bounds__(512) void product_turns_kernel(const Product P) {
 #pragma unroll
     for (int i = 0; i < kFI; ++i) acc[j][i] = F4{0.0f, 0.0f, 0.0f, 0.0f};
 
-  LoadA la(P.a, P.lda, i0, P.ni, steps.first, steps.whole);
-  LoadB lb(P.b, P.ldb, j0, P.nj, steps.first, steps.whole);
+  LoadA la(P.a, P.lda, i0, P.ni, steps.first, steps.whole, P.nt - steps.first * TileA::kT);
+  LoadB lb(P.b, P.ldb, j0, P.nj, steps.first, steps.whole, P.nt - steps.first * TileB::kT);
   const Reader<T, TI, LA, STEP, kFI> ra(wi);
   const Reader<T, TJ, LB, STEP, kFJ> rb(wj);
   // (steps past the end load nothing, every lane out of range, so that the number in flight is always the same)
@@ -877,12 +900,13 @@ __global__ __launch_bounds__(256) void slope_kernel(const Slope S) {
         out.v[e] = (T)v;
       }
       if (S.dz) {
-        if (live == kVec) {
-          store_slice<T, kVec>(gmut<T>(S.dz) + at, out);
+        T FWDMI_GLOBAL* const to = gmut<T>(S.dz) + r * S.ld_dz + c;
+        if (c + kVec <= S.ld_dz) {  // (elements past n come out as zeros)
+          store_slice<T, kVec>(to, out);
         } else {
 #pragma unroll
           for (int e = 0; e < kVec; ++e)
-            if (e < live) gmut<T>(S.dz)[at + e] = out.v[e];
+            if (e < live) to[e] = out.v[e];
         }
       }
     }

@@ -19,7 +19,7 @@ struct Product {
   int64_t lda, ldb;
   int32_t ni, nj, nt;
   int32_t whole_steps, tail;  // t as steps of a tile's depth and the elements that are left (`tail_of`)
-  int32_t steps_per_split;    // of whole_steps (+ 1 for the tail) that one of gridDim.y splits walks
+  int32_t steps_per_split;    // of whole_steps (+ 1 for the tail) that one split walks
   float* partial;           // not null: C goes there unfinished, [split][ni][nj]
   void* c;                  // [ni, nj]
   void* preact;             // nullable
@@ -33,10 +33,10 @@ struct Product {
 struct Slope {
   const void* dy;
   const void* z;   // nullable: dz = dy, only summed
-  void* dz;
+  void* dz;        // nullable; lines of ld_dz elements, zeros past n
   float* part;     // nullable: [gridDim.y][n] column sums of fp32 dz, before its rounding
   int64_t m;
-  int32_t n;
+  int32_t n, ld_dz;
   int32_t act;
 };
 
@@ -52,6 +52,15 @@ constexpr TileShape kTiles[kTileKinds] = {{256, 256, 128}, {256, 128, 128}, {128
 struct Plan {
   TileKind tile;
   int splits, whole_steps, tail, steps_per_split;
+  double us;  // estimate
+};
+
+// Copies of up to two matrices with lines of `ld_out` elements, a multiple of 8, zeros past the `ld` of the source.
+struct Widen {
+  const void* in[2];
+  void* out[2];
+  int64_t lines[2];
+  int32_t ld, ld_out;
 };
 
 inline int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
@@ -61,13 +70,16 @@ inline bool direct_ok(const void* p, int64_t ld, int elem) {
   return reinterpret_cast<uintptr_t>(p) % 4 == 0 && ld * elem % 4 == 0 && ld >= 8 && ld * elem <= (int64_t)1 << 22;
 }
 
-// t as whole steps of `depth` elements and a tail that is loaded element by element.  Direct loads of lines across t
-// take whole chunks, of which a line's last may reach into the next line: where rows do not fill their chunks (`ragged`)
-// the matrix's last line has to be in the tail, so that a line is behind every one that is loaded whole.
-inline void tail_of(int nt, int depth, bool ragged, int& whole, int& tail) {
-  whole = nt / depth;
-  tail = nt % depth;
-  if (ragged && tail == 0 && whole > 0) {
+// How the end of t is loaded.  kWhole: every chunk that begins inside t is loaded whole, the last step like the others
+// (t is a multiple of a chunk, or the lines are zeros from its end to the chunk's).  kTail: the elements past the last
+// whole step go through registers.  kTailLine: so does at least the matrix's last line, because rows across t end
+// inside a chunk and a line's last chunk reaches into the line behind it.
+enum End { kWhole, kTail, kTailLine };
+
+inline void tail_of(int nt, int depth, End end, int& whole, int& tail) {
+  whole = end == kWhole ? ceil_div(nt, depth) : nt / depth;
+  tail = end == kWhole ? 0 : nt % depth;
+  if (end == kTailLine && tail == 0 && whole > 0) {
     --whole;
     tail = depth;
   }
@@ -78,6 +90,7 @@ inline void tail_of(int nt, int depth, bool ragged, int& whole, int& tail) {
 int run_product_f16(Product& P, int layouts, const Plan& plan, bool direct, hipStream_t stream);
 int run_product_bf16(Product& P, int layouts, const Plan& plan, bool direct, hipStream_t stream);
 int run_product_f32(Product& P, int layouts, const Plan& plan, bool direct, hipStream_t stream);
+int run_widen(const Widen& W, hipStream_t stream);  // 16-bit elements of either type
 int run_slope_f16(const Slope& S, int parts, hipStream_t stream);
 int run_slope_bf16(const Slope& S, int parts, hipStream_t stream);
 int run_slope_f32(const Slope& S, int parts, hipStream_t stream);

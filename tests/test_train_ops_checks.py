@@ -98,12 +98,12 @@ def test_linear_launchers_refuse():
     assert d.fwdmi_linear(None, 4, 8, 1 << 40, *none6, 0, lib.F16, None, 0) == lib.ERR_BAD_ARG
     assert d.fwdmi_linear(None, 4, 8, 16, *none6, 0, lib.F16, None, 0) == lib.ERR_BAD_ARG            # null pointers
     assert d.fwdmi_linear(None, 0, 8, 16, *none6, 0, lib.F16, None, 0) == lib.OK                     # nothing to do
-    need = d.fwdmi_linear_workspace(16, 64, 1 << 16, lib.F16)
+    need = d.fwdmi_linear_workspace(64, 64, 1 << 16, lib.F16)
     assert need > 0                                                                                # a long sum is split
     some = [64, 64, None, None, 64, None]
-    assert d.fwdmi_linear(None, 16, 64, 1 << 16, *some, 0, lib.F16, 64, need - 1) == lib.ERR_BAD_ARG
+    assert d.fwdmi_linear(None, 64, 64, 1 << 16, *some, 0, lib.F16, 64, need - 1) == lib.ERR_BAD_ARG
     assert "workspace" in lib.last_error()
-    assert d.fwdmi_linear(None, 16, 64, 1 << 16, *some, 0, lib.F16, 72, need) == lib.ERR_BAD_ARG     # off its boundary
+    assert d.fwdmi_linear(None, 64, 64, 1 << 16, *some, 0, lib.F16, 72, need) == lib.ERR_BAD_ARG     # off its boundary
     none7 = [None] * 7
     assert d.fwdmi_linear_backward(None, 4, 8, 16, *none7, 0, lib.BOOL, None, 0) == lib.ERR_UNSUPPORTED
     assert d.fwdmi_linear_backward(None, 4, 8, 16, *none7, 0, lib.F16, None, 0) == lib.ERR_BAD_ARG
