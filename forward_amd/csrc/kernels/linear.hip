@@ -24,9 +24,15 @@ struct Operands {
 // 8192 x 1024 x 4096 (b across) 66 us with 256 x 128, 81 with 128 x 128;
 // 4096 x 1024 x 8192 (both across) 63 us and 15 to add four splits with 256 x 256, 72 and 9 with 256 x 128 and two; 384 x 1024 x 4096 12 us with 64 x 32, 15 with 64 x 64,
 // 20 and more with 128 x 128.
+const double kRate[2][kTileKinds] = {{6.0e6, 4.6e6, 4.0e6, 3.5e6, 3.0e6}, {6.0e6, 4.3e6, 2.2e6, 3.5e6, 3.0e6}};
+const double kRound[kTileKinds] = {9.0, 4.0, 3.0, 1.5, 1.0};
+double step_us(TileKind kind, const Operands& o) {
+  const TileShape t = kTiles[kind];
+  const double load = (t.ti + t.tj) * t.step_bytes / ((o.direct ? 90.0 : 40.0) * 1024);
+  const double flops = 2.0 * t.ti * t.tj * (t.step_bytes / o.elem) / (o.elem == 2 ? kRate[o.layouts == 2][kind] : 0.47e6);
+  return std::max(load, flops);
+}
 Plan make_plan(int ni, int nj, int nt, const Operands& o) {
-  static const double kRate[2][kTileKinds] = {{6.0e6, 4.6e6, 4.0e6, 3.5e6, 3.0e6}, {6.0e6, 4.3e6, 2.2e6, 3.5e6, 3.0e6}};
-  static const double kRound[kTileKinds] = {9.0, 4.0, 3.0, 1.5, 1.0};
   if (o.layouts == 0 && ni <= kFewRows) return Plan{kFew, 1, 0, 0, 0, 0.0};
   const int cus = device_cus();
   Plan best{};
@@ -37,9 +43,7 @@ Plan make_plan(int ni, int nj, int nt, const Operands& o) {
     tail_of(nt, t.step_bytes / o.elem, o.end, p.whole_steps, p.tail);
     const int all = p.whole_steps + (p.tail > 0);
     const int64_t tiles = (int64_t)ceil_div(ni, t.ti) * ceil_div(nj, t.tj);
-    const double load = (t.ti + t.tj) * t.step_bytes / ((o.direct ? 90.0 : 40.0) * 1024);
-    const double flops = 2.0 * t.ti * t.tj * (t.step_bytes / o.elem) / (o.elem == 2 ? kRate[o.layouts == 2][kind] : 0.47e6);
-    const double step = std::max(load, flops);
+    const double step = step_us((TileKind)kind, o);
     for (int target = 0; target <= 2; ++target) {  // one workgroup per tile, or splits for one or two per CU
       const int64_t want = target == 0 ? 1 : target * (int64_t)cus / tiles;
       if (target > 0 && want < 2) continue;
@@ -70,15 +74,54 @@ End end_of(int layouts, int ni, int nj, int nt, int64_t lda, int64_t ldb, int el
   return (layouts <= 1 && part(nt, lda)) || (layouts == 0 && part(nt, ldb)) ? kTail : kWhole;
 }
 
-int run(Product& P, int layouts, int dtype, void* workspace, hipStream_t stream) {
-  const int elem = dtype == FWDMI_F32 ? 4 : 2;
+Operands operands_of(const Product& P, int layouts, int elem) {
   const bool direct = direct_ok(P.a, P.lda, elem) && direct_ok(P.b, P.ldb, elem);
-  const Operands o{layouts, elem, direct, direct ? end_of(layouts, P.ni, P.nj, P.nt, P.lda, P.ldb, elem) : kTail};
+  return Operands{layouts, elem, direct, direct ? end_of(layouts, P.ni, P.nj, P.nt, P.lda, P.ldb, elem) : kTail};
+}
+
+int elem_size(int dtype) { return dtype == FWDMI_F32 ? 4 : 2; }
+
+int run(Product& P, int layouts, int dtype, void* workspace, hipStream_t stream) {
+  const Operands o = operands_of(P, layouts, elem_size(dtype));
   const Plan plan = make_plan(P.ni, P.nj, P.nt, o);
   P.partial = plan.splits > 1 ? static_cast<float*>(workspace) : nullptr;
-  return dtype == FWDMI_F16    ? run_product_f16(P, layouts, plan, direct, stream)
-         : dtype == FWDMI_BF16 ? run_product_bf16(P, layouts, plan, direct, stream)
-                               : run_product_f32(P, layouts, plan, direct, stream);
+  return dtype == FWDMI_F16    ? run_product_f16(P, layouts, plan, o.direct, stream)
+         : dtype == FWDMI_BF16 ? run_product_bf16(P, layouts, plan, o.direct, stream)
+                               : run_product_f32(P, layouts, plan, o.direct, stream);
+}
+
+// Fills in P as one unsplit pass over 64 x 64 tiles; returns the number of tiles.
+int64_t whole_tiles(Product& P, const Operands& o) {
+  const TileShape t = kTiles[k64x64];
+  tail_of(P.nt, t.step_bytes / o.elem, o.end, P.whole_steps, P.tail);
+  P.steps_per_split = P.whole_steps + (P.tail > 0);
+  P.tiles_i = ceil_div(P.ni, t.ti);
+  P.tiles_j = ceil_div(P.nj, t.tj);
+  return (int64_t)P.tiles_i * P.tiles_j;
+}
+
+// Whether both products of a gradient are faster in one launch of unsplit 64 x 64 tiles than in launches of their own
+// (whose gap is about 3 us), and if so that launch, but for dbias.  771 x 1011 x 768 fp16: 10 and 8 us apart.
+bool together(const Product& x, const Product& w, int dtype, Gradients& G, bool& direct) {
+  const int elem = elem_size(dtype);
+  Operands ox = operands_of(x, 1, elem), ow = operands_of(w, 2, elem);
+  const double apart = make_plan(x.ni, x.nj, x.nt, ox).us + make_plan(w.ni, w.nj, w.nt, ow).us + 3.0;
+  direct = ox.direct && ow.direct;
+  if (!direct) {
+    ox.direct = ow.direct = false;
+    ox.end = ow.end = kTail;
+  }
+  G.x = x;
+  G.w = w;
+  const int64_t tx = whole_tiles(G.x, ox), tw = whole_tiles(G.w, ow);
+  const int sx = G.x.steps_per_split, sw = G.w.steps_per_split;
+  const int cus = device_cus();
+  const double rounds = (double)ceil_div(tx + tw, cus);
+  const double steps = std::max<double>(std::max(sx, sw), ((double)tx * sx + (double)tw * sw) / cus);
+  if (2.0 + rounds * kRound[k64x64] + steps * step_us(k64x64, ow) >= apart) return false;
+  G.blocks_x = (int)tx;
+  G.blocks_w = (int)tw;
+  return true;
 }
 
 // Partial products of any plan that `run` may choose for these sizes (that depends on the operands' alignment too).
@@ -92,7 +135,6 @@ size_t product_bytes(int layouts, int64_t ni, int64_t nj, int64_t nt, int elem) 
   return bytes;
 }
 
-int elem_size(int dtype) { return dtype == FWDMI_F32 ? 4 : 2; }
 size_t align256(size_t v) { return (v + 255) / 256 * 256; }
 int64_t widened(int64_t ld) { return (ld + 7) / 8 * 8; }
 
@@ -246,30 +288,63 @@ int fwdmi_linear_backward(void* stream, int64_t m, int64_t n, int64_t k, const v
   hipStream_t s = static_cast<hipStream_t>(stream);
   char* const ws = static_cast<char*>(workspace);
   const int parts = any ? slope_parts(m, n) : 0;
-  const void* dz = dy;
+  float* const part = reinterpret_cast<float*>(ws + space.dz);
+  char* const wide = ws + space.dz + space.part;
+  void* const partial = wide + space.x + space.w;
+  dx = m > 0 && k > 0 ? dx : nullptr;  // (n == 0 leaves zeros: an empty sum)
+  dw = n > 0 && k > 0 ? dw : nullptr;  // (m == 0 likewise)
+  const bool copy = space.dz && (dx || dw), widen = space.x && (dx || dw);
+  Product X{}, W{};
+  X.a = W.a = copy ? ws : dy;
+  X.lda = W.lda = space.ld_dz;
+  X.b = widen ? wide + space.x : w;
+  W.b = widen ? wide : x;
+  X.ldb = W.ldb = widen ? widened(k) : k;
+  X.ni = W.nt = (int)m;
+  X.nt = W.ni = (int)n;
+  X.nj = W.nj = (int)k;
+  X.c = dx;
+  W.c = dw;
+  Gradients G{};
+  bool direct = false;
+  const bool joint = any && dx && dw && together(X, W, dtype, G, direct);
+  // few rows are summed straight from dy by the joint launch
+  const bool sum_dy = joint && act == FWDMI_ACT_NONE && !copy && m <= 1024;
   int rc = FWDMI_OK;
-  const bool products = k > 0 && (dx || dw);
-  if (any && ((space.dz && products) || dbias)) {
+  if (any && (copy || (dbias && !sum_dy))) {
     Slope S{};
     S.dy = dy;
-    if (act != FWDMI_ACT_NONE) S.z = preact;
-    if (space.dz && products) {
-      S.dz = ws;
-      dz = ws;
-    }
-    S.ld_dz = (int)space.ld_dz;
-    S.part = dbias ? reinterpret_cast<float*>(ws + space.dz) : nullptr;
+    S.z = act != FWDMI_ACT_NONE ? preact : nullptr;
+    S.dz = copy ? ws : nullptr;
+    S.part = dbias ? part : nullptr;
     S.m = m;
     S.n = (int)n;
+    S.ld_dz = (int)space.ld_dz;
     S.act = act;
     rc = dtype == FWDMI_F16    ? run_slope_f16(S, parts, s)
          : dtype == FWDMI_BF16 ? run_slope_bf16(S, parts, s)
                                : run_slope_f32(S, parts, s);
     if (rc != FWDMI_OK) return rc;
   }
+  if (widen) {
+    rc = dx && dw ? run_widen(Widen{{x, w}, {wide, wide + space.x}, {m, n}, (int)k, (int)widened(k)}, s)
+         : dw     ? run_widen(Widen{{x, nullptr}, {wide, nullptr}, {m, 0}, (int)k, (int)widened(k)}, s)
+                  : run_widen(Widen{{w, nullptr}, {wide + space.x, nullptr}, {n, 0}, (int)k, (int)widened(k)}, s);
+    if (rc != FWDMI_OK) return rc;
+  }
+  if (joint) {
+    G.dbias = dbias;
+    G.part = sum_dy ? nullptr : part;
+    G.dy = dy;
+    G.parts = sum_dy ? m : parts;
+    G.n = (int)n;
+    return dtype == FWDMI_F16    ? run_gradients_f16(G, direct, s)
+           : dtype == FWDMI_BF16 ? run_gradients_bf16(G, direct, s)
+                                 : run_gradients_f32(G, direct, s);
+  }
   if (dbias && n > 0) {
     ColumnSums C{};
-    C.part = reinterpret_cast<const float*>(ws + space.dz);
+    C.part = part;
     C.out[0] = dbias;
     C.parts = parts;
     C.ld = (int)n;
@@ -277,38 +352,11 @@ int fwdmi_linear_backward(void* stream, int64_t m, int64_t n, int64_t k, const v
     rc = launch_column_sums(C, s);
     if (rc != FWDMI_OK) return rc;
   }
-  char* const wide = ws + space.dz + space.part;
-  void* const partial = wide + space.x + space.w;
-  Product P{};
-  P.a = dz;
-  P.lda = space.ld_dz;
-  P.ldb = k;
-  if (space.x && products) {
-    rc = dx && dw ? run_widen(Widen{{x, w}, {wide, wide + space.x}, {m, n}, (int)k, (int)widened(k)}, s)
-         : dw     ? run_widen(Widen{{x, nullptr}, {wide, nullptr}, {m, 0}, (int)k, (int)widened(k)}, s)
-                  : run_widen(Widen{{w, nullptr}, {wide + space.x, nullptr}, {n, 0}, (int)k, (int)widened(k)}, s);
-    if (rc != FWDMI_OK) return rc;
-    x = wide;
-    w = wide + space.x;
-    P.ldb = widened(k);
-  }
-  P.nj = (int)k;
-  if (dx && m > 0 && k > 0) {  // (n == 0: an empty sum, zeros)
-    P.b = w;
-    P.ni = (int)m;
-    P.nt = (int)n;
-    P.c = dx;
-    rc = run(P, 1, dtype, partial, s);
+  if (dx) {
+    rc = run(X, 1, dtype, partial, s);
     if (rc != FWDMI_OK) return rc;
   }
-  if (dw && n > 0 && k > 0) {
-    P.b = x;
-    P.ni = (int)n;
-    P.nt = (int)m;
-    P.c = dw;
-    rc = run(P, 2, dtype, partial, s);
-  }
-  return rc;
+  return dw ? run(W, 2, dtype, partial, s) : FWDMI_OK;
 }
 
 }  // extern "C"

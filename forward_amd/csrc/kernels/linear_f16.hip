@@ -34,6 +34,7 @@ int run_widen(const Widen& W, hipStream_t stream) {
 int run_product_f16(Product& P, int layouts, const Plan& plan, bool direct, hipStream_t stream) {
   return run_product<_Float16>(P, layouts, plan, direct, stream);
 }
+int run_gradients_f16(const Gradients& G, bool direct, hipStream_t stream) { return run_gradients<_Float16>(G, direct, stream); }
 int run_slope_f16(const Slope& S, int parts, hipStream_t stream) { return run_slope<_Float16>(S, parts, stream); }
 
 }  // namespace fwdmi

@@ -384,12 +384,12 @@ __device__ __forceinline__ Steps split_steps(const Product& P, int split) {
 // The immediate of s_waitcnt that waits until at most n vector memory operations are in flight (and for nothing else).
 constexpr int wait_loads(int n) { return (n & 15) | (n >> 4) << 14 | 0x0f70; }
 
-// The tile and split of this workgroup.  Workgroups go to the XCDs in turn, so the numbers are dealt out in eight runs
+// The tile and split of workgroup b of `total`.  Workgroups go to the XCDs in turn, so the numbers are dealt out in eight runs
 // of neighbours, one per XCD; a run stays in one split as long as it can and walks columns of at most kGroup tiles, so
 // that the tiles an XCD works on at a time share their lines of A and B in its L2.
 template <int TI, int TJ>
-__device__ __forceinline__ int locate_tile(const Product& P, int& i0, int& j0) {
-  const int tiles = P.tiles_i * P.tiles_j, total = (int)gridDim.x, b = (int)blockIdx.x;
+__device__ __forceinline__ int locate_tile(const Product& P, int b, int total, int& i0, int& j0) {
+  const int tiles = P.tiles_i * P.tiles_j;
   const int xcd = b & 7, per = total >> 3, more = total & 7;
   const int n = xcd * per + min(xcd, more) + (b >> 3);
   const int split = n / tiles, m = n - split * tiles;
@@ -534,8 +534,17 @@ __device__ __forceinline__ void leave_registers(const Product& P, const F4 (&acc
   });
 }
 
+// The work of workgroup `block` of `blocks` on product P.  The waves are WI x WJ over the tile and WK over the halves of
+// a step (their sums meet in LDS): small tiles, whose waves would otherwise have little to do between two barriers.
 template <typename T, int LA, int LB, int TI, int TJ, int WI, int WJ, int WK, int STEP, int STAGES, bool DIRECT>
-__global__ __launch_bounds__(64 * WI * WJ * WK) void product_kernel(const Product P) {
+struct Work {
+  static constexpr int kThreads = 64 * WI * WJ * WK;
+  static constexpr int kRoom = STAGES * (TI + TJ) * STEP;  // bytes of LDS
+  __device__ static __forceinline__ void run(const Product& P, char* s_tile, int block, int blocks);
+};
+template <typename T, int LA, int LB, int TI, int TJ, int WI, int WJ, int WK, int STEP, int STAGES, bool DIRECT>
+__device__ __forceinline__ void Work<T, LA, LB, TI, TJ, WI, WJ, WK, STEP, STAGES, DIRECT>::run(const Product& P, char* s_tile,
+                                                                                               int block, int blocks) {
   constexpr int kNT = 64 * WI * WJ * WK;
   constexpr int kFI = TI / WI / 16, kFJ = TJ / WJ / 16, kHalves = STEP / 64 / WK;
   using TileA = Tile<T, TI, LA, STEP>;
@@ -544,10 +553,9 @@ __global__ __launch_bounds__(64 * WI * WJ * WK) void product_kernel(const Produc
   using LoadB = Loader<T, TJ, LB, STEP, kNT, DIRECT>;
   static_assert(DIRECT || STAGES == 2, "registers hold one step");
   constexpr int kBuffer = TileA::kBytes + TileB::kBytes;  // one step of both operands
-  __shared__ __attribute__((aligned(1024))) char s_tile[STAGES * kBuffer];
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   int i0, j0;
-  const int split = locate_tile<TI, TJ>(P, i0, j0);
+  const int split = locate_tile<TI, TJ>(P, block, blocks, i0, j0);
   const int wi = wave % WI * (TI / WI), wj = wave / WI % WJ * (TJ / WJ), wk = wave / (WI * WJ);
 
   const Steps steps = split_steps(P, split);
@@ -638,6 +646,33 @@ __global__ __launch_bounds__(64 * WI * WJ * WK) void product_kernel(const Produc
   leave_tile<T, TI, TJ, WI, WJ, WK, STAGES * kBuffer, LA == kAlong && LB == kAlong>(P, acc, s_tile, i0, j0, split);
 }
 
+template <typename W>
+__global__ __launch_bounds__(W::kThreads) void product_kernel(const Product P) {
+  __shared__ __attribute__((aligned(1024))) char s_tile[W::kRoom];
+  W::run(P, s_tile, (int)blockIdx.x, (int)gridDim.x);
+}
+
+// Both products of a small gradient and dbias in one launch: workgroups of dx, of dw, and of 64 columns of dbias each.
+template <typename T, bool DIRECT>
+__global__ __launch_bounds__(512) void gradients_kernel(const Gradients G) {
+  using X = Work<T, kAlong, kAcross, 64, 64, 2, 1, 4, 256, 2, DIRECT>;
+  using W = Work<T, kAcross, kAcross, 64, 64, 2, 1, 4, 256, 2, DIRECT>;
+  static_assert(X::kThreads == 512 && W::kThreads == 512 && X::kRoom == W::kRoom, "one shape of workgroup");
+  __shared__ __attribute__((aligned(1024))) char s_tile[X::kRoom];
+  const int b = (int)blockIdx.x;
+  if (b < G.blocks_x) {
+    X::run(G.x, s_tile, b, G.blocks_x);
+  } else if (b < G.blocks_x + G.blocks_w) {
+    W::run(G.w, s_tile, b - G.blocks_x, G.blocks_w);
+  } else {
+    float(*s_red)[64] = reinterpret_cast<float(*)[64]>(s_tile);
+    const int64_t c = (int64_t)(b - G.blocks_x - G.blocks_w) * 64 + (threadIdx.x & 63);
+    const float a = G.part ? column_sum<float, 8>(G.part, G.parts, G.n, c, s_red)
+                           : column_sum<T, 8>(static_cast<const T*>(G.dy), G.parts, G.n, c, s_red);
+    if (threadIdx.x < 64 && c < G.n) gmut<float>(G.dbias)[c] = a;
+  }
+}
+
 template <int... I, typename F>
 __device__ __forceinline__ void unrolled(std::integer_sequence<int, I...>, F&& f) {
   (f(std::integral_constant<int, I>{}), ...);
@@ -666,7 +701,7 @@ __global__ __launch_bounds__(512) void product_turns_kernel(const Product P) {
   __shared__ __attribute__((aligned(1024))) char s_tile[STAGES * kBuffer];
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   int i0, j0;
-  const int split = locate_tile<TI, TJ>(P, i0, j0);
+  const int split = locate_tile<TI, TJ>(P, (int)blockIdx.x, (int)gridDim.x, i0, j0);
   const int wi = wave % WI * (TI / WI), wj = wave / WI * (TJ / WJ);
   const Steps steps = split_steps(P, split);
 
@@ -950,12 +985,12 @@ int launch_product(Product& P, const Plan& plan, hipStream_t stream) {
       hipLaunchKernelGGL((product_turns_kernel<T, LA, LB, 256, 128, 4, 2, 3>), grid, dim3(512), 0, stream, P);
   }
   if (plan.tile == k128x128)
-    hipLaunchKernelGGL((product_kernel<T, LA, LB, 128, 128, 2, 2, 1, 128, 2, DIRECT>), grid, dim3(256), 0, stream, P);
+    hipLaunchKernelGGL((product_kernel<Work<T, LA, LB, 128, 128, 2, 2, 1, 128, 2, DIRECT>>), grid, dim3(256), 0, stream, P);
   if (plan.tile == k64x64)
-    hipLaunchKernelGGL((product_kernel<T, LA, LB, 64, 64, 2, 1, 4, 256, 2, DIRECT>), grid, dim3(512), 0, stream, P);
+    hipLaunchKernelGGL((product_kernel<Work<T, LA, LB, 64, 64, 2, 1, 4, 256, 2, DIRECT>>), grid, dim3(512), 0, stream, P);
   if (plan.tile == k64x32)
-    hipLaunchKernelGGL((product_kernel<T, LA, LB, 64, 32, 2, 1, 4, 256, DIRECT ? 4 : 2, DIRECT>), grid, dim3(512), 0, stream,
-                       P);
+    hipLaunchKernelGGL((product_kernel<Work<T, LA, LB, 64, 32, 2, 1, 4, 256, DIRECT ? 4 : 2, DIRECT>>), grid, dim3(512), 0,
+                       stream, P);
   FWDMI_HIP_CHECK(hipGetLastError());
   if (plan.splits > 1) {
     const int64_t octets = (int64_t)P.ni * ((P.nj + 7) / 8);
@@ -974,6 +1009,16 @@ int launch_layouts(Product& P, int layouts, const Plan& plan, hipStream_t stream
 template <typename T>
 int run_product(Product& P, int layouts, const Plan& plan, bool direct, hipStream_t stream) {
   return direct ? launch_layouts<T, true>(P, layouts, plan, stream) : launch_layouts<T, false>(P, layouts, plan, stream);
+}
+template <typename T>
+int run_gradients(const Gradients& G, bool direct, hipStream_t stream) {
+  const dim3 grid((unsigned)(G.blocks_x + G.blocks_w + (G.dbias ? ceil_div(G.n, 64) : 0)));
+  if (direct)
+    hipLaunchKernelGGL((gradients_kernel<T, true>), grid, dim3(512), 0, stream, G);
+  else
+    hipLaunchKernelGGL((gradients_kernel<T, false>), grid, dim3(512), 0, stream, G);
+  FWDMI_HIP_CHECK(hipGetLastError());
+  return FWDMI_OK;
 }
 template <typename T>
 int run_slope(const Slope& S, int parts, hipStream_t stream) {

@@ -55,6 +55,17 @@ struct Plan {
   double us;  // estimate
 };
 
+// Both products of a gradient, unsplit and in 64 x 64 tiles, and the sums of its columns.
+struct Gradients {
+  Product x, w;
+  int32_t blocks_x, blocks_w;
+  float* dbias;       // nullable
+  const float* part;  // its partials [parts][n], or
+  const void* dy;     // without partials, dy itself [parts][n]
+  int64_t parts;
+  int32_t n;
+};
+
 // Copies of up to two matrices with lines of `ld_out` elements, a multiple of 8, zeros past the `ld` of the source.
 struct Widen {
   const void* in[2];
@@ -90,6 +101,9 @@ inline void tail_of(int nt, int depth, End end, int& whole, int& tail) {
 int run_product_f16(Product& P, int layouts, const Plan& plan, bool direct, hipStream_t stream);
 int run_product_bf16(Product& P, int layouts, const Plan& plan, bool direct, hipStream_t stream);
 int run_product_f32(Product& P, int layouts, const Plan& plan, bool direct, hipStream_t stream);
+int run_gradients_f16(const Gradients& G, bool direct, hipStream_t stream);
+int run_gradients_bf16(const Gradients& G, bool direct, hipStream_t stream);
+int run_gradients_f32(const Gradients& G, bool direct, hipStream_t stream);
 int run_widen(const Widen& W, hipStream_t stream);  // 16-bit elements of either type
 int run_slope_f16(const Slope& S, int parts, hipStream_t stream);
 int run_slope_bf16(const Slope& S, int parts, hipStream_t stream);

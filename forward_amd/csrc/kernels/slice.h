@@ -37,8 +37,32 @@ __device__ __forceinline__ void store_slice(T FWDMI_GLOBAL* p, const Pack<T, N>&
   }
 }
 
-// Adds `parts` rows of partials in a fixed order: 64 columns per workgroup, its sixteen waves each take every
-// sixteenth row.  parts == 0 leaves zeros.
+// The sum over `rows` rows of column c (64 columns per workgroup, one per lane), in a fixed order: each of the WAVES waves
+// adds every WAVES-th row, eight in flight, wave 0 adds the waves' sums and returns it.
+template <typename T, int WAVES>
+__device__ __forceinline__ float column_sum(const T* part, int64_t rows, int64_t width, int64_t c, float (*s_red)[64]) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  float a = 0.0f;
+  if (c < width) {
+    const T FWDMI_GLOBAL* at = gconst<T>(part) + wave * width + c;
+    int64_t left = (rows - wave + WAVES - 1) / WAVES;  // rows of this wave
+    for (; left >= 8; left -= 8, at += 8 * WAVES * width) {
+      T v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = at[k * WAVES * width];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) a += (float)v[k];
+    }
+    for (; left > 0; --left, at += WAVES * width) a += (float)*at;
+  }
+  s_red[wave][lane] = a;
+  __syncthreads();
+  if (wave == 0)
+    for (int k = 1; k < WAVES; ++k) a += s_red[k][lane];
+  return a;
+}
+
+// Adds `parts` rows of partials; parts == 0 leaves zeros.
 struct ColumnSums {
   const float* part;  // [parts][kinds * ld]
   float* out[3];      // [ld] each
@@ -47,26 +71,9 @@ struct ColumnSums {
 constexpr int kSumWaves = 16;
 __global__ __launch_bounds__(64 * kSumWaves) void column_sums_kernel(const ColumnSums S) {
   __shared__ float s_red[kSumWaves][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t width = (int64_t)S.kinds * S.ld;
-  const int64_t c = (int64_t)blockIdx.x * 64 + lane;
-  float a = 0.0f;
-  if (c < width) {
-    const float FWDMI_GLOBAL* at = gconst<float>(S.part) + wave * width + c;
-    int left = (S.parts - wave + kSumWaves - 1) / kSumWaves;  // rows of this wave
-    for (; left >= 8; left -= 8, at += 8 * kSumWaves * width) {  // eight in flight, added in row order
-      float v[8];
-#pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] = at[k * kSumWaves * width];
-#pragma unroll
-      for (int k = 0; k < 8; ++k) a += v[k];
-    }
-    for (; left > 0; --left, at += kSumWaves * width) a += *at;
-  }
-  s_red[wave][lane] = a;
-  __syncthreads();
-  if (wave == 0 && c < width) {
-    for (int k = 1; k < kSumWaves; ++k) a += s_red[k][lane];
+  const int64_t width = (int64_t)S.kinds * S.ld, c = (int64_t)blockIdx.x * 64 + (threadIdx.x & 63);
+  const float a = column_sum<float, kSumWaves>(S.part, S.parts, width, c, s_red);
+  if (threadIdx.x < 64 && c < width) {
     const int kind = (int)(c / S.ld);
     float* const out = kind == 0 ? S.out[0] : kind == 1 ? S.out[1] : S.out[2];
     gmut<float>(out)[c - (int64_t)kind * S.ld] = a;
