@@ -687,11 +687,12 @@ __device__ __forceinline__ void unrolled(std::integer_sequence<int, I...>, F&& f
 // have read that buffer's last fragments (those reads are waited for in front of the multiplications they feed), and every
 // wave waits for its own in the last phase, in front of the barrier behind which the first waves read them.  With
 // three buffers (256 x 128, 144 KB) the loads of the step after next go out in phase 1 and have a whole step more.
-template <typename T, int LA, int LB, int TI, int TJ, int WI, int WJ, int STAGES>
+template <typename T, int LA, int LB, int TI, int TJ, int WI, int WJ, int STEP, int STAGES>
 __global__ __launch_bounds__(512) void product_turns_kernel(const Product P) {
-  constexpr int kNT = 512, STEP = 128;
-  constexpr int kFI = TI / WI / 16, kFJ = TJ / WJ / 16, kQ = kFI / 4, kPhases = 2 * kQ;
-  static_assert(WI * WJ == 8 && kFI % 4 == 0 && kFJ == 4 && (STAGES == 3 || kPhases == 4), "shape of the phases");
+  constexpr int kNT = 512;
+  constexpr int kFI = TI / WI / 16, kFJ = TJ / WJ / 16, kQ = kFI / 4, kPhases = STEP / 64 * kQ;
+  static_assert(WI * WJ == 8 && kFI % 4 == 0 && kFJ == 4 && kPhases >= 2 && (STAGES >= 3 || kPhases == 4),
+                "shape of the phases");
   using TileA = Tile<T, TI, LA, STEP>;
   using TileB = Tile<T, TJ, LB, STEP>;
   using LoadA = Loader<T, TI, LA, STEP, kNT, true>;
@@ -980,9 +981,9 @@ int launch_product(Product& P, const Plan& plan, hipStream_t stream) {
   const dim3 grid((unsigned)(P.tiles_i * P.tiles_j * plan.splits));
   if constexpr (sizeof(T) == 2 && DIRECT) {
     if (plan.tile == k256x256)
-      hipLaunchKernelGGL((product_turns_kernel<T, LA, LB, 256, 256, 2, 4, 2>), grid, dim3(512), 0, stream, P);
+      hipLaunchKernelGGL((product_turns_kernel<T, LA, LB, 256, 256, 2, 4, 128, 2>), grid, dim3(512), 0, stream, P);
     if (plan.tile == k256x128)
-      hipLaunchKernelGGL((product_turns_kernel<T, LA, LB, 256, 128, 4, 2, 3>), grid, dim3(512), 0, stream, P);
+      hipLaunchKernelGGL((product_turns_kernel<T, LA, LB, 256, 128, 4, 2, 128, 3>), grid, dim3(512), 0, stream, P);
   }
   if (plan.tile == k128x128)
     hipLaunchKernelGGL((product_kernel<Work<T, LA, LB, 128, 128, 2, 2, 1, 128, 2, DIRECT>>), grid, dim3(256), 0, stream, P);

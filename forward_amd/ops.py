@@ -382,53 +382,54 @@ def emb_layer_norm(input_ids, segment_ids, input_mask, word, pos, tok, gamma, be
 
 
 # ---- training and linear launchers --------------------------------------------------------------
-# These are short launches that a step issues by the hundred: pointers go to ctypes as plain integers, the stream
-# handle comes without a Stream object around it, and nothing is allocated that the result does not need.
+# Short launches that a step issues by the hundred: an operand is checked in one expression, pointers go to ctypes as
+# plain integers, the stream handle comes without a Stream object around it, and nothing is allocated that the result
+# does not need.
 
-class _On:
-    """Allocations and the launch of one call: on the operands' device whatever the current one is, on the call's stream
-    or that device's current one (results and workspaces then belong to the stream that writes them)."""
-
-    def __init__(self, operands, stream):
-        first = operands[0].device
-        for t in operands:
-            _require(t is None or t.device == first, 'all operands lie on one device')
-        _require(stream is None or stream.device == first, 'stream belongs to the device of the operands')
-        self.device, self.guard = first, None
-        if stream is not None:
-            self.guard = torch.cuda.stream(stream)
-        elif first.index != torch.cuda.current_device():
-            self.guard = torch.cuda.device(first)
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-        return torch._C._cuda_getCurrentRawStream(self.device.index)
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch.cuda.current_device
 
 
-def _ptr(t):
-    return None if t is None else t.data_ptr()
+def _away(x, stream):
+    """The context of a call whose operands lie on another device than the current one, or that runs on a stream of the
+    caller's (its results and workspace then belong to that stream); None for the ordinary call."""
+    if stream is not None:
+        _require(stream.device == x.device, 'stream belongs to the device of the operands')
+        return torch.cuda.stream(stream)
+    return None if x.get_device() == _current_device() else torch.cuda.device(x.device)
 
 
-def _train_dtype(x, name):
-    dt = _TDT.get(x.dtype)
+def _refuse(t, at, what):
+    """Why an operand of the training and linear launchers does not pass."""
+    _require(isinstance(t, torch.Tensor), what + ' (a tensor)')
+    _require(t.get_device() == at, what + ' (on the device of the first operand)')
+    _require(t.is_contiguous(), what + ' (contiguous)')
+    _require(False, '%s, not %s of shape %s' % (what, t.dtype, tuple(t.shape)))
+
+
+def _vector(t, n, at, name):
+    try:
+        if t.get_device() == at and t.dtype == torch.float32 and t.numel() == n and t.is_contiguous():
+            return t.data_ptr()
+    except AttributeError:
+        pass
+    _refuse(t, at, '%s is a float32 vector of %d elements' % (name, n))
+
+
+def _plane(t, shape, dtype, at, name):
+    try:
+        if t.get_device() == at and t.dtype == dtype and t.shape == shape and t.is_contiguous():
+            return t.data_ptr()
+    except AttributeError:
+        pass
+    _refuse(t, at, '%s has shape %s and dtype %s' % (name, tuple(shape), dtype))
+
+
+def _train_dtype(x):
+    dt = _TDT.get(_dev(x, "input").dtype)
     if dt is None:
-        raise TypeError("%s must be float32, float16 or bfloat16, not %s" % (name, x.dtype))
+        raise TypeError("input must be float32, float16 or bfloat16, not %s" % x.dtype)
     return dt
-
-
-def _vector(t, n, name):
-    if t is not None and (_dev(t, name).dtype != torch.float32 or t.numel() != n):
-        _require(False, '%s is float32 with %d elements' % (name, n))
-
-
-def _like(t, shape, dtype, name):
-    if t is not None and (_dev(t, name).dtype != dtype or t.shape != shape):
-        _require(False, '%s has shape %s and dtype %s' % (name, tuple(shape), dtype))
 
 
 def _space(size, device):
@@ -442,23 +443,29 @@ def layer_norm_forward(x, gamma, beta, skip=None, bias=None, eps=0.0, want_sum=F
     ``x`` / ``skip``: float32, float16 or bfloat16; gamma / beta / bias: float32 vectors; mean / rstd: float32,
     ``x.shape[:-1]``.
     """
-    dt = _train_dtype(_dev(x, "input"), "input")
-    shape = x.shape
+    dt, shape, at = _train_dtype(x), x.shape, x.get_device()
     ld = shape[-1] if shape else 0
-    _require(ld > 0, 'input has a last axis of at least one element')
-    _vector(_dev(gamma, "gamma"), ld, "gamma")
-    _vector(_dev(beta, "beta"), ld, "beta")
-    _vector(bias, ld, "bias")
-    _like(skip, shape, x.dtype, "skip")
-    with _On((x, gamma, beta, skip, bias), stream) as s:
+    if ld <= 0:
+        _require(False, 'input has a last axis of at least one element')
+    pg, pb = _vector(gamma, ld, at, "gamma"), _vector(beta, ld, at, "beta")
+    pi = None if bias is None else _vector(bias, ld, at, "bias")
+    ps = None if skip is None else _plane(skip, shape, x.dtype, at, "skip")
+
+    def call():
         y = torch.empty_like(x)
         h = torch.empty_like(x) if want_sum else None
         mean = x.new_empty(shape[:-1], dtype=torch.float32)
         rstd = torch.empty_like(mean)
-        lib.check(lib.dll.fwdmi_layer_norm_forward(s, ld, x.numel(), x.data_ptr(), _ptr(skip), beta.data_ptr(),
-                                                   gamma.data_ptr(), _ptr(bias), y.data_ptr(), _ptr(h), mean.data_ptr(),
+        lib.check(lib.dll.fwdmi_layer_norm_forward(_raw_stream(at), ld, x.numel(), x.data_ptr(), ps, pb, pg, pi,
+                                                   y.data_ptr(), h.data_ptr() if want_sum else None, mean.data_ptr(),
                                                    rstd.data_ptr(), dt, eps))
-    return (y, mean, rstd, h) if want_sum else (y, mean, rstd)
+        return (y, mean, rstd, h) if want_sum else (y, mean, rstd)
+
+    away = _away(x, stream)
+    if away is None:
+        return call()
+    with away:
+        return call()
 
 
 def layer_norm_backward(dy, x, gamma, mean, rstd, skip=None, bias=None, dsum=None, stream=None):
@@ -468,43 +475,57 @@ def layer_norm_backward(dy, x, gamma, mean, rstd, skip=None, bias=None, dsum=Non
     ``x`` and of ``skip`` alike.  ``dsum``: a gradient that reaches the sum from elsewhere, added to ``dx``.
     dgamma / dbeta / dbias are float32, summed over the rows in a fixed order.
     """
-    dt = _train_dtype(_dev(x, "input"), "input")
-    shape, n = x.shape, x.numel()
+    dt, shape, at, n = _train_dtype(x), x.shape, x.get_device(), x.numel()
     ld = shape[-1] if shape else 0
-    _require(ld > 0, 'input has a last axis of at least one element')
-    _like(_dev(dy, "dy"), shape, x.dtype, "dy")
-    _vector(_dev(gamma, "gamma"), ld, "gamma")
-    _vector(_dev(mean, "mean"), n // ld, "mean")
-    _vector(_dev(rstd, "rstd"), n // ld, "rstd")
-    _vector(bias, ld, "bias")
-    _like(skip, shape, x.dtype, "skip")
-    _like(dsum, shape, x.dtype, "dsum")
-    with _On((x, dy, gamma, mean, rstd, skip, bias, dsum), stream) as s:
-        dx = torch.empty_like(x)
-        dgamma, dbeta = torch.empty_like(gamma), torch.empty_like(gamma)
+    if ld <= 0:
+        _require(False, 'input has a last axis of at least one element')
+    pdy = _plane(dy, shape, x.dtype, at, "dy")
+    pg = _vector(gamma, ld, at, "gamma")
+    pm, pr = _vector(mean, n // ld, at, "mean"), _vector(rstd, n // ld, at, "rstd")
+    pi = None if bias is None else _vector(bias, ld, at, "bias")
+    ps = None if skip is None else _plane(skip, shape, x.dtype, at, "skip")
+    pd = None if dsum is None else _plane(dsum, shape, x.dtype, at, "dsum")
+
+    def call():
+        dx, dgamma, dbeta = torch.empty_like(x), torch.empty_like(gamma), torch.empty_like(gamma)
         dbias = None if bias is None else torch.empty_like(gamma)
         size = lib.dll.fwdmi_layer_norm_backward_workspace(ld, n, dt)
         ws = _space(size, x.device)
-        lib.check(lib.dll.fwdmi_layer_norm_backward(s, ld, n, dy.data_ptr(), x.data_ptr(), _ptr(skip), _ptr(dsum),
-                                                    gamma.data_ptr(), _ptr(bias), mean.data_ptr(), rstd.data_ptr(),
-                                                    dx.data_ptr(), dgamma.data_ptr(), dbeta.data_ptr(), _ptr(dbias),
-                                                    _ptr(ws), size, dt))
-    return (dx, dgamma, dbeta) if bias is None else (dx, dgamma, dbeta, dbias)
+        lib.check(lib.dll.fwdmi_layer_norm_backward(_raw_stream(at), ld, n, pdy, x.data_ptr(), ps, pd, pg, pi, pm, pr,
+                                                    dx.data_ptr(), dgamma.data_ptr(), dbeta.data_ptr(),
+                                                    None if bias is None else dbias.data_ptr(),
+                                                    ws.data_ptr() if size else None, size, dt))
+        return (dx, dgamma, dbeta) if bias is None else (dx, dgamma, dbeta, dbias)
+
+    away = _away(x, stream)
+    if away is None:
+        return call()
+    with away:
+        return call()
 
 
 def _act(activation):
-    _require(activation in ACTIVATIONS, 'activation is one of %s' % ", ".join(ACTIVATIONS))
-    return ACTIVATIONS[activation]
+    act = ACTIVATIONS.get(activation)
+    if act is None:
+        _require(False, 'activation is one of %s' % ", ".join(ACTIVATIONS))
+    return act
 
 
-def _linear_sizes(x, weight):
-    """(m, n, k) and the result's shape of a product of ``x`` [..., k] and ``weight`` [n, k]."""
-    _require(_dev(weight, "weight").dim() == 2 and weight.dtype == x.dtype, 'weight is [out, in] of the input dtype')
-    n, k = weight.shape
+def _linear_sizes(x, weight, at):
+    """(m, n, k), the result's shape and weight's address of a product of ``x`` [..., k] and ``weight`` [n, k]."""
     shape = x.shape
-    _require(len(shape) >= 1 and shape[-1] == k, 'the last axis of the input is as long as a row of weight')
-    m = x.numel() // k if k else shape[:-1].numel()
-    return m, n, k, shape[:-1] + (n,)
+    try:
+        n, k = weight.shape
+        ok = shape[-1] == k and weight.get_device() == at and weight.dtype == x.dtype and weight.is_contiguous()
+    except (AttributeError, IndexError, ValueError):
+        ok = False
+    if not ok:
+        _require(isinstance(weight, torch.Tensor) and weight.dim() == 2 and len(shape) > 0 and shape[-1] == weight.shape[1],
+                 'weight is [out, in] and the last axis of the input is as long as a row of it')
+        _refuse(weight, at, 'weight has the dtype of the input')
+    if len(shape) == 2:
+        return shape[0], n, k, (shape[0], n), weight.data_ptr()
+    return shape[:-1].numel(), n, k, shape[:-1] + (n,), weight.data_ptr()
 
 
 def linear(x, weight, bias=None, activation="none", residual=None, want_preact=False, stream=None):
@@ -514,19 +535,26 @@ def linear(x, weight, bias=None, activation="none", residual=None, want_preact=F
     ``bias``: a float32 vector; ``activation``: a key of ``ACTIVATIONS``.  With ``want_preact`` returns
     ``(y, z)``, ``z`` the value in front of the activation, which ``linear_backward`` reads.
     """
-    dt = _train_dtype(_dev(x, "input"), "input")
-    act = _act(activation)
-    m, n, k, shape = _linear_sizes(x, weight)
-    _vector(bias, n, "bias")
-    _like(residual, shape, x.dtype, "residual")
-    with _On((x, weight, bias, residual), stream) as s:
+    dt, act, at = _train_dtype(x), _act(activation), x.get_device()
+    m, n, k, shape, pw = _linear_sizes(x, weight, at)
+    pb = None if bias is None else _vector(bias, n, at, "bias")
+    pr = None if residual is None else _plane(residual, shape, x.dtype, at, "residual")
+
+    def call():
         y = x.new_empty(shape)
         z = torch.empty_like(y) if want_preact else None
         size = lib.dll.fwdmi_linear_workspace(m, n, k, dt)
         ws = _space(size, x.device)
-        lib.check(lib.dll.fwdmi_linear(s, m, n, k, x.data_ptr(), weight.data_ptr(), _ptr(bias), _ptr(residual),
-                                       y.data_ptr(), _ptr(z), act, dt, _ptr(ws), size))
-    return (y, z) if want_preact else y
+        lib.check(lib.dll.fwdmi_linear(_raw_stream(at), m, n, k, x.data_ptr(), pw, pb, pr, y.data_ptr(),
+                                       z.data_ptr() if want_preact else None, act, dt, ws.data_ptr() if size else None,
+                                       size))
+        return (y, z) if want_preact else y
+
+    away = _away(x, stream)
+    if away is None:
+        return call()
+    with away:
+        return call()
 
 
 def linear_backward(dy, x, weight, preact=None, activation="none", want_dx=True, want_dweight=True, want_dbias=True,
@@ -536,18 +564,26 @@ def linear_backward(dy, x, weight, preact=None, activation="none", want_dx=True,
     ``preact``: what ``linear`` returned for ``want_preact``, needed with an activation.  ``dx`` and ``dweight`` have the
     input's dtype, ``dbias`` is float32.
     """
-    dt = _train_dtype(_dev(x, "input"), "input")
-    act = _act(activation)
-    m, n, k, shape = _linear_sizes(x, weight)
-    _like(_dev(dy, "dy"), shape, x.dtype, "dy")
+    dt, act, at = _train_dtype(x), _act(activation), x.get_device()
+    m, n, k, shape, pw = _linear_sizes(x, weight, at)
+    pdy = _plane(dy, shape, x.dtype, at, "dy")
     _require(act == lib.ACT_NONE or preact is not None, 'an activation needs preact')
-    _like(preact, shape, x.dtype, "preact")
-    with _On((x, dy, weight, preact), stream) as s:
+    pz = None if preact is None else _plane(preact, shape, x.dtype, at, "preact")
+
+    def call():
         dx = torch.empty_like(x) if want_dx else None
         dw = torch.empty_like(weight) if want_dweight else None
         db = x.new_empty((n,), dtype=torch.float32) if want_dbias else None
         size = lib.dll.fwdmi_linear_backward_workspace(m, n, k, act, dt)
         ws = _space(size, x.device)
-        lib.check(lib.dll.fwdmi_linear_backward(s, m, n, k, dy.data_ptr(), x.data_ptr(), weight.data_ptr(), _ptr(preact),
-                                                _ptr(dx), _ptr(dw), _ptr(db), act, dt, _ptr(ws), size))
-    return tuple(t for t in (dx, dw, db) if t is not None)
+        lib.check(lib.dll.fwdmi_linear_backward(_raw_stream(at), m, n, k, pdy, x.data_ptr(), pw, pz,
+                                                dx.data_ptr() if want_dx else None, dw.data_ptr() if want_dweight else None,
+                                                db.data_ptr() if want_dbias else None, act, dt,
+                                                ws.data_ptr() if size else None, size))
+        return tuple(t for t in (dx, dw, db) if t is not None)
+
+    away = _away(x, stream)
+    if away is None:
+        return call()
+    with away:
+        return call()
