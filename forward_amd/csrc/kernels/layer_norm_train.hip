@@ -4,7 +4,7 @@
 //   h = x (+ skip) (+ bias),  mean and rstd = 1 / sqrt(var + eps) over a row,  xhat = (h - mean) * rstd
 //   y = gamma * xhat + beta
 //   dh = rstd * (g - mean(g) - xhat * mean(g * xhat)) with g = dy * gamma,  dx = dh (+ dsum)
-//   dgamma = sum over rows of dy * xhat, dbeta = sum of dy, dbias = sum of dh
+//   dgamma = sum over rows of dy * xhat, dbeta = sum of dy, dbias = sum of dx
 //
 // Everything between the loads and the one rounding at the store is fp32.  LPR lanes own a row (a part of a
 // wavefront, a wavefront, or several), 16 bytes per lane and step, NV steps, the row in registers: it is read
@@ -14,8 +14,9 @@
 //
 // The column sums stay in registers over all rows a workgroup processes, are combined through LDS in a fixed
 // order and leave as one row of partials per workgroup; a second small launch adds those, also in a fixed order:
-// no atomics, results repeat bit for bit.  Rows longer than a workgroup's registers are streamed from cache
-// (ln_*_stream_kernel), their column sums by a kernel that walks rows down each column.
+// no atomics, results repeat bit for bit.  Longer rows have their column sums computed by a kernel that walks down the
+// rows (ln_backward_columns_kernel), and rows longer than a workgroup's registers are streamed from cache
+// (ln_*_stream_kernel).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -45,7 +46,7 @@ struct LnTrain {
   float* part_gamma;  // backward: row p of partials starts at part_* + p * part_stride
   float* part_beta;
   float* part_bias;
-  float* c1;          // streamed backward: mean(g * xhat) and mean(g) per row
+  float* c1;          // backward of long rows: mean(g * xhat) and mean(g) per row
   float* c2;
   int64_t part_stride;
   int64_t rows;
@@ -214,12 +215,15 @@ __global__ __launch_bounds__(WG) void ln_forward_kernel(const LnTrain L) {
   }
 }
 
-template <typename T, int VEC, int NV, int WG, int LPR, bool FULL, bool BIAS>
+// SUMS: the column sums ride along in registers.  Rows of more than 16 elements per lane have none left for them
+// (2700 x 12288 fp16 took 164 us with the sums spilled): those leave c1 and c2 and ln_backward_columns_kernel reads dy and
+// x once more.
+template <typename T, int VEC, int NV, int WG, int LPR, bool FULL, bool BIAS, bool SUMS>
 __global__ __launch_bounds__(WG) void ln_backward_kernel(const LnTrain L) {
   constexpr int kRows = WG / LPR;
   constexpr int kSlots = LPR * NV * VEC;  // elements of a row, as the lanes hold them
   __shared__ float s_red[4 * (WG / 64)];
-  __shared__ float s_col[LPR < WG ? kRows * kSlots : 1];
+  __shared__ float s_col[LPR < WG && SUMS ? kRows * kSlots : 1];
   const int gl = threadIdx.x % LPR;
   const int group = threadIdx.x / LPR;
   const Columns<VEC, NV, LPR, FULL> C(gl, L.ld);
@@ -282,8 +286,10 @@ __global__ __launch_bounds__(WG) void ln_backward_kernel(const LnTrain L) {
         const float xl = live ? xh[j][e] : 0.0f;  // (a column or row of another lane may hold anything)
         a1 = __builtin_fmaf(gy[j][e], xl, a1);
         a2 += gy[j][e];
-        sum_g[j][e] = __builtin_fmaf(w, xl, sum_g[j][e]);
-        sum_b[j][e] += w;
+        if (SUMS) {
+          sum_g[j][e] = __builtin_fmaf(w, xl, sum_g[j][e]);
+          sum_b[j][e] += w;
+        }
         add[j][e] = has_dsum ? (float)d[j].v[e] : 0.0f;
       }
     if (r0 + step < L.rows) fetch(r + step);
@@ -311,6 +317,10 @@ __global__ __launch_bounds__(WG) void ln_backward_kernel(const LnTrain L) {
       }
     }
     const float c1 = a1 * inv_n, c2 = a2 * inv_n;
+    if (!SUMS && row_ok && gl == 0) {
+      gmut<float>(L.c1)[r] = c1;
+      gmut<float>(L.c2)[r] = c2;
+    }
     T FWDMI_GLOBAL* const po = gmut<T>(L.out) + r * L.ld;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
@@ -318,16 +328,18 @@ __global__ __launch_bounds__(WG) void ln_backward_kernel(const LnTrain L) {
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
         const float dh = rstd * __builtin_fmaf(-xh[j][e], c1, gy[j][e] - c2);
-        if (BIAS) sum_h[j][e] += row_ok && C.own(j, e) ? dh : 0.0f;
-        o.v[e] = (T)(dh + add[j][e]);
+        const float total = dh + add[j][e];
+        if (BIAS && SUMS) sum_h[j][e] += row_ok && C.own(j, e) ? total : 0.0f;
+        o.v[e] = (T)total;
       }
       if (row_ok) C.store(po, j, o);
     }
   }
 
+  if constexpr (!SUMS) return;
   // One row of partials per workgroup: the groups' sums in group order.
   auto leave = [&](float (&v)[NV][VEC], float* part) {
-    if constexpr (LPR < WG) {
+    if constexpr (LPR < WG && SUMS) {
       __syncthreads();
 #pragma unroll
       for (int j = 0; j < NV; ++j)
@@ -369,95 +381,210 @@ __device__ __forceinline__ float wg_sum(float x, float* scratch) {
   return row_sum<WG, WG>(x, scratch);
 }
 
-template <typename T>
-__device__ __forceinline__ float ln_input(const LnTrain& L, int64_t base, int c) {
-  float v = (float)gconst<T>(L.x)[base + c];
-  if (L.skip) v += (float)gconst<T>(L.skip)[base + c];
-  if (L.bias) v += L.bias[c];
-  return v;
+// Calls f(column, number of elements that exist) for the slices of a row that this lane takes: all of them whole but for
+// the row's last, which is a call of its own so that the others compile to vector accesses.
+template <int VEC, typename F>
+__device__ __forceinline__ void row_slices(int ld, F&& f) {
+  int c = (int)threadIdx.x * VEC;
+  for (; c + VEC <= ld; c += kStreamWG * VEC) f(c, std::integral_constant<bool, true>{}, VEC);
+  if (c < ld) f(c, std::integral_constant<bool, false>{}, ld - c);
+}
+template <typename T, int VEC, bool WHOLE>
+__device__ __forceinline__ void slice_in(const T* p, int64_t at, int n, float (&v)[VEC]) {
+  if (WHOLE) {
+    const Pack<T, VEC> x = load_slice<T, VEC>(gconst<T>(p) + at);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) v[e] = (float)x.v[e];
+  } else {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) v[e] = e < n ? (float)gconst<T>(p)[at + e] : 0.0f;
+  }
+}
+template <typename T, int VEC, bool WHOLE>
+__device__ __forceinline__ void slice_out(void* p, int64_t at, int n, const float (&v)[VEC]) {
+  Pack<T, VEC> o;
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) o.v[e] = (T)v[e];
+  if (WHOLE) {
+    store_slice<T, VEC>(gmut<T>(p) + at, o);
+  } else {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e)
+      if (e < n) gmut<T>(p)[at + e] = o.v[e];
+  }
+}
+// h of a slice
+template <typename T, int VEC, bool WHOLE>
+__device__ __forceinline__ void ln_input(const LnTrain& L, int64_t base, int c, int n, float (&h)[VEC]) {
+  slice_in<T, VEC, WHOLE>(static_cast<const T*>(L.x), base + c, n, h);
+  if (L.skip) {
+    float v[VEC];
+    slice_in<T, VEC, WHOLE>(static_cast<const T*>(L.skip), base + c, n, v);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) h[e] += v[e];
+  }
+  if (L.bias) {
+    float v[VEC];
+    slice_in<float, VEC, WHOLE>(L.bias, c, n, v);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) h[e] += v[e];
+  }
 }
 
 template <typename T>
 __global__ __launch_bounds__(kStreamWG) void ln_forward_stream_kernel(const LnTrain L) {
+  constexpr int VEC = 16 / sizeof(T);
   __shared__ float s_red[kStreamWG / 64];
   const float inv_n = 1.0f / (float)L.ld;
   for (int64_t r = blockIdx.x; r < L.rows; r += gridDim.x) {
     const int64_t base = r * L.ld;
     float a = 0.0f;
-    for (int c = threadIdx.x; c < L.ld; c += kStreamWG) a += ln_input<T>(L, base, c);
+    row_slices<VEC>(L.ld, [&](int c, auto whole, int n) {
+      float h[VEC];
+      ln_input<T, VEC, decltype(whole)::value>(L, base, c, n, h);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) a += e < n ? h[e] : 0.0f;
+    });
     const float mu = wg_sum<kStreamWG>(a, s_red) * inv_n;
     a = 0.0f;
-    for (int c = threadIdx.x; c < L.ld; c += kStreamWG) {
-      const float d = ln_input<T>(L, base, c) - mu;
-      a = __builtin_fmaf(d, d, a);
-    }
+    row_slices<VEC>(L.ld, [&](int c, auto whole, int n) {
+      float h[VEC];
+      ln_input<T, VEC, decltype(whole)::value>(L, base, c, n, h);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const float d = e < n ? h[e] - mu : 0.0f;
+        a = __builtin_fmaf(d, d, a);
+      }
+    });
     const float rs = __builtin_amdgcn_rsqf(__builtin_fmaf(wg_sum<kStreamWG>(a, s_red), inv_n, L.eps));
     if (threadIdx.x == 0) {
-      L.mean[r] = mu;
-      L.rstd[r] = rs;
+      gmut<float>(L.mean)[r] = mu;
+      gmut<float>(L.rstd)[r] = rs;
     }
-    for (int c = threadIdx.x; c < L.ld; c += kStreamWG) {
-      const float h = ln_input<T>(L, base, c);
-      if (L.sum) gmut<T>(L.sum)[base + c] = (T)h;
-      gmut<T>(L.out)[base + c] = (T)__builtin_fmaf(L.gamma[c], (h - mu) * rs, L.beta[c]);
-    }
+    row_slices<VEC>(L.ld, [&](int c, auto whole, int n) {
+      constexpr bool kWhole = decltype(whole)::value;
+      float h[VEC], g[VEC], b[VEC];
+      ln_input<T, VEC, kWhole>(L, base, c, n, h);
+      slice_in<float, VEC, kWhole>(L.gamma, c, n, g);
+      slice_in<float, VEC, kWhole>(L.beta, c, n, b);
+      if (L.sum) slice_out<T, VEC, kWhole>(L.sum, base + c, n, h);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) h[e] = __builtin_fmaf(g[e], (h[e] - mu) * rs, b[e]);
+      slice_out<T, VEC, kWhole>(L.out, base + c, n, h);
+    });
   }
 }
 
 template <typename T>
 __global__ __launch_bounds__(kStreamWG) void ln_backward_stream_kernel(const LnTrain L) {
+  constexpr int VEC = 16 / sizeof(T);
   __shared__ float s_red[kStreamWG / 64];
   const float inv_n = 1.0f / (float)L.ld;
   for (int64_t r = blockIdx.x; r < L.rows; r += gridDim.x) {
     const int64_t base = r * L.ld;
-    const float mu = L.mean[r], rs = L.rstd[r];
+    const float mu = gconst<float>(L.mean)[r], rs = gconst<float>(L.rstd)[r];
     float a1 = 0.0f, a2 = 0.0f;
-    for (int c = threadIdx.x; c < L.ld; c += kStreamWG) {
-      const float gy = (float)gconst<T>(L.dy)[base + c] * L.gamma[c];
-      a1 = __builtin_fmaf(gy, (ln_input<T>(L, base, c) - mu) * rs, a1);
-      a2 += gy;
-    }
+    row_slices<VEC>(L.ld, [&](int c, auto whole, int n) {
+      constexpr bool kWhole = decltype(whole)::value;
+      float h[VEC], dy[VEC], g[VEC];
+      ln_input<T, VEC, kWhole>(L, base, c, n, h);
+      slice_in<T, VEC, kWhole>(static_cast<const T*>(L.dy), base + c, n, dy);
+      slice_in<float, VEC, kWhole>(L.gamma, c, n, g);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const float gy = dy[e] * g[e];  // (zeros past the row's end)
+        a1 = __builtin_fmaf(gy, (h[e] - mu) * rs, a1);
+        a2 += gy;
+      }
+    });
     const float c1 = wg_sum<kStreamWG>(a1, s_red) * inv_n;
     const float c2 = wg_sum<kStreamWG>(a2, s_red) * inv_n;
     if (threadIdx.x == 0) {
-      L.c1[r] = c1;
-      L.c2[r] = c2;
+      gmut<float>(L.c1)[r] = c1;
+      gmut<float>(L.c2)[r] = c2;
     }
-    for (int c = threadIdx.x; c < L.ld; c += kStreamWG) {
-      const float xh = (ln_input<T>(L, base, c) - mu) * rs;
-      float dh = rs * __builtin_fmaf(-xh, c1, (float)gconst<T>(L.dy)[base + c] * L.gamma[c] - c2);
-      if (L.dsum) dh += (float)gconst<T>(L.dsum)[base + c];
-      gmut<T>(L.out)[base + c] = (T)dh;
-    }
+    row_slices<VEC>(L.ld, [&](int c, auto whole, int n) {
+      constexpr bool kWhole = decltype(whole)::value;
+      float h[VEC], dy[VEC], g[VEC], d[VEC] = {};
+      ln_input<T, VEC, kWhole>(L, base, c, n, h);
+      slice_in<T, VEC, kWhole>(static_cast<const T*>(L.dy), base + c, n, dy);
+      slice_in<float, VEC, kWhole>(L.gamma, c, n, g);
+      if (L.dsum) slice_in<T, VEC, kWhole>(static_cast<const T*>(L.dsum), base + c, n, d);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e)
+        h[e] = rs * __builtin_fmaf(-((h[e] - mu) * rs), c1, dy[e] * g[e] - c2) + d[e];
+      slice_out<T, VEC, kWhole>(L.out, base + c, n, h);
+    });
   }
 }
 
-// Column sums of streamed rows: a lane per column, blockIdx.y takes every gridDim.y-th row.
+// Column sums of long rows: eight columns per lane (fp32 four), every (4 gridDim.y)-th row per wave, the four waves'
+// sums through LDS.
 template <typename T>
 __global__ __launch_bounds__(256) void ln_backward_columns_kernel(const LnTrain L) {
-  const int64_t c64 = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (c64 >= L.ld) return;
-  const int c = (int)c64;
-  float sg = 0.0f, sb = 0.0f, sh = 0.0f;
-  for (int64_t r = blockIdx.y; r < L.rows; r += gridDim.y) {
-    const int64_t base = r * L.ld;
-    const float rs = L.rstd[r];
-    const float w = (float)gconst<T>(L.dy)[base + c];
-    const float xh = (ln_input<T>(L, base, c) - L.mean[r]) * rs;
-    sg = __builtin_fmaf(w, xh, sg);
-    sb += w;
-    if (L.part_bias) sh += rs * __builtin_fmaf(-xh, L.c1[r], w * L.gamma[c] - L.c2[r]);
-  }
-  const int64_t p = blockIdx.y * L.part_stride;
-  L.part_gamma[p + c] = sg;
-  L.part_beta[p + c] = sb;
-  if (L.part_bias) L.part_bias[p + c] = sh;
+  constexpr int kVec = 16 / sizeof(T);
+  __shared__ float s_sum[4][64 * kVec];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t c = ((int64_t)blockIdx.x * 64 + lane) * kVec;
+  const int live = (int)min((int64_t)kVec, max((int64_t)L.ld - c, (int64_t)0));
+  float sg[kVec] = {}, sb[kVec] = {}, sh[kVec] = {}, g[kVec] = {}, bi[kVec] = {};
+#pragma unroll
+  for (int e = 0; e < kVec; ++e)
+    if (e < live) {
+      g[e] = gconst<float>(L.gamma)[c + e];
+      if (L.bias) bi[e] = gconst<float>(L.bias)[c + e];
+    }
+  auto some = [&](const void* p, int64_t at) {
+    Pack<T, kVec> v{};
+    if (live == kVec) {
+      v = load_slice<T, kVec>(gconst<T>(p) + at);
+    } else {
+#pragma unroll
+      for (int e = 0; e < kVec; ++e)
+        if (e < live) v.v[e] = gconst<T>(p)[at + e];
+    }
+    return v;
+  };
+  if (live > 0)
+    for (int64_t r = blockIdx.y * 4 + wave; r < L.rows; r += 4 * gridDim.y) {
+      const int64_t at = r * L.ld + c;
+      const float mu = gconst<float>(L.mean)[r], rs = gconst<float>(L.rstd)[r];
+      const float c1 = gconst<float>(L.c1)[r], c2 = gconst<float>(L.c2)[r];
+      const Pack<T, kVec> dy = some(L.dy, at), x = some(L.x, at);
+      Pack<T, kVec> s{}, d{};
+      if (L.skip) s = some(L.skip, at);
+      if (L.part_bias && L.dsum) d = some(L.dsum, at);
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) {
+        float h = (float)x.v[e];
+        if (L.skip) h += (float)s.v[e];
+        h += bi[e];
+        const float w = (float)dy.v[e], xh = (h - mu) * rs;
+        sg[e] = __builtin_fmaf(w, xh, sg[e]);
+        sb[e] += w;
+        sh[e] += rs * __builtin_fmaf(-xh, c1, w * g[e] - c2) + (float)d.v[e];
+      }
+    }
+  auto leave = [&](const float (&v)[kVec], float* part) {
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) s_sum[wave][lane * kVec + e] = v[e];
+    __syncthreads();
+    for (int i = threadIdx.x; i < 64 * kVec; i += 256) {
+      const int64_t col = (int64_t)blockIdx.x * 64 * kVec + i;
+      if (col < L.ld)
+        gmut<float>(part)[blockIdx.y * L.part_stride + col] = ((s_sum[0][i] + s_sum[1][i]) + s_sum[2][i]) + s_sum[3][i];
+    }
+  };
+  leave(sg, L.part_gamma);
+  leave(sb, L.part_beta);
+  if (L.part_bias) leave(sh, L.part_bias);
 }
 
 // ---- launch ---------------------------------------------------------------------------------------------------
 
 constexpr int kMaxParts = 256;       // rows of partials a backward launch leaves (its workgroups)
-constexpr int kStreamParts = 64;     // the same for streamed rows
+constexpr int kLongParts = 32;       // the same for long rows, whose column sums are a launch of their own
 constexpr int kBackwardWG = 512;
 
 // Lanes per row and steps per lane of a row of `ld` elements in slices of VEC; steps == 0: streamed.
@@ -474,8 +601,11 @@ Shape row_shape(int ld, int vec) {
     if (slices <= 64 * nv) return {64, nv};
   for (int nv = 1; nv <= deep; nv *= 2)
     if (slices <= 256 * nv) return {256, nv};
-  for (int nv = deep; nv <= 2 * deep; nv *= 2)
-    if (slices <= 512 * nv) return {512, nv};
+  if (slices <= 512 * deep) return {512, deep};
+  // fp32 rows of more than 16 elements per lane do not fit its registers: 2700 x 12288 took 124 us forward and 275 us
+  // backward that way, 74 and 146
+  // streamed
+  if (vec == 8 && slices <= 1024 * deep) return {512, 2 * deep};
   return {0, 0};
 }
 
@@ -495,8 +625,9 @@ int launch_forward(const LnTrain& L, hipStream_t stream) {
 
 template <typename T, int VEC, int NV, int LPR>
 int launch_backward(const LnTrain& L, unsigned grid, hipStream_t stream) {
+  constexpr bool kSums = NV * VEC <= 16;
 #define FWDMI_LN_LAUNCH(FULL_, BIAS_)                                                                          \
-  hipLaunchKernelGGL((ln_backward_kernel<T, VEC, NV, kBackwardWG, LPR, FULL_, BIAS_>), dim3(grid),             \
+  hipLaunchKernelGGL((ln_backward_kernel<T, VEC, NV, kBackwardWG, LPR, FULL_, BIAS_, kSums>), dim3(grid),      \
                      dim3(kBackwardWG), 0, stream, L)
   if (L.ld == LPR * VEC * NV) {
     if (L.bias)
@@ -542,24 +673,29 @@ bool with_shape(int ld, F&& f) {
     FWDMI_SHAPE(256, 4)
   }
   FWDMI_SHAPE(512, kDeep)
-  FWDMI_SHAPE(512, 2 * kDeep)
+  if constexpr (kVec == 8) {
+    FWDMI_SHAPE(512, 2 * kDeep)
+  }
 #undef FWDMI_SHAPE
   return false;
 }
 
-// Rows of partials of a backward launch: its workgroups.
-int64_t backward_parts(int ld, int64_t rows, int dtype) {
-  if (rows == 0) return 0;
+// Rows of more than 16 elements per lane, or streamed: column sums by ln_backward_columns_kernel.
+bool long_rows(int ld, int dtype) {
   const int vec = dtype == FWDMI_F32 ? 4 : 8;
-  const Shape s = ld < vec ? Shape{8, 1} : row_shape(ld, vec);
-  if (s.lpr == 0) return std::min<int64_t>(rows, kStreamParts);
-  const int per = kBackwardWG / s.lpr;
-  return std::min<int64_t>((rows + per - 1) / per, kMaxParts);
+  if (ld < vec) return false;
+  const Shape s = row_shape(ld, vec);
+  return s.lpr == 0 || s.nv * vec > 16;
 }
 
-bool streamed(int ld, int dtype) {
+// Rows of partials of a backward call.
+int64_t backward_parts(int ld, int64_t rows, int dtype) {
+  if (rows == 0) return 0;
+  if (long_rows(ld, dtype)) return std::min<int64_t>((rows + 3) / 4, kLongParts);
   const int vec = dtype == FWDMI_F32 ? 4 : 8;
-  return ld >= vec && row_shape(ld, vec).lpr == 0;
+  const Shape s = ld < vec ? Shape{8, 1} : row_shape(ld, vec);
+  const int per = kBackwardWG / s.lpr;
+  return std::min<int64_t>((rows + per - 1) / per, kMaxParts);
 }
 
 template <typename T>
@@ -576,16 +712,19 @@ int forward_typed(const LnTrain& L, hipStream_t stream) {
 }
 
 template <typename T>
-int backward_typed(const LnTrain& L, int64_t parts, hipStream_t stream) {
+int backward_typed(const LnTrain& L, int64_t parts, bool long_row, hipStream_t stream) {
   int rc = FWDMI_OK;
+  const int64_t grid = long_row ? std::min<int64_t>(L.rows, (int64_t)device_cus() * 2) : parts;
   const bool done = with_shape<T>(L.ld, [&](auto vec, auto nv, auto lpr) {
-    rc = launch_backward<T, decltype(vec)::value, decltype(nv)::value, decltype(lpr)::value>(L, (unsigned)parts, stream);
+    rc = launch_backward<T, decltype(vec)::value, decltype(nv)::value, decltype(lpr)::value>(L, (unsigned)grid, stream);
   });
-  if (done) return rc;
-  const unsigned grid = (unsigned)std::min<int64_t>(L.rows, (int64_t)device_cus() * 4);
-  hipLaunchKernelGGL((ln_backward_stream_kernel<T>), dim3(grid), dim3(kStreamWG), 0, stream, L);
-  FWDMI_HIP_CHECK(hipGetLastError());
-  const dim3 cgrid((unsigned)(((int64_t)L.ld + 255) / 256), (unsigned)parts);
+  if (!done) {
+    hipLaunchKernelGGL((ln_backward_stream_kernel<T>), dim3((unsigned)grid), dim3(kStreamWG), 0, stream, L);
+    FWDMI_HIP_CHECK(hipGetLastError());
+  }
+  if (rc != FWDMI_OK || !long_row) return rc;
+  constexpr int kColumns = 64 * 16 / (int)sizeof(T);
+  const dim3 cgrid((unsigned)(((int64_t)L.ld + kColumns - 1) / kColumns), (unsigned)parts);
   hipLaunchKernelGGL((ln_backward_columns_kernel<T>), cgrid, dim3(256), 0, stream, L);
   FWDMI_HIP_CHECK(hipGetLastError());
   return FWDMI_OK;
@@ -629,7 +768,7 @@ size_t fwdmi_layer_norm_backward_workspace(int32_t ld, int64_t n, int32_t dtype)
   if (!is_train_dtype(dtype) || ld <= 0 || n <= 0 || n % ld != 0) return 0;
   const int64_t rows = n / ld;
   size_t bytes = (size_t)backward_parts(ld, rows, dtype) * 3 * (size_t)ld * sizeof(float);
-  if (streamed(ld, dtype)) bytes += (size_t)rows * 2 * sizeof(float);
+  if (long_rows(ld, dtype)) bytes += (size_t)rows * 2 * sizeof(float);
   return bytes;
 }
 
@@ -665,7 +804,8 @@ int fwdmi_layer_norm_backward(void* stream, int32_t ld, int64_t n, const void* d
     L.rows = rows;
     L.ld = ld;
     float* const ws = static_cast<float*>(workspace);
-    L.c1 = ws + parts * 3 * (int64_t)ld;  // read and written by streamed rows only
+    const bool long_row = long_rows(ld, dtype);
+    L.c1 = ws + parts * 3 * (int64_t)ld;  // of long rows
     L.c2 = L.c1 + rows;
     if (parts == 1) {  // one workgroup's sums are the result
       L.part_gamma = dgamma;
@@ -677,9 +817,9 @@ int fwdmi_layer_norm_backward(void* stream, int32_t ld, int64_t n, const void* d
       L.part_bias = bias ? ws + 2 * (int64_t)ld : nullptr;
       L.part_stride = (int64_t)kinds * ld;
     }
-    const int rc = dtype == FWDMI_F16    ? backward_typed<_Float16>(L, parts, s)
-                   : dtype == FWDMI_BF16 ? backward_typed<__bf16>(L, parts, s)
-                                         : backward_typed<float>(L, parts, s);
+    const int rc = dtype == FWDMI_F16    ? backward_typed<_Float16>(L, parts, long_row, s)
+                   : dtype == FWDMI_BF16 ? backward_typed<__bf16>(L, parts, long_row, s)
+                                         : backward_typed<float>(L, parts, long_row, s);
     if (rc != FWDMI_OK || parts == 1) return rc;
   }
   ColumnSums S{};

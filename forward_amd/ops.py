@@ -472,8 +472,8 @@ def layer_norm_backward(dy, x, gamma, mean, rstd, skip=None, bias=None, dsum=Non
     """Gradient of ``layer_norm_forward``: ``(dx, dgamma, dbeta)``, with a bias ``(dx, dgamma, dbeta, dbias)``.
 
     ``x`` / ``skip`` / ``bias`` as the forward call took them, or its sum as ``x`` alone; ``dx`` is the gradient of
-    ``x`` and of ``skip`` alike.  ``dsum``: a gradient that reaches the sum from elsewhere, added to ``dx``.
-    dgamma / dbeta / dbias are float32, summed over the rows in a fixed order.
+    ``x`` and of ``skip`` alike, and ``dbias`` its sum over the rows.  ``dsum``: a gradient that reaches the sum from
+    elsewhere, added to ``dx``.  dgamma / dbeta / dbias are float32, summed in a fixed order.
     """
     dt, shape, at, n = _train_dtype(x), x.shape, x.get_device(), x.numel()
     ld = shape[-1] if shape else 0

@@ -5,11 +5,13 @@ source/fwd_torch/torch_engine/torch_engine.cpp:134-174): there, int64 ids are co
 outputs are copied out of engine buffers; here the bag ops consume int32 or int64 ids as they are and
 write straight into the tensors they return, or, in their ``*_out`` forms, into tensors the caller
 supplies (declared to PyTorch as mutated arguments), so that a serving loop reuses its buffers.
+``linear`` and ``layer_norm_train`` (with their ``*_preact`` / ``*_sum`` forms) are differentiable and back the modules
+``Linear``, ``LayerNorm`` and ``FeedForward``, which train as well as serve.
 The BERT ops (``emb_layer_norm``, ``emb_skip_layer_norm``) take the ``[B, S]`` tensors a PyTorch model
 holds (``batch_major``) or the plugin's ``[S, B]``.  ``nn.EmbeddingBag`` / ``nn.Embedding`` modules of an
 inference model can be swapped for the HIP path with ``replace_embedding_modules``.
 """
-from typing import List, Optional
+from typing import List, Optional, Tuple
 
 import torch
 
@@ -183,6 +185,235 @@ def emb_layer_norm_out(out: torch.Tensor, mask_idx: Optional[torch.Tensor], inpu
                        bias2=_f32(bias2), eps2=eps2)
 
 
+# ---- the dense half of a layer: differentiable ---------------------------------------------------
+# Each forward op keeps what its backward op reads.  Parameters may have any floating type: the launchers take biases and
+# norm parameters as float32, and gradients go back in the parameter's own type.
+
+def _opt(t):
+    return None if t is None else t.contiguous()
+
+
+def _like_param(grad, p):
+    return None if p is None else grad.to(p.dtype)
+
+
+@torch.library.custom_op("fwdmi::linear", mutates_args=())
+def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor], residual: Optional[torch.Tensor],
+           activation: str) -> torch.Tensor:
+    """``act(x weight^T + bias) + residual``.  Under autograd with an activation use ``linear_preact``, whose backward pass
+    reads what it kept."""
+    return ops.linear(x.contiguous(), weight.contiguous(), bias=_f32(bias), activation=activation, residual=_opt(residual))
+
+
+@linear.register_fake
+def _(x, weight, bias, residual, activation):
+    return x.new_empty(tuple(x.shape[:-1]) + (weight.shape[0],))
+
+
+@torch.library.custom_op("fwdmi::linear_preact", mutates_args=())
+def linear_preact(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor], residual: Optional[torch.Tensor],
+                  activation: str) -> Tuple[torch.Tensor, torch.Tensor]:
+    """``(act(z) + residual, z)`` with ``z = x weight^T + bias``; no gradient flows into ``z``."""
+    return ops.linear(x.contiguous(), weight.contiguous(), bias=_f32(bias), activation=activation, residual=_opt(residual),
+                      want_preact=True)
+
+
+@linear_preact.register_fake
+def _(x, weight, bias, residual, activation):
+    y = x.new_empty(tuple(x.shape[:-1]) + (weight.shape[0],))
+    return y, torch.empty_like(y)
+
+
+@torch.library.custom_op("fwdmi::linear_backward", mutates_args=())
+def linear_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, preact: Optional[torch.Tensor],
+                    activation: str, want_dx: bool, want_dweight: bool, want_dbias: bool) -> List[torch.Tensor]:
+    """Those of ``[dx, dweight, dbias (float32)]`` that are wanted."""
+    return list(ops.linear_backward(dy.contiguous(), x.contiguous(), weight.contiguous(), preact=_opt(preact),
+                                    activation=activation, want_dx=want_dx, want_dweight=want_dweight,
+                                    want_dbias=want_dbias))
+
+
+@linear_backward.register_fake
+def _(dy, x, weight, preact, activation, want_dx, want_dweight, want_dbias):
+    out = [torch.empty(x.shape, dtype=x.dtype, device=x.device)] if want_dx else []
+    if want_dweight:
+        out.append(torch.empty(weight.shape, dtype=weight.dtype, device=weight.device))
+    if want_dbias:
+        out.append(x.new_empty((weight.shape[0],), dtype=torch.float32))
+    return out
+
+
+def _linear_setup(ctx, inputs, output):
+    x, weight, bias, residual, activation = inputs
+    z = None
+    if isinstance(output, tuple):
+        z = output[1]
+        ctx.mark_non_differentiable(z)
+    elif activation != "none" and any(ctx.needs_input_grad):
+        raise RuntimeError("fwdmi::linear keeps no pre-activation for the gradient of %r: use fwdmi::linear_preact" % activation)
+    ctx.set_materialize_grads(False)
+    ctx.save_for_backward(x, weight, bias, z)
+    ctx.activation = activation
+
+
+def _linear_grad(ctx, dy, *_):
+    if dy is None:
+        return None, None, None, None, None
+    x, weight, bias, z = ctx.saved_tensors
+    need = list(ctx.needs_input_grad[:3])
+    got = iter(torch.ops.fwdmi.linear_backward(dy, x, weight, z if ctx.activation != "none" else None, ctx.activation,
+                                               *need) if any(need) else ())
+    dx, dw, db = (next(got) if n else None for n in need)
+    return dx, dw, None if db is None else _like_param(db, bias), dy if ctx.needs_input_grad[3] else None, None
+
+
+linear.register_autograd(_linear_grad, setup_context=_linear_setup)
+linear_preact.register_autograd(_linear_grad, setup_context=_linear_setup)
+
+
+@torch.library.custom_op("fwdmi::layer_norm_train", mutates_args=())
+def layer_norm_train(x: torch.Tensor, skip: Optional[torch.Tensor], gamma: torch.Tensor, beta: torch.Tensor,
+                     bias: Optional[torch.Tensor], eps: float) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """``(LN(x + skip + bias), mean, rstd)``; no gradient flows into the statistics."""
+    return ops.layer_norm_forward(x.contiguous(), _f32(gamma), _f32(beta), skip=_opt(skip), bias=_f32(bias), eps=eps)
+
+
+@layer_norm_train.register_fake
+def _(x, skip, gamma, beta, bias, eps):
+    mean = x.new_empty(x.shape[:-1], dtype=torch.float32)
+    return torch.empty(x.shape, dtype=x.dtype, device=x.device), mean, torch.empty_like(mean)
+
+
+@torch.library.custom_op("fwdmi::layer_norm_train_sum", mutates_args=())
+def layer_norm_train_sum(x: torch.Tensor, skip: Optional[torch.Tensor], gamma: torch.Tensor, beta: torch.Tensor,
+                         bias: Optional[torch.Tensor], eps: float
+                         ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """``(LN(h), h, mean, rstd)`` with ``h = x + skip + bias``, the residual stream of a pre-norm layer."""
+    y, mean, rstd, h = ops.layer_norm_forward(x.contiguous(), _f32(gamma), _f32(beta), skip=_opt(skip), bias=_f32(bias),
+                                              eps=eps, want_sum=True)
+    return y, h, mean, rstd
+
+
+@layer_norm_train_sum.register_fake
+def _(x, skip, gamma, beta, bias, eps):
+    mean = x.new_empty(x.shape[:-1], dtype=torch.float32)
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    return y, torch.empty_like(y), mean, torch.empty_like(mean)
+
+
+@torch.library.custom_op("fwdmi::layer_norm_backward", mutates_args=())
+def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, skip: Optional[torch.Tensor], gamma: torch.Tensor,
+                        bias: Optional[torch.Tensor], mean: torch.Tensor, rstd: torch.Tensor,
+                        dsum: Optional[torch.Tensor]) -> List[torch.Tensor]:
+    """``[dx, dgamma, dbeta]``, with a bias ``[dx, dgamma, dbeta, dbias]``; all but dx float32."""
+    return list(ops.layer_norm_backward(dy.contiguous(), x.contiguous(), _f32(gamma), mean, rstd, skip=_opt(skip),
+                                        bias=_f32(bias), dsum=_opt(dsum)))
+
+
+@layer_norm_backward.register_fake
+def _(dy, x, skip, gamma, bias, mean, rstd, dsum):
+    out = [torch.empty(x.shape, dtype=x.dtype, device=x.device)]
+    return out + [gamma.new_empty(gamma.shape, dtype=torch.float32) for _ in range(2 if bias is None else 3)]
+
+
+def _norm_setup(ctx, inputs, output):
+    x, skip, gamma, beta, bias, _ = inputs
+    mean, rstd = output[-2:]
+    ctx.mark_non_differentiable(mean, rstd)
+    ctx.set_materialize_grads(False)
+    ctx.has_sum = len(output) == 4
+    ctx.types = (skip is not None, gamma.dtype, beta.dtype, None if bias is None else bias.dtype)
+    if ctx.has_sum and bias is None:      # the kept sum stands for x and skip
+        x, skip = output[1], None
+    ctx.save_for_backward(x, skip, gamma, bias, mean, rstd)
+
+
+def _norm_grad(ctx, dy, *rest):
+    x, skip, gamma, bias, mean, rstd = ctx.saved_tensors
+    dsum = rest[0] if ctx.has_sum else None
+    had_skip, gamma_t, beta_t, bias_t = ctx.types
+    if dy is None:
+        if dsum is None:
+            return None, None, None, None, None, None
+        dy = torch.zeros_like(x)
+    got = torch.ops.fwdmi.layer_norm_backward(dy, x, skip, gamma, bias, mean, rstd, dsum)
+    dx = got[0]
+    return (dx, dx if had_skip else None, got[1].to(gamma_t), got[2].to(beta_t), got[3].to(bias_t) if bias is not None else None,
+            None)
+
+
+layer_norm_train.register_autograd(_norm_grad, setup_context=_norm_setup)
+layer_norm_train_sum.register_autograd(_norm_grad, setup_context=_norm_setup)
+
+
+class Linear(torch.nn.Module):
+    """``nn.Linear`` with its activation and a residual in the product's epilogue: ``act(x W^T + b) (+ residual)``.
+    Trains and serves; ``activation`` is a key of ``ops.ACTIVATIONS``."""
+
+    def __init__(self, in_features, out_features, bias=True, activation="none", device=None, dtype=None):
+        super().__init__()
+        m = torch.nn.Linear(in_features, out_features, bias=bias, device=device, dtype=dtype)
+        self.weight, self.bias = m.weight, m.bias
+        self.activation = activation
+
+    @classmethod
+    def from_torch(cls, m, activation="none"):
+        """Shares the parameters of an ``nn.Linear``."""
+        out = cls.__new__(cls)
+        torch.nn.Module.__init__(out)
+        out.weight, out.bias, out.activation = m.weight, m.bias, activation
+        return out
+
+    def forward(self, x, residual=None):
+        keep = self.activation != "none" and torch.is_grad_enabled() and (
+            x.requires_grad or self.weight.requires_grad or (self.bias is not None and self.bias.requires_grad)
+            or (residual is not None and residual.requires_grad))
+        if keep:
+            return torch.ops.fwdmi.linear_preact(x, self.weight, self.bias, residual, self.activation)[0]
+        return torch.ops.fwdmi.linear(x, self.weight, self.bias, residual, self.activation)
+
+
+class LayerNorm(torch.nn.Module):
+    """``nn.LayerNorm`` over the last axis of ``x (+ skip) (+ bias)``, for training and serving.  ``forward(x, skip, bias)``
+    returns the normalised rows, with ``keep_sum`` ``(rows, sum)``: the residual stream of a pre-norm layer."""
+
+    def __init__(self, size, eps=1e-5, keep_sum=False, device=None, dtype=None):
+        super().__init__()
+        self.gamma = torch.nn.Parameter(torch.ones(size, device=device, dtype=dtype))
+        self.beta = torch.nn.Parameter(torch.zeros(size, device=device, dtype=dtype))
+        self.eps, self.keep_sum = float(eps), keep_sum
+
+    @classmethod
+    def from_torch(cls, m, keep_sum=False):
+        """Shares the parameters of an ``nn.LayerNorm`` over one axis with weight and bias."""
+        if len(m.normalized_shape) != 1 or m.weight is None or m.bias is None:
+            raise NotImplementedError("layer norm over one axis, with weight and bias")
+        out = cls.__new__(cls)
+        torch.nn.Module.__init__(out)
+        out.gamma, out.beta, out.eps, out.keep_sum = m.weight, m.bias, float(m.eps), keep_sum
+        return out
+
+    def forward(self, x, skip=None, bias=None):
+        op = torch.ops.fwdmi.layer_norm_train_sum if self.keep_sum else torch.ops.fwdmi.layer_norm_train
+        got = op(x, skip, self.gamma, self.beta, bias, self.eps)
+        return got[:2] if self.keep_sum else got[0]
+
+
+class FeedForward(torch.nn.Module):
+    """The feed-forward half of a BERT layer, post-norm: ``LN(x + W2 act(W1 x + b1) + b2)``: two products and one norm, the
+    second product's bias and the residual joined in the norm."""
+
+    def __init__(self, hidden, inner, activation="gelu", eps=1e-12, device=None, dtype=None):
+        super().__init__()
+        self.up = Linear(hidden, inner, activation=activation, device=device, dtype=dtype)
+        self.down = Linear(inner, hidden, device=device, dtype=dtype)
+        self.norm = LayerNorm(hidden, eps=eps, device=device, dtype=dtype)
+
+    def forward(self, x):
+        f = torch.ops.fwdmi.linear(self.up(x), self.down.weight, None, None, "none")
+        return self.norm(f, skip=x, bias=self.down.bias)
+
+
 class BertEmbeddings(torch.nn.Module):
     """Inference replacement of a BERT embedding block (word + position + token-type lookup, then
     LayerNorm) on ``[B, S]`` tensors: ``forward(input_ids, token_type_ids, attention_mask)`` returns
@@ -276,4 +507,18 @@ def replace_embedding_modules(model):
             setattr(model, name, Embedding(child.weight))
         else:
             replace_embedding_modules(child)
+    return model
+
+
+def replace_dense_modules(model):
+    """Swaps every ``nn.Linear`` and every ``nn.LayerNorm`` over one axis (with weight and bias) in place; the parameters
+    are shared, so an optimizer that holds them keeps working."""
+    for name, child in list(model.named_children()):
+        if type(child) is torch.nn.Linear:
+            setattr(model, name, Linear.from_torch(child))
+        elif type(child) is torch.nn.LayerNorm and len(child.normalized_shape) == 1 and child.weight is not None \
+                and child.bias is not None:
+            setattr(model, name, LayerNorm.from_torch(child))
+        else:
+            replace_dense_modules(child)
     return model

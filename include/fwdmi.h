@@ -327,7 +327,7 @@ int fwdmi_layer_norm_forward(void* stream, int32_t ld, int64_t n, const void* x,
 
 /*
  * Its gradient: dx = dLN(dy) (+ dsum), dgamma, dbeta and, where there is a bias, dbias.
- *   dx is the gradient of x, of skip and of each row's bias alike (dbias sums it over the rows, without dsum);
+ *   dx is the gradient of x, of skip and of each row's bias alike (dbias sums it over the rows, before its rounding);
  *   x / skip / bias as given to the forward call, or x = its `sum` with skip = bias = NULL;
  *   dsum (may be NULL) [rows, ld]: a gradient that reaches the sum from elsewhere;
  *   dgamma, dbeta, dbias fp32 [ld], overwritten (zeros for n == 0); dbias is NULL exactly where bias is.

@@ -98,7 +98,7 @@ def check_backward(s, mean, rstd):
     check(out[2], dy.sum(0), C * U * dy.abs().sum(0), "dbeta")
     assert len(out) == (4 if s["bias"] is not None else 3)
     if s["bias"] is not None:
-        check(out[3], dh.sum(0), (C * U * dh.abs() + bh).sum(0), "dbias")
+        check(out[3], dx.sum(0), (C * U * dx.abs() + bx).sum(0), "dbias")
     return out
 
 
