@@ -16,41 +16,59 @@ struct Operands {
   End end;
 };
 
-// The tile and the number of splits of t with the shortest estimated time.  A CU works off its workgroups' steps, each
-// as long as its loads (direct ones reach 90 KB/us per CU, those through registers 40) or its matrix instructions take
+// The tile and the number of splits of t with the shortest estimated time.  A CU's time is its workgroups' steps: each as
+// long as its loads (direct ones reach 90 KB/us per CU, those through registers 40) or its matrix instructions take
 // (kRate: flop/us per CU that the steps of each tile sustain in bf16, for operands along t or only b across, and both
-// across; fp32 instructions bound all tiles alike), plus what a round of tiles spends outside its steps and, with splits,
-// the second launch and the partial products' way through the caches.  Measured: 8192 x 4096 x 1024 64 us with 256 x 256, 74 with 256 x 128, 84 with 128 x 128;
-// 8192 x 1024 x 4096 (b across) 66 us with 256 x 128, 81 with 128 x 128;
-// 4096 x 1024 x 8192 (both across) 63 us and 15 to add four splits with 256 x 256, 72 and 9 with 256 x 128 and two; 384 x 1024 x 4096 12 us with 64 x 32, 15 with 64 x 64,
-// 20 and more with 128 x 128.
-const double kRate[2][kTileKinds] = {{6.0e6, 4.6e6, 4.0e6, 3.5e6, 3.0e6}, {6.0e6, 4.3e6, 2.2e6, 3.5e6, 3.0e6}};
-const double kRound[kTileKinds] = {9.0, 4.0, 3.0, 1.5, 1.0};
-double step_us(TileKind kind, const Operands& o) {
+// across; in fp32 kStep32, per workgroup when a CU has one and when it has several), plus what a round of tiles spends
+// outside its steps and, with splits, the second launch and the partial products' way through the caches.  Measured, us:
+//   bf16  8192 x 4096 x 1024                  64 with 256 x 256, 74 with 256 x 128, 84 with 128 x 128
+//         8192 x 1024 x 4096, b across        66 with 256 x 128, 81 with 128 x 128
+//         4096 x 1024 x 8192, both across     63 + 13 to add the splits with 256 x 256 and four, 72 + 9 with 256 x 128 and two
+//         384 x 1024 x 4096                   12 with 64 x 32, 15 with 64 x 64, 20 and more with 128 x 128
+//   fp32  512 x 512 x 512                     7 with 32 x 32, 9 with 64 x 32, 13 with 64 x 64
+//         1003 x 517 x 1001                   21 with 32 x 32, 25 with 64 x 64, 28 with 64 x 32
+//         256 x 1024 x 4096                   26 with 64 x 64 and four splits, 27 with 32 x 32 and two, 48 with 32 x 32 alone
+const double kRate[2][kTileKinds] = {{6.0e6, 4.6e6, 4.0e6, 3.5e6, 3.0e6, 2.0e6}, {6.0e6, 4.3e6, 2.2e6, 3.5e6, 3.0e6, 2.0e6}};
+const double kStep32[2][kTileKinds] = {{1e30, 1e30, 2.2, 1.2, 0.8, 0.5}, {1e30, 1e30, 2.1, 1.15, 0.65, 0.36}};
+const double kRound[kTileKinds] = {9.0, 4.0, 3.0, 1.5, 1.0, 1.0};
+// One step of each of `wgs` workgroups on a CU.
+double step_us(TileKind kind, const Operands& o, double wgs) {
   const TileShape t = kTiles[kind];
-  const double load = (t.ti + t.tj) * t.step_bytes / ((o.direct ? 90.0 : 40.0) * 1024);
-  const double flops = 2.0 * t.ti * t.tj * (t.step_bytes / o.elem) / (o.elem == 2 ? kRate[o.layouts == 2][kind] : 0.47e6);
-  return std::max(load, flops);
+  const double load = wgs * (t.ti + t.tj) * t.step_bytes / ((o.direct ? 90.0 : 40.0) * 1024);
+  if (o.elem == 4) return std::max(load, std::max(kStep32[0][kind], wgs * kStep32[1][kind]));
+  return std::max(load, wgs * 2.0 * t.ti * t.tj * (t.step_bytes / 2) / kRate[o.layouts == 2][kind]);
 }
+// A few rows: whole rows of w per workgroup, unless there are so few workgroups and so long rows that a second launch to
+// add splits costs less than it gains.  A CU draws w and x at 38 KB/us through registers: 16 x 4096 x 1024 fp32 takes 16 us
+// on 64 CUs, 9 with four splits and their sum.
+Plan few_plan(int ni, int nj, int nt, int elem) {
+  const int pieces = nt / (128 / elem), wgs = ceil_div(nj, 16);
+  const double us = (16.0 + (ni <= 16 ? 16 : 32)) * nt * elem / (38.0 * 1024);
+  int splits = 1;
+  if (us > 11.0) splits = std::max(1, std::min(std::min(8, device_cus() / wgs), pieces / 16));
+  const int per = std::max(1, ceil_div(pieces, splits));
+  return Plan{kFew, std::max(1, ceil_div(pieces, per)), 0, 0, per, us};
+}
+
 Plan make_plan(int ni, int nj, int nt, const Operands& o) {
-  if (o.layouts == 0 && ni <= kFewRows) return Plan{kFew, 1, 0, 0, 0, 0.0};
+  if (o.layouts == 0 && ni <= kFewRows) return few_plan(ni, nj, nt, o.elem);
   const int cus = device_cus();
   Plan best{};
   double best_us = 1e30;
-  for (int kind = o.elem == 2 && o.direct ? k256x256 : k128x128; kind < kTileKinds; ++kind) {
+  for (int kind = o.elem == 2 && o.direct ? k256x256 : k128x128; kind <= (o.elem == 2 ? k64x32 : k32x32); ++kind) {
     const TileShape t = kTiles[kind];
     Plan p{(TileKind)kind, 1, 0, 0, 0, 0.0};
     tail_of(nt, t.step_bytes / o.elem, o.end, p.whole_steps, p.tail);
     const int all = p.whole_steps + (p.tail > 0);
     const int64_t tiles = (int64_t)ceil_div(ni, t.ti) * ceil_div(nj, t.tj);
-    const double step = step_us((TileKind)kind, o);
     for (int target = 0; target <= 2; ++target) {  // one workgroup per tile, or splits for one or two per CU
       const int64_t want = target == 0 ? 1 : target * (int64_t)cus / tiles;
       if (target > 0 && want < 2) continue;
       const int splits = (int)std::min<int64_t>(want, std::max(1, all / 2));
       p.steps_per_split = std::max(1, ceil_div(all, splits));
       p.splits = std::max(1, ceil_div(all, p.steps_per_split));
-      double us = 2.0 + ceil_div(tiles * p.splits, cus) * (kRound[kind] + p.steps_per_split * step);
+      const double wgs = ceil_div(tiles * p.splits, cus);
+      double us = 2.0 + wgs * kRound[kind] + p.steps_per_split * step_us((TileKind)kind, o, wgs);
       if (p.splits > 1) us += 3.0 + 6.0 * p.splits * ni * nj / 5.0e6;
       if (us < best_us) {
         best_us = us;
@@ -90,9 +108,9 @@ int run(Product& P, int layouts, int dtype, void* workspace, hipStream_t stream)
                                : run_product_f32(P, layouts, plan, o.direct, stream);
 }
 
-// Fills in P as one unsplit pass over 64 x 64 tiles; returns the number of tiles.
-int64_t whole_tiles(Product& P, const Operands& o) {
-  const TileShape t = kTiles[k64x64];
+// Fills in P as one unsplit pass over tiles of `kind`; returns the number of tiles.
+int64_t whole_tiles(Product& P, TileKind kind, const Operands& o) {
+  const TileShape t = kTiles[kind];
   tail_of(P.nt, t.step_bytes / o.elem, o.end, P.whole_steps, P.tail);
   P.steps_per_split = P.whole_steps + (P.tail > 0);
   P.tiles_i = ceil_div(P.ni, t.ti);
@@ -100,28 +118,37 @@ int64_t whole_tiles(Product& P, const Operands& o) {
   return (int64_t)P.tiles_i * P.tiles_j;
 }
 
-// Whether both products of a gradient are faster in one launch of unsplit 64 x 64 tiles than in launches of their own
-// (whose gap is about 3 us), and if so that launch, but for dbias.  771 x 1011 x 768 fp16: 10 and 8 us apart.
+// Whether both products of a gradient are faster in one launch of unsplit tiles than in launches of their own (whose gap
+// is about 3 us), and if so that launch, but for dbias.  771 x 1011 x 768 fp16: 12 us together, 10 and 8 us apart.
 bool together(const Product& x, const Product& w, int dtype, Gradients& G, bool& direct) {
-  const int elem = elem_size(dtype);
+  const int elem = elem_size(dtype), cus = device_cus();
   Operands ox = operands_of(x, 1, elem), ow = operands_of(w, 2, elem);
-  const double apart = make_plan(x.ni, x.nj, x.nt, ox).us + make_plan(w.ni, w.nj, w.nt, ow).us + 3.0;
+  double best = make_plan(x.ni, x.nj, x.nt, ox).us + make_plan(w.ni, w.nj, w.nt, ow).us + 3.0;
   direct = ox.direct && ow.direct;
   if (!direct) {
     ox.direct = ow.direct = false;
     ox.end = ow.end = kTail;
   }
-  G.x = x;
-  G.w = w;
-  const int64_t tx = whole_tiles(G.x, ox), tw = whole_tiles(G.w, ow);
-  const int sx = G.x.steps_per_split, sw = G.w.steps_per_split;
-  const int cus = device_cus();
-  const double rounds = (double)ceil_div(tx + tw, cus);
-  const double steps = std::max<double>(std::max(sx, sw), ((double)tx * sx + (double)tw * sw) / cus);
-  if (2.0 + rounds * kRound[k64x64] + steps * step_us(k64x64, ow) >= apart) return false;
-  G.blocks_x = (int)tx;
-  G.blocks_w = (int)tw;
-  return true;
+  bool found = false;
+  for (TileKind kind : {k64x64, k32x32}) {
+    if (kind == k32x32 && elem == 2) break;
+    Product px = x, pw = w;
+    const int64_t tx = whole_tiles(px, kind, ox), tw = whole_tiles(pw, kind, ow);
+    const int sx = px.steps_per_split, sw = pw.steps_per_split;
+    const double wgs = ceil_div(tx + tw, cus), mean = ((double)tx * sx + (double)tw * sw) / (double)(tx + tw);
+    const double us = 2.0 + wgs * kRound[kind] +
+                      std::max(std::max(sx, sw) * step_us(kind, ow, 1.0), mean * step_us(kind, ow, wgs));
+    if (us < best) {
+      best = us;
+      found = true;
+      G.x = px;
+      G.w = pw;
+      G.tile = kind;
+      G.blocks_x = (int)tx;
+      G.blocks_w = (int)tw;
+    }
+  }
+  return found;
 }
 
 // Partial products of any plan that `run` may choose for these sizes (that depends on the operands' alignment too).

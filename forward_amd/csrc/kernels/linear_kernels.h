@@ -371,6 +371,26 @@ __device__ __forceinline__ F4 multiply(const Frag<T>& b, const Frag<T>& a, F4 ac
   }
 }
 
+// All of a fragment row against all of a fragment column; fp32 goes through one step of t for every accumulator before the
+// next, so that no instruction waits for the sum of the one before it.
+template <typename T, int FI, int FJ>
+__device__ __forceinline__ void multiply_all(const Frag<T> (&b)[FJ], const Frag<T> (&a)[FI], F4 (&acc)[FJ][FI]) {
+  if constexpr (sizeof(T) == 2) {
+#pragma unroll
+    for (int j = 0; j < FJ; ++j)
+#pragma unroll
+      for (int i = 0; i < FI; ++i) acc[j][i] = multiply<T>(b[j], a[i], acc[j][i]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+#pragma unroll
+      for (int j = 0; j < FJ; ++j)
+#pragma unroll
+        for (int i = 0; i < FI; ++i)
+          acc[j][i] = __builtin_amdgcn_mfma_f32_16x16x4f32(b[j].v.v[e], a[i].v.v[e], acc[j][i], 0, 0, 0);
+  }
+}
+
 // The steps of t that a split walks: whole ones from `first` on, and `tail` elements of a last one.
 struct Steps {
   int first, whole, tail;
@@ -574,10 +594,7 @@ __device__ __forceinline__ void Work<T, LA, LB, TI, TJ, WI, WJ, WK, STEP, STAGES
       Frag<T> fa[kFI], fb[kFJ];
       ra.read(now, wk * kHalves + h, fa);
       rb.read(now + TileA::kBytes, wk * kHalves + h, fb);
-#pragma unroll
-      for (int j = 0; j < kFJ; ++j)
-#pragma unroll
-        for (int i = 0; i < kFI; ++i) acc[j][i] = multiply<T>(fb[j], fa[i], acc[j][i]);
+      multiply_all<T>(fb, fa, acc);
     }
   };
   if constexpr (DIRECT) {
@@ -653,11 +670,11 @@ __global__ __launch_bounds__(W::kThreads) void product_kernel(const Product P) {
 }
 
 // Both products of a small gradient and dbias in one launch: workgroups of dx, of dw, and of 64 columns of dbias each.
-template <typename T, bool DIRECT>
-__global__ __launch_bounds__(512) void gradients_kernel(const Gradients G) {
-  using X = Work<T, kAlong, kAcross, 64, 64, 2, 1, 4, 256, 2, DIRECT>;
-  using W = Work<T, kAcross, kAcross, 64, 64, 2, 1, 4, 256, 2, DIRECT>;
-  static_assert(X::kThreads == 512 && W::kThreads == 512 && X::kRoom == W::kRoom, "one shape of workgroup");
+template <typename T, int TILE, bool DIRECT>
+__global__ __launch_bounds__(TILE * 8) void gradients_kernel(const Gradients G) {
+  using X = Work<T, kAlong, kAcross, TILE, TILE, TILE / 32, 1, 4, 256, 2, DIRECT>;
+  using W = Work<T, kAcross, kAcross, TILE, TILE, TILE / 32, 1, 4, 256, 2, DIRECT>;
+  static_assert(X::kThreads == TILE * 8 && W::kThreads == X::kThreads && X::kRoom == W::kRoom, "one shape of workgroup");
   __shared__ __attribute__((aligned(1024))) char s_tile[X::kRoom];
   const int b = (int)blockIdx.x;
   if (b < G.blocks_x) {
@@ -667,8 +684,8 @@ __global__ __launch_bounds__(512) void gradients_kernel(const Gradients G) {
   } else {
     float(*s_red)[64] = reinterpret_cast<float(*)[64]>(s_tile);
     const int64_t c = (int64_t)(b - G.blocks_x - G.blocks_w) * 64 + (threadIdx.x & 63);
-    const float a = G.part ? column_sum<float, 8>(G.part, G.parts, G.n, c, s_red)
-                           : column_sum<T, 8>(static_cast<const T*>(G.dy), G.parts, G.n, c, s_red);
+    const float a = G.part ? column_sum<float, TILE / 8>(G.part, G.parts, G.n, c, s_red)
+                           : column_sum<T, TILE / 8>(static_cast<const T*>(G.dy), G.parts, G.n, c, s_red);
     if (threadIdx.x < 64 && c < G.n) gmut<float>(G.dbias)[c] = a;
   }
 }
@@ -784,7 +801,7 @@ __global__ __launch_bounds__(512) void product_turns_kernel(const Product P) {
 // A few rows (at most 16 MB tokens) through a matrix of weights: one pass over w.  A workgroup takes 16 rows of w and
 // all of x; its waves take 128-byte pieces of t in turn, straight from memory to the matrix instructions (a piece is
 // read by one wave alone, LDS would only add a stop), two pieces in flight, and their sums meet in LDS in wave order.
-// Rows past the last repeat it, their products are dropped.
+// Rows past the last repeat it, their products are dropped.  blockIdx.y: splits of the pieces (few rows of w, long ones).
 template <typename T, int MB>
 __global__ __launch_bounds__(1024) void product_few_kernel(const Product P) {
   extern __shared__ __attribute__((aligned(16))) F4 s_sum[];  // [waves][MB][64]
@@ -800,7 +817,7 @@ __global__ __launch_bounds__(1024) void product_few_kernel(const Product P) {
 #pragma unroll
   for (int b = 0; b < MB; ++b) acc[b] = F4{0.0f, 0.0f, 0.0f, 0.0f};
 
-  const int pieces = P.nt / kPiece;
+  const int split = (int)blockIdx.y, pieces = min(P.nt / kPiece, (split + 1) * P.steps_per_split);
   constexpr int kBatch = 2;
   auto batch = [&](int piece, auto count) {
     constexpr int kN = decltype(count)::value;
@@ -821,10 +838,11 @@ __global__ __launch_bounds__(1024) void product_few_kernel(const Product P) {
 #pragma unroll
         for (int b = 0; b < MB; ++b) acc[b] = multiply<T>(w[k][h], x[k][h][b], acc[b]);
   };
-  int piece = wave;
+  int piece = split * P.steps_per_split + wave;
   for (; piece + (kBatch - 1) * waves < pieces; piece += kBatch * waves) batch(piece, std::integral_constant<int, kBatch>{});
   for (; piece < pieces; piece += waves) batch(piece, std::integral_constant<int, 1>{});
-  if (piece == pieces && P.nt % kPiece != 0) {  // the wave whose turn it is takes what is left, element by element
+  // the wave whose turn it is in the last split takes what is left, element by element
+  if (piece == pieces && split + 1 == (int)gridDim.y && P.nt % kPiece != 0) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int t = pieces * kPiece + h * kHalf, n = P.nt - t - g * kChunk<T>;
@@ -850,7 +868,11 @@ __global__ __launch_bounds__(1024) void product_few_kernel(const Product P) {
       for (int e = 0; e < 4; ++e) v[e] += part[e];
     }
     const int i = wave * 16 + r, j = j0 + g * 4;
-    if (i < P.ni && j < P.nj) {
+    if (P.partial && i < P.ni) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (j + e < P.nj) gmut<float>(P.partial)[((int64_t)split * P.ni + i) * P.nj + j + e] = v[e];
+    } else if (i < P.ni && j < P.nj) {
       float b[4];
       load_bias(P, j, b);
       with_act(P.act, [&](auto act) { finish<T, decltype(act)::value, false>(P, i, j, v, b); });
@@ -957,19 +979,28 @@ __global__ __launch_bounds__(256) void slope_kernel(const Slope S) {
   }
 }
 
+template <typename T>
+int launch_finish(const Product& P, int splits, hipStream_t stream) {
+  const int64_t octets = (int64_t)P.ni * ((P.nj + 7) / 8);
+  hipLaunchKernelGGL((finish_kernel<T>), dim3((unsigned)ceil_div(octets, 256)), dim3(256), 0, stream, P, splits);
+  FWDMI_HIP_CHECK(hipGetLastError());
+  return FWDMI_OK;
+}
+
 template <typename T, int LA, int LB, bool DIRECT>
 int launch_product(Product& P, const Plan& plan, hipStream_t stream) {
   if constexpr (LA == kAlong && LB == kAlong) {
     if (plan.tile == kFew) {
-      const int pieces = P.nt / (128 / (int)sizeof(T));
+      const int pieces = plan.steps_per_split;
       const int waves = pieces >= 32 ? 16 : pieces >= 16 ? 8 : 4;
-      const dim3 grid((unsigned)ceil_div(P.nj, 16)), block(64 * waves);
+      P.steps_per_split = pieces;
+      const dim3 grid((unsigned)ceil_div(P.nj, 16), (unsigned)plan.splits), block(64 * waves);
       if (P.ni <= 16)
         hipLaunchKernelGGL((product_few_kernel<T, 1>), grid, block, waves * 1024, stream, P);
       else
         hipLaunchKernelGGL((product_few_kernel<T, 2>), grid, block, waves * 2048, stream, P);
       FWDMI_HIP_CHECK(hipGetLastError());
-      return FWDMI_OK;
+      return plan.splits > 1 ? launch_finish<T>(P, plan.splits, stream) : FWDMI_OK;
     }
   }
   const TileShape tile = kTiles[plan.tile];
@@ -992,13 +1023,12 @@ int launch_product(Product& P, const Plan& plan, hipStream_t stream) {
   if (plan.tile == k64x32)
     hipLaunchKernelGGL((product_kernel<Work<T, LA, LB, 64, 32, 2, 1, 4, 256, DIRECT ? 4 : 2, DIRECT>>), grid, dim3(512), 0,
                        stream, P);
-  FWDMI_HIP_CHECK(hipGetLastError());
-  if (plan.splits > 1) {
-    const int64_t octets = (int64_t)P.ni * ((P.nj + 7) / 8);
-    hipLaunchKernelGGL((finish_kernel<T>), dim3((unsigned)ceil_div(octets, 256)), dim3(256), 0, stream, P, plan.splits);
-    FWDMI_HIP_CHECK(hipGetLastError());
+  if constexpr (sizeof(T) == 4) {
+    if (plan.tile == k32x32)
+      hipLaunchKernelGGL((product_kernel<Work<T, LA, LB, 32, 32, 1, 1, 4, 256, 2, DIRECT>>), grid, dim3(256), 0, stream, P);
   }
-  return FWDMI_OK;
+  FWDMI_HIP_CHECK(hipGetLastError());
+  return plan.splits > 1 ? launch_finish<T>(P, plan.splits, stream) : FWDMI_OK;
 }
 
 template <typename T, bool DIRECT>
@@ -1014,10 +1044,20 @@ int run_product(Product& P, int layouts, const Plan& plan, bool direct, hipStrea
 template <typename T>
 int run_gradients(const Gradients& G, bool direct, hipStream_t stream) {
   const dim3 grid((unsigned)(G.blocks_x + G.blocks_w + (G.dbias ? ceil_div(G.n, 64) : 0)));
-  if (direct)
-    hipLaunchKernelGGL((gradients_kernel<T, true>), grid, dim3(512), 0, stream, G);
-  else
-    hipLaunchKernelGGL((gradients_kernel<T, false>), grid, dim3(512), 0, stream, G);
+  if (G.tile == k64x64) {
+    if (direct)
+      hipLaunchKernelGGL((gradients_kernel<T, 64, true>), grid, dim3(512), 0, stream, G);
+    else
+      hipLaunchKernelGGL((gradients_kernel<T, 64, false>), grid, dim3(512), 0, stream, G);
+  }
+  if constexpr (sizeof(T) == 4) {
+    if (G.tile == k32x32) {
+      if (direct)
+        hipLaunchKernelGGL((gradients_kernel<T, 32, true>), grid, dim3(256), 0, stream, G);
+      else
+        hipLaunchKernelGGL((gradients_kernel<T, 32, false>), grid, dim3(256), 0, stream, G);
+    }
+  }
   FWDMI_HIP_CHECK(hipGetLastError());
   return FWDMI_OK;
 }

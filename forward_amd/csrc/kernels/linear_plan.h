@@ -40,14 +40,16 @@ struct Slope {
   int32_t act;
 };
 
-// The tiles there are.  The first two are the eight-wave kernel of 16-bit operands (product_turns_kernel).
+// The tiles there are.  The first two are the eight-wave kernel of 16-bit operands (product_turns_kernel), the last is
+// for fp32 operands.
 // kFew: product_few_kernel, at most kFewRows rows of x.
-enum TileKind { k256x256, k256x128, k128x128, k64x64, k64x32, kTileKinds, kFew = kTileKinds };
+enum TileKind { k256x256, k256x128, k128x128, k64x64, k64x32, k32x32, kTileKinds, kFew = kTileKinds };
 constexpr int kFewRows = 32;
 struct TileShape {
   int ti, tj, step_bytes;
 };
-constexpr TileShape kTiles[kTileKinds] = {{256, 256, 128}, {256, 128, 128}, {128, 128, 128}, {64, 64, 256}, {64, 32, 256}};
+constexpr TileShape kTiles[kTileKinds] = {{256, 256, 128}, {256, 128, 128}, {128, 128, 128}, {64, 64, 256}, {64, 32, 256},
+                                                {32, 32, 256}};
 
 struct Plan {
   TileKind tile;
@@ -55,10 +57,11 @@ struct Plan {
   double us;  // estimate
 };
 
-// Both products of a gradient, unsplit and in 64 x 64 tiles, and the sums of its columns.
+// Both products of a gradient, unsplit and in tiles of one size, and the sums of its columns.
 struct Gradients {
   Product x, w;
   int32_t blocks_x, blocks_w;
+  TileKind tile;      // k64x64 or k32x32
   float* dbias;       // nullable
   const float* part;  // its partials [parts][n], or
   const void* dy;     // without partials, dy itself [parts][n]
