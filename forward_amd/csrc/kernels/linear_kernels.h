@@ -109,12 +109,11 @@ __device__ __forceinline__ void load_bias(const Product& P, int j, float (&b)[N]
   }
 }
 
-// y = act(z) + residual, z = acc + bias, of N neighbours of one row: columns j .. j + N - 1, all of them (WHOLE) or
-// those below nj.
-template <typename T, int ACT, bool WHOLE, int N>
+// y = act(z) + residual, z = acc + bias, of N neighbours of one row: those of columns j .. j + N - 1 that are below nj.
+template <typename T, int ACT, int N>
 __device__ __forceinline__ void finish(const Product& P, int64_t i, int j, const float (&acc)[N], const float (&b)[N]) {
   const int64_t at = i * P.nj + j;
-  const int live = WHOLE ? N : min(P.nj - j, N);
+  const int live = min(P.nj - j, N);
   Pack<T, N> y, z, r{};
   if (P.residual) {
     if (live == N) {
@@ -489,22 +488,21 @@ __device__ __forceinline__ void leave_tile(const Product& P, const F4 (&acc)[FJ]
         leave([&](int64_t i, int j, const float (&v)[8]) {
           float b[8];
           load_bias(P, j, b);
-          finish<T, decltype(act)::value, false>(P, i, j, v, b);
+          finish<T, decltype(act)::value>(P, i, j, v, b);
         });
       });
     } else {  // the gradient's products have no epilogue
       leave([&](int64_t i, int j, const float (&v)[8]) {
         const float b[8] = {};
-        finish<T, FWDMI_ACT_NONE, false>(P, i, j, v, b);
+        finish<T, FWDMI_ACT_NONE>(P, i, j, v, b);
       });
     }
   }
 }
 
-// A tile whose columns all exist leaves straight from the accumulators.  A lane holds four neighbouring columns of
-// blocks 2 p and 2 p + 1; exchanges between the lane rows (16 lanes each) give it eight neighbouring columns of one
-// block, so that a store instruction writes 64 contiguous bytes of each of its 16 rows: no LDS, no barrier, and the two
-// waves of a SIMD overlap each other's arithmetic and stores.
+// A tile of 16-bit results whose columns all exist leaves straight from the accumulators: no LDS, no barrier, and the two
+// waves of a SIMD overlap each other's arithmetic and stores.  A lane holds four neighbouring columns of blocks 2 p and
+// 2 p + 1; exchanges between the lane rows (16 lanes each) give it eight neighbouring columns of one block.
 template <typename T, int TI, int TJ, int WI, int WJ, bool EPILOGUE, int FI, int FJ>
 __device__ __forceinline__ void leave_registers(const Product& P, const F4 (&acc)[FJ][FI], int i0, int j0, int split) {
   const int lane = threadIdx.x & 63, g = lane >> 4;
@@ -537,19 +535,60 @@ __device__ __forceinline__ void leave_registers(const Product& P, const F4 (&acc
       v[e + 4] = __uint_as_float(b[1]);
     }
   };
+  static_assert(sizeof(T) == 2 && FJ == 4, "two slices of 16 bytes per lane and row");
+  const bool second = (lane & 8) != 0;
+  const int row = i_lane - (lane & 15) + (lane & 7), col = j_lane + (second ? 32 : 0);
+  // Slices 0 and 1 of 16 rows, every lane with its row's: lanes eight apart trade one each, so that each store writes whole
+  // 128-byte lines of eight rows (half lines cost 8 % more time where the results go to memory).
+  auto store_rows = [&](void* to, int i, const Pack<T, 8> (&v)[2]) {
+    uint32_t u[2][4];
+    __builtin_memcpy(u, v, 32);
+    uint32_t low[4], high[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const uint32_t other0 = __builtin_amdgcn_update_dpp(0, (int)u[0][k], 0x128, 0xf, 0xf, true);  // of the row eight on
+      const uint32_t other1 = __builtin_amdgcn_update_dpp(0, (int)u[1][k], 0x128, 0xf, 0xf, true);
+      low[k] = second ? other1 : u[0][k];
+      high[k] = second ? u[1][k] : other0;
+    }
+    Pack<T, 8> o;
+    T FWDMI_GLOBAL* const at = gmut<T>(to) + (int64_t)(row + i * 16) * P.nj + col;
+    if (row + i * 16 < P.ni) {
+      __builtin_memcpy(&o, low, 16);
+      store_slice<T, 8>(at, o);
+    }
+    if (row + i * 16 + 8 < P.ni) {
+      __builtin_memcpy(&o, high, 16);
+      store_slice<T, 8>(at + 8 * (int64_t)P.nj, o);
+    }
+  };
   with_act(EPILOGUE ? P.act : FWDMI_ACT_NONE, [&](auto act) {
     if (!EPILOGUE && decltype(act)::value != FWDMI_ACT_NONE) return;
+    float b[2][8] = {};
+    if (EPILOGUE)
 #pragma unroll
-    for (int p = 0; p < FJ / 2; ++p) {
-      const int j = j_lane + p * 32;
-      float b[8] = {};
-      if (EPILOGUE) load_bias(P, j, b);
+      for (int p = 0; p < 2; ++p) load_bias(P, j_lane + p * 32, b[p]);
 #pragma unroll
-      for (int i = 0; i < FI; ++i) {
+    for (int i = 0; i < FI; ++i) {
+      const int ii = i_lane + i * 16;
+      Pack<T, 8> y[2], z[2], r[2] = {};
+      if (EPILOGUE && P.residual && ii < P.ni)
+#pragma unroll
+        for (int p = 0; p < 2; ++p)
+          r[p] = load_slice<T, 8>(gconst<T>(P.residual) + (int64_t)ii * P.nj + j_lane + p * 32);
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
         float v[8];
         eight(p, i, v);
-        if (i_lane + i * 16 < P.ni) finish<T, decltype(act)::value, true>(P, i_lane + i * 16, j, v, b);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float s = v[e] + b[p][e];
+          z[p].v[e] = (T)s;
+          y[p].v[e] = (T)(activate<decltype(act)::value, false>(s) + (float)r[p].v[e]);
+        }
       }
+      store_rows(P.c, i, y);
+      if (EPILOGUE && P.preact) store_rows(P.preact, i, z);
     }
   });
 }
@@ -875,7 +914,7 @@ __global__ __launch_bounds__(1024) void product_few_kernel(const Product P) {
     } else if (i < P.ni && j < P.nj) {
       float b[4];
       load_bias(P, j, b);
-      with_act(P.act, [&](auto act) { finish<T, decltype(act)::value, false>(P, i, j, v, b); });
+      with_act(P.act, [&](auto act) { finish<T, decltype(act)::value>(P, i, j, v, b); });
     }
   }
 }
@@ -919,7 +958,7 @@ __global__ __launch_bounds__(256) void finish_kernel(const Product P, int splits
   }
   float b[8];
   load_bias(P, j, b);
-  with_act(P.act, [&](auto act) { finish<T, decltype(act)::value, false>(P, i, j, acc, b); });
+  with_act(P.act, [&](auto act) { finish<T, decltype(act)::value>(P, i, j, acc, b); });
 }
 
 // ---- dz = dy * act'(z) and its column sums -----------------------------------------------------------------------
