@@ -681,6 +681,8 @@ bool with_shape(int ld, F&& f) {
 }
 
 // Rows of more than 16 elements per lane, or streamed: column sums by ln_backward_columns_kernel.
+constexpr int32_t kMaxLd = 1 << 30;  // column numbers stay in 31 bits a slice past the row's end
+
 bool long_rows(int ld, int dtype) {
   const int vec = dtype == FWDMI_F32 ? 4 : 8;
   if (ld < vec) return false;
@@ -741,7 +743,7 @@ int fwdmi_layer_norm_forward(void* stream, int32_t ld, int64_t n, const void* x,
   using namespace fwdmi;
   clear_error();
   if (!is_train_dtype(dtype)) return set_error(FWDMI_ERR_UNSUPPORTED, "layer norm forward: unsupported dtype %d", dtype);
-  FWDMI_REQUIRE(ld > 0 && n >= 0 && n % ld == 0, "layer norm forward: n=%lld is not a multiple of ld=%d", (long long)n, ld);
+  FWDMI_REQUIRE(ld > 0 && ld <= kMaxLd && n >= 0 && n % ld == 0, "layer norm forward: n=%lld is not a multiple of ld=%d (at most 2^30)", (long long)n, ld);
   if (n == 0) return FWDMI_OK;
   FWDMI_REQUIRE(x && beta && gamma && y && mean && rstd, "layer norm forward: null pointer");
   LnTrain L{};
@@ -765,7 +767,7 @@ int fwdmi_layer_norm_forward(void* stream, int32_t ld, int64_t n, const void* x,
 
 size_t fwdmi_layer_norm_backward_workspace(int32_t ld, int64_t n, int32_t dtype) {
   using namespace fwdmi;
-  if (!is_train_dtype(dtype) || ld <= 0 || n <= 0 || n % ld != 0) return 0;
+  if (!is_train_dtype(dtype) || ld <= 0 || ld > kMaxLd || n <= 0 || n % ld != 0) return 0;
   const int64_t rows = n / ld;
   size_t bytes = (size_t)backward_parts(ld, rows, dtype) * 3 * (size_t)ld * sizeof(float);
   if (long_rows(ld, dtype)) bytes += (size_t)rows * 2 * sizeof(float);
@@ -779,7 +781,7 @@ int fwdmi_layer_norm_backward(void* stream, int32_t ld, int64_t n, const void* d
   using namespace fwdmi;
   clear_error();
   if (!is_train_dtype(dtype)) return set_error(FWDMI_ERR_UNSUPPORTED, "layer norm backward: unsupported dtype %d", dtype);
-  FWDMI_REQUIRE(ld > 0 && n >= 0 && n % ld == 0, "layer norm backward: n=%lld is not a multiple of ld=%d", (long long)n, ld);
+  FWDMI_REQUIRE(ld > 0 && ld <= kMaxLd && n >= 0 && n % ld == 0, "layer norm backward: n=%lld is not a multiple of ld=%d (at most 2^30)", (long long)n, ld);
   FWDMI_REQUIRE(dgamma && dbeta && (bias == nullptr) == (dbias == nullptr),
                 "layer norm backward: dgamma and dbeta are written always, dbias exactly where there is a bias");
   const int64_t rows = n / ld;

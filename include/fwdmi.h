@@ -318,7 +318,7 @@ int fwdmi_emb_layer_norm_ex(void* stream, int32_t S, int32_t B, int32_t ld, cons
  *   sum (may be NULL) [rows, ld] in `dtype`: h rounded once, for layers whose residual stream goes on unnormalised
  *   (y is computed from the unrounded h);
  *   mean, rstd fp32 [rows];  gamma / beta / bias fp32 [ld], bias may be NULL.
- * Operands need the alignment of their elements only; outputs overlap neither each other nor an input.
+ * Operands need the alignment of their elements only; outputs overlap neither each other nor an input.  ld <= 2^30.
  * (The reference is an inference engine and has no counterpart of this and the next launcher.)
  */
 int fwdmi_layer_norm_forward(void* stream, int32_t ld, int64_t n, const void* x, const void* skip, const float* beta,
@@ -346,7 +346,7 @@ int fwdmi_layer_norm_backward(void* stream, int32_t ld, int64_t n, const void* d
  *   x [m, k], w [n, k], residual [m, n] (may be NULL), y [m, n] in `dtype` (FWDMI_F32 | FWDMI_F16 | FWDMI_BF16),
  *   packed rows; bias fp32 [n] or NULL; preact (may be NULL) [m, n]: z rounded to `dtype`, what the backward pass
  *   reads; act: FWDMI_ACT_*.  Sums, activation and residual are fp32, rounded once.
- * Any sizes up to 2^30 each and any element alignment; operands of whole 16-byte lines (k a multiple of 8, fp32 4,
+ * Any sizes up to 2^30 each (2^40 for a product of two) and any element alignment; operands of whole 16-byte lines (k a multiple of 8, fp32 4,
  * and pointers of 16) are the fast ones.  Outputs overlap neither each other nor an input.
  * `workspace`: fwdmi_linear_workspace(m, n, k, dtype) bytes (often 0) on a 16-byte boundary, used by this call alone
  * until it has run on `stream` (calls in flight together need one each).

@@ -121,3 +121,40 @@ def test_linear_workspace_sizes():
     # dz and the column sums' partials at least
     assert d.fwdmi_linear_backward_workspace(100, 64, 64, lib.ACT_GELU, lib.F16) >= 100 * 64 * 2 + 64 * 4
     assert d.fwdmi_linear_backward_workspace(0, 64, 64, lib.ACT_GELU, lib.F16) == 0
+
+
+@pytest.mark.skipif(lib.dll.fwdmi_device_count() > 0, reason="made-up addresses: only where nothing can be launched")
+def test_arguments_at_the_ends_of_their_types_return_a_status():
+    """Every call below returns: refused, nothing to do, or (no device here) a launch that the runtime turns down; and the
+    workspace sizes neither wrap round nor fall short of what a call then asks for."""
+    import itertools
+    import random
+    rng = random.Random(3)
+    d = lib.dll
+    ends = [0, 1, 2, 7, 8, 63, 64, 1000, 4095, 1 << 16, (1 << 30) - 1, 1 << 30, (1 << 30) + 1, (1 << 31) - 1, (1 << 62), -1, -(1 << 62)]
+    dtypes = [lib.F32, lib.F16, lib.BF16, lib.I8, lib.I64, -5, 1 << 30]
+    allowed = {lib.OK, lib.ERR_BAD_ARG, lib.ERR_UNSUPPORTED, lib.ERR_HIP}
+    p = 1 << 20
+    for m, n, k in itertools.chain(itertools.product(ends, repeat=3), ((rng.choice(ends) + rng.randint(-3, 3),) * 3 for _ in range(500))):
+        dt = rng.choice(dtypes)
+        size = d.fwdmi_linear_workspace(m, n, k, dt)
+        back = d.fwdmi_linear_backward_workspace(m, n, k, rng.choice([0, 2]), dt)
+        assert size < 1 << 60 and back < 1 << 60
+        rc = d.fwdmi_linear(None, m, n, k, p, p, p, p, p, p, rng.choice([0, 1, 2, 3, 4, 5, -1]), dt, p, (1 << 64) - 1)
+        assert rc in allowed
+        if rc == lib.ERR_HIP and size:
+            assert d.fwdmi_linear(None, m, n, k, p, p, p, p, p, p, 0, dt, p, size - 1) == lib.ERR_BAD_ARG
+            assert d.fwdmi_linear(None, m, n, k, p, p, p, p, p, p, 0, dt, p, size) == lib.ERR_HIP
+        rc = d.fwdmi_linear_backward(None, m, n, k, p, p, p, p, p, p, p, rng.choice([0, 1, 2, 3, 4, 5, -1]), dt, p, (1 << 64) - 1)
+        assert rc in allowed
+    for ld, rows in itertools.product([e for e in ends if abs(e) < 1 << 31], ends):
+        n = ld * rows
+        if abs(n) >= 1 << 63:
+            continue
+        dt = rng.choice(dtypes)
+        assert d.fwdmi_layer_norm_forward(None, ld, n, *[p] * 9, dt, 1e-5) in allowed
+        size = d.fwdmi_layer_norm_backward_workspace(ld, n, dt)
+        rc = d.fwdmi_layer_norm_backward(None, ld, n, *[p] * 12, p, (1 << 64) - 1, dt)
+        assert rc in allowed
+        if rc == lib.ERR_HIP and size:
+            assert d.fwdmi_layer_norm_backward(None, ld, n, *[p] * 12, p, size - 1, dt) == lib.ERR_BAD_ARG
