@@ -51,6 +51,7 @@ struct LnTrain {
   int64_t part_stride;
   int64_t rows;
   int32_t ld;
+  int32_t row_blocks;  // backward: workgroups of rows; those behind them sum columns (see ln_columns)
   float eps;
 };
 
@@ -215,15 +216,83 @@ __global__ __launch_bounds__(WG) void ln_forward_kernel(const LnTrain L) {
   }
 }
 
+// gamma's and beta's gradients of 64 columns straight from dy and x, whose mean and rstd are known: for few rows, whose
+// column sums then need no partials and no second launch.  A lane takes 16 bytes of a row, the lanes of a wave several
+// rows; their sums are added across the lanes of a column, then across the waves, in a fixed order.
+template <typename T, int WG>
+__device__ __forceinline__ void ln_columns(const LnTrain& L, int block, float (*s_sum)[2][64]) {
+  constexpr int kVec = 16 / sizeof(T), kLanes = 64 / kVec, kWaveRows = 64 / kLanes, kRows = WG / 64 * kWaveRows;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t c = (int64_t)block * 64 + lane % kLanes * kVec;
+  const int live = (int)min((int64_t)kVec, max((int64_t)L.ld - c, (int64_t)0));
+  float sg[kVec] = {}, sb[kVec] = {};
+  auto some = [&](const void* p, int64_t at) {
+    Pack<T, kVec> v{};
+    if (live == kVec) {
+      v = load_slice<T, kVec>(gconst<T>(p) + at);
+    } else {
+#pragma unroll
+      for (int e = 0; e < kVec; ++e)
+        if (e < live) v.v[e] = gconst<T>(p)[at + e];
+    }
+    return v;
+  };
+  if (live > 0) {
+#pragma unroll 4
+    for (int64_t r = wave * kWaveRows + lane / kLanes; r < L.rows; r += kRows) {
+      const int64_t at = r * L.ld + c;
+      const float mu = gconst<float>(L.mean)[r], rs = gconst<float>(L.rstd)[r];
+      const Pack<T, kVec> dy = some(L.dy, at), x = some(L.x, at);
+      Pack<T, kVec> s{};
+      if (L.skip) s = some(L.skip, at);
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) {
+        float h = (float)x.v[e];
+        if (L.skip) h += (float)s.v[e];
+        const float w = (float)dy.v[e];
+        sg[e] = __builtin_fmaf(w, (h - mu) * rs, sg[e]);
+        sb[e] += w;
+      }
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < kVec; ++e) {
+#pragma unroll
+    for (int m = kLanes; m < 64; m <<= 1) {
+      sg[e] += __shfl_xor(sg[e], m);
+      sb[e] += __shfl_xor(sb[e], m);
+    }
+    if (lane < kLanes) {
+      s_sum[wave][0][lane * kVec + e] = sg[e];
+      s_sum[wave][1][lane * kVec + e] = sb[e];
+    }
+  }
+  __syncthreads();
+  const int kind = (int)threadIdx.x >> 6, col = (int)threadIdx.x & 63;
+  if (kind < 2 && (int64_t)block * 64 + col < L.ld) {
+    float a = s_sum[0][kind][col];
+#pragma unroll
+    for (int k = 1; k < WG / 64; ++k) a += s_sum[k][kind][col];
+    gmut<float>(kind == 0 ? L.part_gamma : L.part_beta)[(int64_t)block * 64 + col] = a;
+  }
+}
+
 // SUMS: the column sums ride along in registers.  Rows of more than 16 elements per lane have none left for them
 // (2700 x 12288 fp16 took 164 us with the sums spilled): those leave c1 and c2 and ln_backward_columns_kernel reads dy and
-// x once more.
+// x once more.  Without sums and without a bias the launch may hold workgroups that sum columns (ln_columns).
 template <typename T, int VEC, int NV, int WG, int LPR, bool FULL, bool BIAS, bool SUMS>
 __global__ __launch_bounds__(WG) void ln_backward_kernel(const LnTrain L) {
   constexpr int kRows = WG / LPR;
   constexpr int kSlots = LPR * NV * VEC;  // elements of a row, as the lanes hold them
   __shared__ float s_red[4 * (WG / 64)];
   __shared__ float s_col[LPR < WG && SUMS ? kRows * kSlots : 1];
+  if constexpr (!SUMS && !BIAS) {
+    if ((int)blockIdx.x >= L.row_blocks) {
+      __shared__ float s_sum[WG / 64][2][64];
+      ln_columns<T, WG>(L, (int)blockIdx.x - L.row_blocks, s_sum);
+      return;
+    }
+  }
   const int gl = threadIdx.x % LPR;
   const int group = threadIdx.x / LPR;
   const Columns<VEC, NV, LPR, FULL> C(gl, L.ld);
@@ -249,7 +318,7 @@ __global__ __launch_bounds__(WG) void ln_backward_kernel(const LnTrain L) {
     }
   };
 
-  const int64_t step = (int64_t)gridDim.x * kRows;
+  const int64_t step = (int64_t)L.row_blocks * kRows;
   const int64_t first = (int64_t)blockIdx.x * kRows;
   fetch(first + group);
   float g[NV][VEC], bi[NV][VEC], sum_g[NV][VEC], sum_b[NV][VEC], sum_h[NV][VEC];
@@ -317,7 +386,7 @@ __global__ __launch_bounds__(WG) void ln_backward_kernel(const LnTrain L) {
       }
     }
     const float c1 = a1 * inv_n, c2 = a2 * inv_n;
-    if (!SUMS && row_ok && gl == 0) {
+    if (!SUMS && L.c1 && row_ok && gl == 0) {
       gmut<float>(L.c1)[r] = c1;
       gmut<float>(L.c2)[r] = c2;
     }
@@ -625,6 +694,16 @@ int launch_forward(const LnTrain& L, hipStream_t stream) {
 
 template <typename T, int VEC, int NV, int LPR>
 int launch_backward(const LnTrain& L, unsigned grid, hipStream_t stream) {
+  if ((int)grid > L.row_blocks) {  // with workgroups that sum columns
+    if (L.ld == LPR * VEC * NV)
+      hipLaunchKernelGGL((ln_backward_kernel<T, VEC, NV, kBackwardWG, LPR, true, false, false>), dim3(grid),
+                         dim3(kBackwardWG), 0, stream, L);
+    else
+      hipLaunchKernelGGL((ln_backward_kernel<T, VEC, NV, kBackwardWG, LPR, false, false, false>), dim3(grid),
+                         dim3(kBackwardWG), 0, stream, L);
+    FWDMI_HIP_CHECK(hipGetLastError());
+    return FWDMI_OK;
+  }
   constexpr bool kSums = NV * VEC <= 16;
 #define FWDMI_LN_LAUNCH(FULL_, BIAS_)                                                                          \
   hipLaunchKernelGGL((ln_backward_kernel<T, VEC, NV, kBackwardWG, LPR, FULL_, BIAS_, kSums>), dim3(grid),      \
@@ -690,14 +769,26 @@ bool long_rows(int ld, int dtype) {
   return s.lpr == 0 || s.nv * vec > 16;
 }
 
-// Rows of partials of a backward call.
-int64_t backward_parts(int ld, int64_t rows, int dtype) {
-  if (rows == 0) return 0;
-  if (long_rows(ld, dtype)) return std::min<int64_t>((rows + 3) / 4, kLongParts);
+// Workgroups of rows of a backward call with column sums in registers.
+int64_t row_groups(int ld, int64_t rows, int dtype) {
   const int vec = dtype == FWDMI_F32 ? 4 : 8;
   const Shape s = ld < vec ? Shape{8, 1} : row_shape(ld, vec);
   const int per = kBackwardWG / s.lpr;
-  return std::min<int64_t>((rows + per - 1) / per, kMaxParts);
+  return (rows + per - 1) / per;
+}
+
+// Few rows of more than one workgroup, no bias: rows and column sums in one launch (509 x 768 fp32: 6 us; 5 and 3 us in
+// two launches, and 5 us less on the host).
+constexpr int64_t kFewRows = 1024;
+bool joint_rows(int ld, int64_t rows, int dtype, bool bias) {
+  return !bias && rows <= kFewRows && !long_rows(ld, dtype) && row_groups(ld, rows, dtype) > 1;
+}
+
+// Rows of partials of a backward call.
+int64_t backward_parts(int ld, int64_t rows, int dtype, bool bias) {
+  if (rows == 0 || joint_rows(ld, rows, dtype, bias)) return 0;
+  if (long_rows(ld, dtype)) return std::min<int64_t>((rows + 3) / 4, kLongParts);
+  return std::min<int64_t>(row_groups(ld, rows, dtype), kMaxParts);
 }
 
 template <typename T>
@@ -714,9 +805,17 @@ int forward_typed(const LnTrain& L, hipStream_t stream) {
 }
 
 template <typename T>
-int backward_typed(const LnTrain& L, int64_t parts, bool long_row, hipStream_t stream) {
+int backward_typed(LnTrain& L, int64_t parts, bool long_row, hipStream_t stream) {
   int rc = FWDMI_OK;
-  const int64_t grid = long_row ? std::min<int64_t>(L.rows, (int64_t)device_cus() * 2) : parts;
+  int64_t grid = parts;
+  if (parts == 0) {
+    const int dtype = sizeof(T) == 4 ? FWDMI_F32 : FWDMI_F16;
+    L.row_blocks = (int)row_groups(L.ld, L.rows, dtype);
+    grid = L.row_blocks + ((int64_t)L.ld + 63) / 64;
+  } else {
+    if (long_row) grid = std::min<int64_t>(L.rows, (int64_t)device_cus() * 2);
+    L.row_blocks = (int)grid;
+  }
   const bool done = with_shape<T>(L.ld, [&](auto vec, auto nv, auto lpr) {
     rc = launch_backward<T, decltype(vec)::value, decltype(nv)::value, decltype(lpr)::value>(L, (unsigned)grid, stream);
   });
@@ -765,11 +864,12 @@ int fwdmi_layer_norm_forward(void* stream, int32_t ld, int64_t n, const void* x,
   return forward_typed<float>(L, s);
 }
 
-size_t fwdmi_layer_norm_backward_workspace(int32_t ld, int64_t n, int32_t dtype) {
+size_t fwdmi_layer_norm_backward_workspace(int32_t ld, int64_t n, int32_t with_bias, int32_t dtype) {
   using namespace fwdmi;
   if (!is_train_dtype(dtype) || ld <= 0 || ld > kMaxLd || n <= 0 || n % ld != 0) return 0;
   const int64_t rows = n / ld;
-  size_t bytes = (size_t)backward_parts(ld, rows, dtype) * 3 * (size_t)ld * sizeof(float);
+  const int64_t parts = backward_parts(ld, rows, dtype, with_bias != 0);
+  size_t bytes = parts > 1 ? (size_t)parts * (with_bias ? 3 : 2) * (size_t)ld * sizeof(float) : 0;
   if (long_rows(ld, dtype)) bytes += (size_t)rows * 2 * sizeof(float);
   return bytes;
 }
@@ -787,12 +887,12 @@ int fwdmi_layer_norm_backward(void* stream, int32_t ld, int64_t n, const void* d
   const int64_t rows = n / ld;
   const int kinds = bias ? 3 : 2;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const int64_t parts = backward_parts(ld, rows, dtype);
+  const int64_t parts = backward_parts(ld, rows, dtype, bias != nullptr);
   LnTrain L{};
   if (rows > 0) {
     FWDMI_REQUIRE(dy && x && gamma && mean && rstd && dx, "layer norm backward: null pointer");
-    const size_t need = fwdmi_layer_norm_backward_workspace(ld, n, dtype);
-    FWDMI_REQUIRE(workspace && workspace_size >= need && reinterpret_cast<uintptr_t>(workspace) % 4 == 0,
+    const size_t need = fwdmi_layer_norm_backward_workspace(ld, n, bias != nullptr, dtype);
+    FWDMI_REQUIRE(need == 0 || (workspace && workspace_size >= need && reinterpret_cast<uintptr_t>(workspace) % 4 == 0),
                   "layer norm backward: workspace of %zu bytes, %zu needed", workspace ? workspace_size : (size_t)0, need);
     L.dy = dy;
     L.x = x;
@@ -807,9 +907,11 @@ int fwdmi_layer_norm_backward(void* stream, int32_t ld, int64_t n, const void* d
     L.ld = ld;
     float* const ws = static_cast<float*>(workspace);
     const bool long_row = long_rows(ld, dtype);
-    L.c1 = ws + parts * 3 * (int64_t)ld;  // of long rows
-    L.c2 = L.c1 + rows;
-    if (parts == 1) {  // one workgroup's sums are the result
+    if (long_row) {
+      L.c1 = ws + (parts > 1 ? parts * kinds * (int64_t)ld : 0);
+      L.c2 = L.c1 + rows;
+    }
+    if (parts <= 1) {  // one workgroup's sums are the result, or the columns' own
       L.part_gamma = dgamma;
       L.part_beta = dbeta;
       L.part_bias = dbias;
@@ -822,7 +924,7 @@ int fwdmi_layer_norm_backward(void* stream, int32_t ld, int64_t n, const void* d
     const int rc = dtype == FWDMI_F16    ? backward_typed<_Float16>(L, parts, long_row, s)
                    : dtype == FWDMI_BF16 ? backward_typed<__bf16>(L, parts, long_row, s)
                                          : backward_typed<float>(L, parts, long_row, s);
-    if (rc != FWDMI_OK || parts == 1) return rc;
+    if (rc != FWDMI_OK || parts <= 1) return rc;
   }
   ColumnSums S{};
   S.part = static_cast<const float*>(workspace);

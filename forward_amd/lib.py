@@ -104,7 +104,7 @@ SIGNATURES = {
     "fwdmi_emb_layer_norm_ex": (C.c_int, [_vp, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _i32,
                                           _i32, _vp, _vp, _i32, C.c_float, _vp, C.POINTER(EmbExt)]),
     "fwdmi_layer_norm_forward": (C.c_int, [_vp, _i32, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, C.c_float]),
-    "fwdmi_layer_norm_backward_workspace": (_sz, [_i32, _i64, _i32]),
+    "fwdmi_layer_norm_backward_workspace": (_sz, [_i32, _i64, _i32, _i32]),
     "fwdmi_layer_norm_backward": (C.c_int, [_vp, _i32, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
                                             _vp, _sz, _i32]),
     "fwdmi_linear_workspace": (_sz, [_i64, _i64, _i64, _i32]),

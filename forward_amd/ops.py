@@ -489,7 +489,7 @@ def layer_norm_backward(dy, x, gamma, mean, rstd, skip=None, bias=None, dsum=Non
     def call():
         dx, dgamma, dbeta = torch.empty_like(x), torch.empty_like(gamma), torch.empty_like(gamma)
         dbias = None if bias is None else torch.empty_like(gamma)
-        size = lib.dll.fwdmi_layer_norm_backward_workspace(ld, n, dt)
+        size = lib.dll.fwdmi_layer_norm_backward_workspace(ld, n, bias is not None, dt)
         ws = _space(size, x.device)
         lib.check(lib.dll.fwdmi_layer_norm_backward(_raw_stream(at), ld, n, pdy, x.data_ptr(), ps, pd, pg, pi, pm, pr,
                                                     dx.data_ptr(), dgamma.data_ptr(), dbeta.data_ptr(),

@@ -331,11 +331,11 @@ int fwdmi_layer_norm_forward(void* stream, int32_t ld, int64_t n, const void* x,
  *   x / skip / bias as given to the forward call, or x = its `sum` with skip = bias = NULL;
  *   dsum (may be NULL) [rows, ld]: a gradient that reaches the sum from elsewhere;
  *   dgamma, dbeta, dbias fp32 [ld], overwritten (zeros for n == 0); dbias is NULL exactly where bias is.
- * `workspace`: device memory of fwdmi_layer_norm_backward_workspace(ld, n, dtype) bytes, 4-byte aligned, used by
+ * `workspace`: device memory of fwdmi_layer_norm_backward_workspace(ld, n, bias != NULL, dtype) bytes (may be 0), 4-byte aligned, used by
  * this call alone until it has run on `stream` (calls in flight together need one each).
  * Sums are added in a fixed order: results repeat bit for bit.
  */
-size_t fwdmi_layer_norm_backward_workspace(int32_t ld, int64_t n, int32_t dtype);
+size_t fwdmi_layer_norm_backward_workspace(int32_t ld, int64_t n, int32_t with_bias, int32_t dtype);
 int fwdmi_layer_norm_backward(void* stream, int32_t ld, int64_t n, const void* dy, const void* x, const void* skip,
                               const void* dsum, const float* gamma, const float* bias, const float* mean,
                               const float* rstd, void* dx, float* dgamma, float* dbeta, float* dbias, void* workspace,
