@@ -24,13 +24,16 @@ struct Operands {
 //   bf16  8192 x 4096 x 1024                  64 with 256 x 256, 74 with 256 x 128, 84 with 128 x 128
 //         8192 x 1024 x 4096, b across        66 with 256 x 128, 81 with 128 x 128
 //         4096 x 1024 x 8192, both across     63 + 13 to add the splits with 256 x 256 and four, 72 + 9 with 256 x 128 and two
+//         4096 x 1024 x 4096                  42 with 128 x 128 in turns, 45 with four waves, 48 with 256 x 128 on half the CUs
+//         the same, b across or both          52 with 128 x 128 in turns, 63 with four waves, 58 with 64 x 64
 //         384 x 1024 x 4096                   12 with 64 x 32, 15 with 64 x 64, 20 and more with 128 x 128
 //   fp32  512 x 512 x 512                     7 with 32 x 32, 9 with 64 x 32, 13 with 64 x 64
 //         1003 x 517 x 1001                   21 with 32 x 32, 25 with 64 x 64, 28 with 64 x 32
 //         256 x 1024 x 4096                   26 with 64 x 64 and four splits, 27 with 32 x 32 and two, 48 with 32 x 32 alone
-const double kRate[2][kTileKinds] = {{6.0e6, 4.6e6, 4.0e6, 3.5e6, 3.0e6, 2.0e6}, {6.0e6, 4.3e6, 2.2e6, 3.5e6, 3.0e6, 2.0e6}};
-const double kStep32[2][kTileKinds] = {{1e30, 1e30, 2.2, 1.2, 0.8, 0.5}, {1e30, 1e30, 2.1, 1.15, 0.65, 0.36}};
-const double kRound[kTileKinds] = {9.0, 4.0, 3.0, 1.5, 1.0, 1.0};
+const double kRate[2][kTileKinds] = {{6.0e6, 4.6e6, 3.7e6, 4.0e6, 3.5e6, 3.0e6, 2.0e6},
+                                     {6.0e6, 4.3e6, 2.9e6, 2.2e6, 2.8e6, 3.0e6, 2.0e6}};
+const double kStep32[2][kTileKinds] = {{1e30, 1e30, 1e30, 2.2, 1.2, 0.8, 0.5}, {1e30, 1e30, 1e30, 2.1, 1.15, 0.65, 0.36}};
+const double kRound[kTileKinds] = {9.0, 4.0, 3.0, 3.0, 1.5, 1.0, 1.0};
 // One step of each of `wgs` workgroups on a CU.
 double step_us(TileKind kind, const Operands& o, double wgs) {
   const TileShape t = kTiles[kind];
@@ -68,6 +71,8 @@ Plan make_plan(int ni, int nj, int nt, const Operands& o) {
       p.steps_per_split = std::max(1, ceil_div(all, splits));
       p.splits = std::max(1, ceil_div(all, p.steps_per_split));
       const double wgs = ceil_div(tiles * p.splits, cus);
+      if (kind == k128x128Turns && wgs > 1) continue;
+      if (kind == k128x128 && wgs <= 1 && o.elem == 2 && o.direct) continue;  // (in turns instead)
       double us = 2.0 + wgs * kRound[kind] + p.steps_per_split * step_us((TileKind)kind, o, wgs);
       if (p.splits > 1) us += 3.0 + 6.0 * p.splits * ni * nj / 5.0e6;
       if (us < best_us) {

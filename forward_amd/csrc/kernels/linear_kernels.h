@@ -742,12 +742,12 @@ __device__ __forceinline__ void unrolled(std::integer_sequence<int, I...>, F&& f
 // the next step's loads go into the buffer of the step before this one: they start in phase 1, when the late waves
 // have read that buffer's last fragments (those reads are waited for in front of the multiplications they feed), and every
 // wave waits for its own in the last phase, in front of the barrier behind which the first waves read them.  With
-// three buffers (256 x 128, 144 KB) the loads of the step after next go out in phase 1 and have a whole step more.
+// three buffers (256 x 128, 144 KB; 128 x 128, 96 KB) the loads of the step after next go out in phase 1 and have a whole step more.
 template <typename T, int LA, int LB, int TI, int TJ, int WI, int WJ, int STEP, int STAGES>
 __global__ __launch_bounds__(512) void product_turns_kernel(const Product P) {
   constexpr int kNT = 512;
   constexpr int kFI = TI / WI / 16, kFJ = TJ / WJ / 16, kQ = kFI / 4, kPhases = STEP / 64 * kQ;
-  static_assert(WI * WJ == 8 && kFI % 4 == 0 && kFJ == 4 && kPhases >= 2 && (STAGES >= 3 || kPhases == 4),
+  static_assert(WI * WJ == 8 && kFI % 4 == 0 && kPhases >= 2 && (STAGES >= 3 || kPhases == 4),
                 "shape of the phases");
   using TileA = Tile<T, TI, LA, STEP>;
   using TileB = Tile<T, TJ, LB, STEP>;
@@ -831,10 +831,11 @@ __global__ __launch_bounds__(512) void product_turns_kernel(const Product P) {
       multiply_block(std::integral_constant<int, q * 4>{});
     });
   }
-  if (j0 + TJ <= P.nj)
-    leave_registers<T, TI, TJ, WI, WJ, LA == kAlong && LB == kAlong>(P, acc, i0, j0, split);
-  else
-    leave_tile<T, TI, TJ, WI, WJ, 1, STAGES * kBuffer, LA == kAlong && LB == kAlong>(P, acc, s_tile, i0, j0, split);
+  if constexpr (kFJ == 4) {  // (a wave's 64 columns are whole 128-byte lines)
+    if (j0 + TJ <= P.nj)
+      return leave_registers<T, TI, TJ, WI, WJ, LA == kAlong && LB == kAlong>(P, acc, i0, j0, split);
+  }
+  leave_tile<T, TI, TJ, WI, WJ, 1, STAGES * kBuffer, LA == kAlong && LB == kAlong>(P, acc, s_tile, i0, j0, split);
 }
 
 // A few rows (at most 16 MB tokens) through a matrix of weights: one pass over w.  A workgroup takes 16 rows of w and
@@ -1054,6 +1055,8 @@ int launch_product(Product& P, const Plan& plan, hipStream_t stream) {
       hipLaunchKernelGGL((product_turns_kernel<T, LA, LB, 256, 256, 2, 4, 128, 2>), grid, dim3(512), 0, stream, P);
     if (plan.tile == k256x128)
       hipLaunchKernelGGL((product_turns_kernel<T, LA, LB, 256, 128, 4, 2, 128, 3>), grid, dim3(512), 0, stream, P);
+    if (plan.tile == k128x128Turns)
+      hipLaunchKernelGGL((product_turns_kernel<T, LA, LB, 128, 128, 2, 4, 128, 3>), grid, dim3(512), 0, stream, P);
   }
   if (plan.tile == k128x128)
     hipLaunchKernelGGL((product_kernel<Work<T, LA, LB, 128, 128, 2, 2, 1, 128, 2, DIRECT>>), grid, dim3(256), 0, stream, P);

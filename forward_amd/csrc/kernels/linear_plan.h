@@ -40,16 +40,16 @@ struct Slope {
   int32_t act;
 };
 
-// The tiles there are.  The first two are the eight-wave kernel of 16-bit operands (product_turns_kernel), the last is
-// for fp32 operands.
+// The tiles there are.  The first three are the eight-wave kernel of 16-bit operands (product_turns_kernel), the last is
+// for fp32 operands.  k128x128Turns is for launches of at most one workgroup per CU, k128x128 for more (two fit a CU).
 // kFew: product_few_kernel, at most kFewRows rows of x.
-enum TileKind { k256x256, k256x128, k128x128, k64x64, k64x32, k32x32, kTileKinds, kFew = kTileKinds };
+enum TileKind { k256x256, k256x128, k128x128Turns, k128x128, k64x64, k64x32, k32x32, kTileKinds, kFew = kTileKinds };
 constexpr int kFewRows = 32;
 struct TileShape {
   int ti, tj, step_bytes;
 };
-constexpr TileShape kTiles[kTileKinds] = {{256, 256, 128}, {256, 128, 128}, {128, 128, 128}, {64, 64, 256}, {64, 32, 256},
-                                                {32, 32, 256}};
+constexpr TileShape kTiles[kTileKinds] = {{256, 256, 128}, {256, 128, 128}, {128, 128, 128}, {128, 128, 128},
+                                          {64, 64, 256},   {64, 32, 256},   {32, 32, 256}};
 
 struct Plan {
   TileKind tile;
