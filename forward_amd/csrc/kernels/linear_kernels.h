@@ -6,14 +6,14 @@
 //
 // One kernel does the three products: C(i, j) = sum over t of A(i, t) B(j, t) with either operand stored along t
 // (kAlong: x and w of the forward product, dz of dx) or across it (kAcross: w of dx, both operands of dw).  A
-// workgroup owns a TI x TJ tile of C and walks t in steps of 128 bytes; two LDS buffers, the next step's loads in
-// flight while this one is multiplied, one barrier a step.  Sums are fp32 (the accumulators of the matrix cores).
+// workgroup owns a TI x TJ tile of C and walks t in steps of 128 or 256 bytes; two to four LDS buffers, the next
+// steps' loads in flight while this one is multiplied.  Sums are fp32 (the accumulators of the matrix cores).
 //
 // LDS holds a tile in 16-byte chunks, XOR-permuted so that the reads of a fragment spread over all banks:
-//   kAlong   [row][128 bytes of t], chunk c of row r at c ^ (r & 7): a fragment is one ds_read_b128 a lane;
+//   kAlong   [row][bytes of t of a step], chunk c of row r at c ^ (r & 7): a fragment is one ds_read_b128 a lane;
 //   kAcross  [t][rows], the 32-byte (fp32: 64-byte) unit u of line t at u ^ f(t): 16-bit fragments are read
 //            transposed (ds_read_b64_tr_b16), fp32 ones element by element.
-// Operands whose lines are whole 16-byte chunks go from memory straight to LDS (buffer loads, whose range check
+// Operands whose lines are whole 4-byte words go from memory straight to LDS (buffer loads, whose range check
 // supplies the zeros past the end of t); any other size or alignment passes through registers.
 #pragma once
 
@@ -71,7 +71,8 @@ __device__ __forceinline__ float slope(float z) {
     return __builtin_fmaf(z * 0.39894228040143268f, exp_(-0.5f * z * z), normal_cdf<EXACT>(z));
   if (ACT == FWDMI_ACT_GELU_TANH) {
     const float p = logistic(kTanhIn * __builtin_fmaf(0.044715f * z, z * z, z));
-    return __builtin_fmaf(z * p * (1.0f - p) * kTanhIn, __builtin_fmaf(0.134145f * z, z, 1.0f), p);
+    const float zz = fminf(z * z, 1e30f);  // (where it would overflow p (1 - p) is zero; NaN comes back with p)
+    return __builtin_fmaf(z * p * (1.0f - p) * kTanhIn, __builtin_fmaf(0.134145f, zz, 1.0f), p);
   }
   if (ACT == FWDMI_ACT_SILU) {
     const float p = logistic(z);
@@ -157,7 +158,7 @@ struct Tile {
   static constexpr int kUnit = sizeof(T) == 2 ? 2 : 4;                        // chunks of a kAcross unit
   static constexpr int kUnits = kLine / (16 * kUnit);
   // what XOR permutes the chunks of row r by: eight neighbouring rows of one chunk fill 128 bytes
-  __device__ static __forceinline__ int along(int r) { return STEP >= 128 ? r & 7 : (r >> 1) & 3; }
+  __device__ static __forceinline__ int along(int r) { return r & 7; }
   // what XOR permutes the units of line t by; fragments read 16 lines at a time: the bits that differ among them
   __device__ static __forceinline__ int across(int t) {
     const int f = sizeof(T) == 2 ? (t & 3) | ((t >> 1) & 4) : (t >> 2) & 3;
@@ -220,16 +221,6 @@ struct Loader {
     return ((lines - 1) * (uint32_t)ld + last) * (uint32_t)sizeof(T);
   }
   __device__ __forceinline__ void load(char* lds) {
-    load_part<0, kLoads>(lds);
-    advance();
-  }
-  __device__ __forceinline__ void advance() {
-    base += step_elems;
-    t_left -= Tl::kT;
-    --left;
-  }
-  template <int FIRST, int COUNT>
-  __device__ __forceinline__ void load_part(char* lds) {
     // Few scalar instructions: a wave's loads wait for them at the head of every step.
     if (left == partial) {  // also past the end, where there is nothing to read
       bytes = left > 0 ? readable(t_left) : 0;
@@ -241,9 +232,12 @@ struct Loader {
     const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, (int)bytes, 0x00020000);
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
 #pragma unroll
-    for (int i = FIRST; i < FIRST + COUNT; ++i)
+    for (int i = 0; i < kLoads; ++i)
       __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (FWDMI_LDS void*)(lds + (i * NT + wave * 64) * 16), 16,
                                                (int)offset[i], 0, 0, 0);
+    base += step_elems;
+    t_left -= Tl::kT;
+    --left;
   }
 
   // ---- through registers
@@ -593,7 +587,10 @@ __device__ __forceinline__ void leave_registers(const Product& P, const F4 (&acc
   });
 }
 
-// The work of workgroup `block` of `blocks` on product P.  The waves are WI x WJ over the tile and WK over the halves of
+// The work of workgroup `block` of `blocks` on product P.  Products of these sizes are bound by the latency of their few
+// steps (384 x 1024 x 4096 fp16 with residual: 13.6 us of 64 steps' loads, 236 TFLOP/s) or, in fp32, by the matrix
+// instructions and LDS in turn (1003 x 517 x 1001: 22 us, 46 TFLOP/s; 8192 x 1024 x 4096: 126, where a large library product
+// reaches 145).  The waves are WI x WJ over the tile and WK over the halves of
 // a step (their sums meet in LDS): small tiles, whose waves would otherwise have little to do between two barriers.
 template <typename T, int LA, int LB, int TI, int TJ, int WI, int WJ, int WK, int STEP, int STAGES, bool DIRECT>
 struct Work {
@@ -708,7 +705,8 @@ __global__ __launch_bounds__(W::kThreads) void product_kernel(const Product P) {
   W::run(P, s_tile, (int)blockIdx.x, (int)gridDim.x);
 }
 
-// Both products of a small gradient and dbias in one launch: workgroups of dx, of dw, and of 64 columns of dbias each.
+// Both products of a small gradient and dbias in one launch (771 x 1011 x 768 fp16: 11.6 us, bound by the latency of each
+// workgroup's steps; 1.5 us of arithmetic): workgroups of dx, of dw, and of 64 columns of dbias each.
 template <typename T, int TILE, bool DIRECT>
 __global__ __launch_bounds__(TILE * 8) void gradients_kernel(const Gradients G) {
   using X = Work<T, kAlong, kAcross, TILE, TILE, TILE / 32, 1, 4, 256, 2, DIRECT>;
@@ -737,6 +735,10 @@ __device__ __forceinline__ void unrolled(std::integer_sequence<int, I...>, F&& f
 // Large products of 16-bit operands: eight waves, two on every SIMD of the CU, take turns.  While one multiplies (16
 // matrix instructions, 256 cycles of its SIMD), the other reads the fragments of its next 16 from LDS, and both change
 // over at a barrier.  Waves 4 .. 7 run half a phase behind 0 .. 3, by one barrier more in front and one fewer behind.
+//
+// Bound by the matrix cores where the operands are warm (8192 x 4096 x 1024 bf16: 64 us, 1.07 PFLOP/s), by the loads' way
+// from memory and the results' way there where they are cold (75 us); an erf GELU and its stored z add 20 us, for 134 MB
+// of results leave together.  rocprofv3 counts no LDS bank conflict, and matrix instructions in 0.4 of the busy cycles.
 //
 // A step of 64 t has a phase for each half of t and each 64 rows of the wave.  With two buffers (256 x 256 tiles, 128 KB)
 // the next step's loads go into the buffer of the step before this one: they start in phase 1, when the late waves
@@ -838,7 +840,8 @@ __global__ __launch_bounds__(512) void product_turns_kernel(const Product P) {
   leave_tile<T, TI, TJ, WI, WJ, 1, STAGES * kBuffer, LA == kAlong && LB == kAlong>(P, acc, s_tile, i0, j0, split);
 }
 
-// A few rows (at most 16 MB tokens) through a matrix of weights: one pass over w.  A workgroup takes 16 rows of w and
+// A few rows (at most 16 MB tokens) through a matrix of weights: one pass over w, which bounds it.  1 x 4096 x 1024 fp16
+// (8.4 MB): 4.0 us, of which 2 are a launch's own and the rest one trip to memory per wave.  A workgroup takes 16 rows of w and
 // all of x; its waves take 128-byte pieces of t in turn, straight from memory to the matrix instructions (a piece is
 // read by one wave alone, LDS would only add a stop), two pieces in flight, and their sums meet in LDS in wave order.
 // Rows past the last repeat it, their products are dropped.  blockIdx.y: splits of the pieces (few rows of w, long ones).
@@ -920,7 +923,8 @@ __global__ __launch_bounds__(1024) void product_few_kernel(const Product P) {
   }
 }
 
-// Adds the splits' partial products in split order and finishes them; eight neighbours of a row per lane.
+// Adds the splits' partial products in split order and finishes them; bound by memory (four splits of 4096 x 1024: 75 MB in
+// 13 us, 5.8 TB/s, the partials partly from cache); eight neighbours of a row per lane.
 template <typename T>
 __global__ __launch_bounds__(256) void finish_kernel(const Product P, int splits) {
   const int per = (P.nj + 7) / 8;
@@ -964,7 +968,7 @@ __global__ __launch_bounds__(256) void finish_kernel(const Product P, int splits
 
 // ---- dz = dy * act'(z) and its column sums -----------------------------------------------------------------------
 
-// 512 columns (8 per lane) x every (4 gridDim.y)-th row per wave, the four waves' sums through LDS.
+// Bound by memory: 8192 x 4096 bf16, 201 MB, 46 us (4.4 TB/s; a large copy reaches 5.2).  512 columns (8 per lane) x every (4 gridDim.y)-th row per wave, the four waves' sums through LDS.
 template <typename T>
 __global__ __launch_bounds__(256) void slope_kernel(const Slope S) {
   constexpr int kVec = 8;
@@ -1022,6 +1026,7 @@ __global__ __launch_bounds__(256) void slope_kernel(const Slope S) {
 template <typename T>
 int launch_finish(const Product& P, int splits, hipStream_t stream) {
   const int64_t octets = (int64_t)P.ni * ((P.nj + 7) / 8);
+  if (const int rc = check_launch((octets + 255) / 256, 256)) return rc;
   hipLaunchKernelGGL((finish_kernel<T>), dim3((unsigned)ceil_div(octets, 256)), dim3(256), 0, stream, P, splits);
   FWDMI_HIP_CHECK(hipGetLastError());
   return FWDMI_OK;
@@ -1035,6 +1040,7 @@ int launch_product(Product& P, const Plan& plan, hipStream_t stream) {
       const int waves = pieces >= 32 ? 16 : pieces >= 16 ? 8 : 4;
       P.steps_per_split = pieces;
       const dim3 grid((unsigned)ceil_div(P.nj, 16), (unsigned)plan.splits), block(64 * waves);
+      if (const int rc = check_launch((int64_t)grid.x * grid.y, 64 * waves)) return rc;
       if (P.ni <= 16)
         hipLaunchKernelGGL((product_few_kernel<T, 1>), grid, block, waves * 1024, stream, P);
       else
@@ -1049,7 +1055,9 @@ int launch_product(Product& P, const Plan& plan, hipStream_t stream) {
   P.whole_steps = plan.whole_steps;
   P.tail = plan.tail;
   P.steps_per_split = plan.steps_per_split;
-  const dim3 grid((unsigned)(P.tiles_i * P.tiles_j * plan.splits));
+  const int64_t tiles = (int64_t)P.tiles_i * P.tiles_j * plan.splits;
+  if (const int rc = check_launch(tiles, 512)) return rc;
+  const dim3 grid((unsigned)tiles);
   if constexpr (sizeof(T) == 2 && DIRECT) {
     if (plan.tile == k256x256)
       hipLaunchKernelGGL((product_turns_kernel<T, LA, LB, 256, 256, 2, 4, 128, 2>), grid, dim3(512), 0, stream, P);
@@ -1106,6 +1114,7 @@ int run_gradients(const Gradients& G, bool direct, hipStream_t stream) {
 template <typename T>
 int run_slope(const Slope& S, int parts, hipStream_t stream) {
   const dim3 grid((unsigned)ceil_div(S.n, 512), (unsigned)parts);
+  if (const int rc = check_launch((int64_t)grid.x * grid.y, 256)) return rc;
   hipLaunchKernelGGL((slope_kernel<T>), grid, dim3(256), 0, stream, S);
   FWDMI_HIP_CHECK(hipGetLastError());
   return FWDMI_OK;

@@ -318,7 +318,7 @@ int fwdmi_emb_layer_norm_ex(void* stream, int32_t S, int32_t B, int32_t ld, cons
  *   sum (may be NULL) [rows, ld] in `dtype`: h rounded once, for layers whose residual stream goes on unnormalised
  *   (y is computed from the unrounded h);
  *   mean, rstd fp32 [rows];  gamma / beta / bias fp32 [ld], bias may be NULL.
- * Operands need the alignment of their elements only; outputs overlap neither each other nor an input.  ld <= 2^30.
+ * Operands need the alignment of their elements only; outputs overlap neither each other nor an input.  ld <= 2^26.
  * (The reference is an inference engine and has no counterpart of this and the next launcher.)
  */
 int fwdmi_layer_norm_forward(void* stream, int32_t ld, int64_t n, const void* x, const void* skip, const float* beta,
@@ -333,7 +333,7 @@ int fwdmi_layer_norm_forward(void* stream, int32_t ld, int64_t n, const void* x,
  *   dgamma, dbeta, dbias fp32 [ld], overwritten (zeros for n == 0); dbias is NULL exactly where bias is.
  * `workspace`: device memory of fwdmi_layer_norm_backward_workspace(ld, n, bias != NULL, dtype) bytes (may be 0), 4-byte aligned, used by
  * this call alone until it has run on `stream` (calls in flight together need one each).
- * Sums are added in a fixed order: results repeat bit for bit.
+ * Sums are added in a fixed order: results repeat bit for bit.  Outputs overlap neither each other nor an input.
  */
 size_t fwdmi_layer_norm_backward_workspace(int32_t ld, int64_t n, int32_t with_bias, int32_t dtype);
 int fwdmi_layer_norm_backward(void* stream, int32_t ld, int64_t n, const void* dy, const void* x, const void* skip,
@@ -346,8 +346,9 @@ int fwdmi_layer_norm_backward(void* stream, int32_t ld, int64_t n, const void* d
  *   x [m, k], w [n, k], residual [m, n] (may be NULL), y [m, n] in `dtype` (FWDMI_F32 | FWDMI_F16 | FWDMI_BF16),
  *   packed rows; bias fp32 [n] or NULL; preact (may be NULL) [m, n]: z rounded to `dtype`, what the backward pass
  *   reads; act: FWDMI_ACT_*.  Sums, activation and residual are fp32, rounded once.
- * Any sizes up to 2^30 each (2^40 for a product of two) and any element alignment; operands of whole 16-byte lines (k a multiple of 8, fp32 4,
- * and pointers of 16) are the fast ones.  Outputs overlap neither each other nor an input.
+ * Any sizes up to 2^30 each (2^40 for a product of two) whose launches stay below 2^32 work-items (refused otherwise:
+ * a w of some 2^26 rows and more), any element alignment; operands whose lines are whole 4-byte words (16-bit types: an
+ * even k) are the fast ones.  Outputs overlap neither each other nor an input.
  * `workspace`: fwdmi_linear_workspace(m, n, k, dtype) bytes (often 0) on a 16-byte boundary, used by this call alone
  * until it has run on `stream` (calls in flight together need one each).
  * (In the reference a fully connected layer is TensorRT's own, followed by activation and element-wise layers.)
@@ -362,7 +363,7 @@ int fwdmi_linear(void* stream, int64_t m, int64_t n, int64_t k, const void* x, c
  * gradient is dy itself).  dx [m, k], dw [n, k] in `dtype`, dbias fp32 [n]: each may be NULL when not wanted, the
  * others are overwritten.  preact is not read with FWDMI_ACT_NONE.  dz is rounded to `dtype` before the products (as
  * the operand of a matrix instruction has to be); dbias sums it unrounded.  relu's slope at 0 is 0.
- * Sums run in a fixed order: results repeat bit for bit.  `workspace` as above.
+ * Sums run in a fixed order: results repeat bit for bit.  Sizes, overlap and `workspace` as above.
  */
 size_t fwdmi_linear_backward_workspace(int64_t m, int64_t n, int64_t k, int32_t act, int32_t dtype);
 int fwdmi_linear_backward(void* stream, int64_t m, int64_t n, int64_t k, const void* dy, const void* x, const void* w,

@@ -150,6 +150,20 @@ def test_activations(act, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("act", ACTS)
+def test_far_pre_activations(act, dtype):
+    """Where every activation is z or 0 and its slope 1 or 0, up to the ends of the type."""
+    big = torch.finfo(dtype).max
+    z = torch.tensor([[100.0, min(1e20, big), big, -100.0, -min(1e20, big), -big]], device="cuda").to(dtype)
+    one, eye = torch.ones(1, 6, dtype=dtype, device="cuda"), torch.eye(6, dtype=dtype, device="cuda")
+    want = torch.where((z > 0) | torch.tensor(act == "none", device="cuda"), z, torch.zeros_like(z))
+    assert torch.equal(ops.linear(z, eye, activation=act), want)         # (products with zeros are exact)
+    dx, _, db = ops.linear_backward(one, z, eye, preact=z if act != "none" else None, activation=act)
+    slope = (want != 0).to(dtype)
+    assert torch.equal(dx, slope) and torch.equal(db, slope.float()[0])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("offset", [1, 2, 3, 7])
 def test_operands_start_at_any_element(offset, dtype):
     s = make(70, 136, 200, dtype, offset, offset=offset)

@@ -124,6 +124,22 @@ def test_linear_workspace_sizes():
 
 
 @pytest.mark.skipif(lib.dll.fwdmi_device_count() > 0, reason="made-up addresses: only where nothing can be launched")
+def test_launches_that_a_device_cannot_hold_are_refused():
+    d, p, big = lib.dll, 1 << 20, (1 << 64) - 1
+    call = lambda m, n, k, ptr=p: d.fwdmi_linear(None, m, n, k, p, p, None, None, ptr, None, 0, lib.F16, p, big)
+    assert call(1, 1 << 26, 8) == lib.ERR_HIP            # (no device here: it got as far as the launch)
+    assert call(1, 1 << 30, 8) == lib.ERR_UNSUPPORTED    # 2^26 workgroups of 256
+    assert call(33, 1 << 30, 8) == lib.ERR_UNSUPPORTED
+    back = lambda m, n, k: d.fwdmi_linear_backward(None, m, n, k, p, p, p, None, p, None, None, 0, lib.F16, p, big)
+    assert back(1 << 20, 8, 1 << 10) == lib.ERR_HIP      # (dx alone)
+    assert back(1 << 30, 8, 1 << 10) == lib.ERR_UNSUPPORTED
+    width = (1 << 26) + 1
+    assert d.fwdmi_layer_norm_forward(None, width, width, *[p] * 9, lib.F16, 1e-5) == lib.ERR_BAD_ARG
+    assert d.fwdmi_layer_norm_backward(None, width, width, *[p] * 12, p, big, lib.F16) == lib.ERR_BAD_ARG
+    assert d.fwdmi_layer_norm_forward(None, width - 1, width - 1, *[p] * 9, lib.F16, 1e-5) == lib.ERR_HIP
+
+
+@pytest.mark.skipif(lib.dll.fwdmi_device_count() > 0, reason="made-up addresses: only where nothing can be launched")
 def test_arguments_at_the_ends_of_their_types_return_a_status():
     """Every call below returns: refused, nothing to do, or (no device here) a launch that the runtime turns down; and the
     workspace sizes neither wrap round nor fall short of what a call then asks for."""
