@@ -555,7 +555,8 @@ __global__ __launch_bounds__(kStreamWG) void ln_forward_stream_kernel(const LnTr
   }
 }
 
-// Two passes, likewise; with the columns that follow, 2700 x 12288 fp32 takes 146 us.
+// Two passes, likewise, and the columns' kernel reads dy and x a third time: 2700 x 12288 fp32 takes 146 us in all, 129 of
+// them what its 660 MB from and to memory take at a large copy's rate.
 template <typename T>
 __global__ __launch_bounds__(kStreamWG) void ln_backward_stream_kernel(const LnTrain L) {
   constexpr int VEC = 16 / sizeof(T);
