@@ -6,7 +6,7 @@
 //
 // One kernel does the three products: C(i, j) = sum over t of A(i, t) B(j, t) with either operand stored along t
 // (kAlong: x and w of the forward product, dz of dx) or across it (kAcross: w of dx, both operands of dw).  A
-// workgroup owns a TI x TJ tile of C and walks t in steps of 128 or 256 bytes; two to four LDS buffers, the next
+// workgroup owns a TI x TJ tile of C and walks t in steps of 128 to 512 bytes; two to four LDS buffers, the next
 // steps' loads in flight while this one is multiplied.  Sums are fp32 (the accumulators of the matrix cores).
 //
 // LDS holds a tile in 16-byte chunks, XOR-permuted so that the reads of a fragment spread over all banks:
@@ -588,7 +588,7 @@ __device__ __forceinline__ void leave_registers(const Product& P, const F4 (&acc
 }
 
 // The work of workgroup `block` of `blocks` on product P.  Products of these sizes are bound by the latency of their few
-// steps (384 x 1024 x 4096 fp16 with residual: 13.6 us of 64 steps' loads, 236 TFLOP/s) or, in fp32, by the matrix
+// steps and by what a CU loads, 90 KB/us (384 x 1024 x 4096 fp16: 9.6 us, 335 TFLOP/s, of which 7.1 are its 640 KB), or, in fp32, by the matrix
 // instructions and LDS in turn (1003 x 517 x 1001: 22 us, 46 TFLOP/s; 8192 x 1024 x 4096: 126, where a large library product
 // reaches 145).  The waves are WI x WJ over the tile and WK over the halves of
 // a step (their sums meet in LDS): small tiles, whose waves would otherwise have little to do between two barriers.
@@ -1070,9 +1070,19 @@ int launch_product(Product& P, const Plan& plan, hipStream_t stream) {
     hipLaunchKernelGGL((product_kernel<Work<T, LA, LB, 128, 128, 2, 2, 1, 128, 2, DIRECT>>), grid, dim3(256), 0, stream, P);
   if (plan.tile == k64x64)
     hipLaunchKernelGGL((product_kernel<Work<T, LA, LB, 64, 64, 2, 1, 4, 256, 2, DIRECT>>), grid, dim3(512), 0, stream, P);
-  if (plan.tile == k64x32)
-    hipLaunchKernelGGL((product_kernel<Work<T, LA, LB, 64, 32, 2, 1, 4, 256, DIRECT ? 4 : 2, DIRECT>>), grid, dim3(512), 0,
-                       stream, P);
+  if constexpr (sizeof(T) == 2 && DIRECT) {
+    if (plan.tile == k64x32)
+      hipLaunchKernelGGL((product_kernel<Work<T, LA, LB, 64, 32, 2, 1, 4, 512, 3, true>>), grid, dim3(512), 0, stream, P);
+    if constexpr (LA == kAlong && LB == kAlong)
+      if (plan.tile == k48x32)
+        hipLaunchKernelGGL((product_kernel<Work<T, LA, LB, 48, 32, 1, 1, 8, 512, 3, true>>), grid, dim3(512), 0, stream, P);
+    if (plan.tile == k32x32)
+      hipLaunchKernelGGL((product_kernel<Work<T, LA, LB, 32, 32, 1, 1, 8, 512, 3, true>>), grid, dim3(512), 0, stream, P);
+  } else {
+    if (plan.tile == k64x32)
+      hipLaunchKernelGGL((product_kernel<Work<T, LA, LB, 64, 32, 2, 1, 4, 256, DIRECT ? 4 : 2, DIRECT>>), grid, dim3(512), 0,
+                         stream, P);
+  }
   if constexpr (sizeof(T) == 4) {
     if (plan.tile == k32x32)
       hipLaunchKernelGGL((product_kernel<Work<T, LA, LB, 32, 32, 1, 1, 4, 256, 2, DIRECT>>), grid, dim3(256), 0, stream, P);

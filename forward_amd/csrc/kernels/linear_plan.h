@@ -40,16 +40,22 @@ struct Slope {
   int32_t act;
 };
 
-// The tiles there are.  The first three are the eight-wave kernel of 16-bit operands (product_turns_kernel), the last is
-// for fp32 operands.  k128x128Turns is for launches of at most one workgroup per CU, k128x128 for more (two fit a CU).
+// The tiles there are.  The first three are the eight-wave kernel of 16-bit operands (product_turns_kernel).
+// k128x128Turns is for launches of at most one workgroup per CU, k128x128 for more (two fit a CU); k48x32 is for 16-bit
+// operands along t, k32x32 for fp32 and for 16-bit operands that are loaded directly.
 // kFew: product_few_kernel, at most kFewRows rows of x.
-enum TileKind { k256x256, k256x128, k128x128Turns, k128x128, k64x64, k64x32, k32x32, kTileKinds, kFew = kTileKinds };
+enum TileKind { k256x256, k256x128, k128x128Turns, k128x128, k64x64, k64x32, k48x32, k32x32, kTileKinds, kFew = kTileKinds };
 constexpr int kFewRows = 32;
 struct TileShape {
-  int ti, tj, step_bytes;
+  int ti, tj;
 };
-constexpr TileShape kTiles[kTileKinds] = {{256, 256, 128}, {256, 128, 128}, {128, 128, 128}, {128, 128, 128},
-                                          {64, 64, 256},   {64, 32, 256},   {32, 32, 256}};
+constexpr TileShape kTiles[kTileKinds] = {{256, 256}, {256, 128}, {128, 128}, {128, 128}, {64, 64}, {64, 32}, {48, 32}, {32, 32}};
+
+// Bytes of t in a step.  The smallest tiles have the least to do between two barriers: 16-bit operands straight from memory,
+// which need no registers on the way, take 512 (512 x 1024 x 4096: 10.5 us, with 256 11.8).
+inline int step_bytes(TileKind kind, int elem, bool direct) {
+  return kind <= k128x128 ? 128 : kind >= k64x32 && elem == 2 && direct ? 512 : 256;
+}
 
 struct Plan {
   TileKind tile;
