@@ -18,31 +18,33 @@ struct Operands {
 
 // The tile and the number of splits of t with the shortest estimated time.  A CU's time is its workgroups' steps: each as
 // long as its loads (direct ones reach 90 KB/us per CU, those through registers 40) or its matrix instructions take
-// (kRate: flop/us per CU that the steps of each tile sustain in bf16, for operands along t or only b across, and both
-// across; in fp32 kStep32, per workgroup when a CU has one and when it has several), plus what a round of tiles spends
+// (kRate: flop/us per CU that the steps of each tile sustain in bf16, by layout; in fp32 kStep32, per workgroup when a CU has one and when it has several), plus what a round of tiles spends
 // outside its steps and, with splits, the second launch and the partial products' way through the caches.  Measured, us:
 //   bf16  8192 x 4096 x 1024                  64 with 256 x 256, 74 with 256 x 128, 84 with 128 x 128
 //         8192 x 1024 x 4096, b across        66 with 256 x 128, 81 with 128 x 128
 //         4096 x 1024 x 8192, both across     63 + 13 to add the splits with 256 x 256 and four, 72 + 9 with 256 x 128 and two
 //         4096 x 1024 x 4096                  42 with 128 x 128 in turns, 45 with four waves, 48 with 256 x 128 on half the CUs
 //         the same, b across or both          52 with 128 x 128 in turns, 63 with four waves, 58 with 64 x 64
+//         1024 x 1024 x 4096                  15 with 64 x 64 and three buffers, 23 with two
+//         the same, b across or both          22 and 24 with 64 x 64 and steps of 512 bytes, 27 with 256 and two or three buffers
 //         512 x 1024 x 4096                   10 with 64 x 32, 13 with 32 x 32, 18 with 48 x 32 (two workgroups on some CUs)
 //         384 x 1024 x 4096                   10 with 48 x 32, 11 with 64 x 32, 14 with 32 x 32, 15 with 64 x 64
 //         256 x 1024 x 4096                   8 with 32 x 32, 9 with 48 x 32, 10 with 64 x 32
 //   fp32  512 x 512 x 512                     7 with 32 x 32, 9 with 64 x 32, 13 with 64 x 64
 //         1003 x 517 x 1001                   21 with 32 x 32, 25 with 64 x 64, 28 with 64 x 32
 //         256 x 1024 x 4096                   26 with 64 x 64 and four splits, 27 with 32 x 32 and two, 48 with 32 x 32 alone
-const double kRate[2][kTileKinds] = {{6.0e6, 4.6e6, 3.7e6, 4.0e6, 3.5e6, 3.0e6, 3.0e6, 2.0e6},
-                                     {6.0e6, 4.3e6, 2.9e6, 2.2e6, 2.8e6, 3.0e6, 3.0e6, 2.0e6}};
-const double kStep32[2][kTileKinds] = {{1e30, 1e30, 1e30, 2.2, 1.2, 0.8, 1e30, 0.5}, {1e30, 1e30, 1e30, 2.1, 1.15, 0.65, 1e30, 0.36}};
-const double kRound[kTileKinds] = {9.0, 4.0, 3.0, 3.0, 1.5, 1.0, 1.0, 1.0};
+const double kRate[3][kTileKinds] = {{6.0e6, 4.6e6, 3.7e6, 3.5e6, 4.0e6, 3.5e6, 3.0e6, 3.0e6, 2.0e6},
+                                     {6.0e6, 4.6e6, 2.9e6, 1.9e6, 3.7e6, 3.0e6, 1.4e6, 0.0, 0.9e6},
+                                     {6.0e6, 4.3e6, 2.9e6, 1.8e6, 2.2e6, 2.8e6, 1.4e6, 0.0, 0.8e6}};
+const double kStep32[2][kTileKinds] = {{0, 0, 0, 0, 2.2, 1.2, 0.8, 0, 0.5}, {0, 0, 0, 0, 2.1, 1.15, 0.65, 0, 0.36}};
+const double kRound[kTileKinds] = {9.0, 4.0, 3.0, 1.5, 3.0, 1.5, 1.0, 1.0, 1.0};
 // One step of each of `wgs` workgroups on a CU.
 double step_us(TileKind kind, const Operands& o, double wgs) {
   const TileShape t = kTiles[kind];
-  const int bytes = step_bytes(kind, o.elem, o.direct);
+  const int bytes = step_bytes(kind, o.layouts, o.elem, o.direct);
   const double load = wgs * (t.ti + t.tj) * bytes / ((o.direct ? 90.0 : 40.0) * 1024);
   if (o.elem == 4) return std::max(load, std::max(kStep32[0][kind], wgs * kStep32[1][kind]));
-  return std::max(load, wgs * 2.0 * t.ti * t.tj * (bytes / 2) / kRate[o.layouts == 2][kind]);
+  return std::max(load, wgs * 2.0 * t.ti * t.tj * (bytes / 2) / kRate[o.layouts][kind]);
 }
 // A few rows: whole rows of w per workgroup, unless there are so few workgroups and so long rows that a second launch to
 // add splits costs less than it gains.  A CU draws w and x at 38 KB/us through registers: 16 x 4096 x 1024 fp32 takes 16 us
@@ -65,7 +67,7 @@ Plan make_plan(int ni, int nj, int nt, const Operands& o) {
     if (kind == k48x32 && (o.elem == 4 || o.layouts != 0)) continue;
     const TileShape t = kTiles[kind];
     Plan p{(TileKind)kind, 1, 0, 0, 0, 0.0};
-    tail_of(nt, step_bytes(p.tile, o.elem, o.direct) / o.elem, o.end, p.whole_steps, p.tail);
+    tail_of(nt, step_bytes(p.tile, o.layouts, o.elem, o.direct) / o.elem, o.end, p.whole_steps, p.tail);
     const int all = p.whole_steps + (p.tail > 0);
     const int64_t tiles = (int64_t)ceil_div(ni, t.ti) * ceil_div(nj, t.tj);
     for (int target = 0; target <= 2; ++target) {  // one workgroup per tile, or splits for one or two per CU
@@ -75,8 +77,8 @@ Plan make_plan(int ni, int nj, int nt, const Operands& o) {
       p.steps_per_split = std::max(1, ceil_div(all, splits));
       p.splits = std::max(1, ceil_div(all, p.steps_per_split));
       const double wgs = ceil_div(tiles * p.splits, cus);
-      if (kind == k128x128Turns && wgs > 1) continue;
-      if (kind == k128x128 && wgs <= 1 && o.elem == 2 && o.direct) continue;  // (in turns instead)
+      if ((kind == k128x128Turns || kind == k64x64Alone) && wgs > 1) continue;
+      if ((kind == k128x128 || kind == k64x64) && wgs <= 1 && o.elem == 2 && o.direct) continue;  // (those instead)
       double us = 2.0 + wgs * kRound[kind] + p.steps_per_split * step_us((TileKind)kind, o, wgs);
       if (p.splits > 1) us += 3.0 + 6.0 * p.splits * ni * nj / 5.0e6;
       if (us < best_us) {
@@ -120,7 +122,7 @@ int run(Product& P, int layouts, int dtype, void* workspace, hipStream_t stream)
 // Fills in P as one unsplit pass over tiles of `kind`; returns the number of tiles.
 int64_t whole_tiles(Product& P, TileKind kind, const Operands& o) {
   const TileShape t = kTiles[kind];
-  tail_of(P.nt, step_bytes(kind, o.elem, o.direct) / o.elem, o.end, P.whole_steps, P.tail);
+  tail_of(P.nt, step_bytes(kind, o.layouts, o.elem, o.direct) / o.elem, o.end, P.whole_steps, P.tail);
   P.steps_per_split = P.whole_steps + (P.tail > 0);
   P.tiles_i = ceil_div(P.ni, t.ti);
   P.tiles_j = ceil_div(P.nj, t.tj);

@@ -157,12 +157,13 @@ struct Tile {
   static constexpr int kLine = LAYOUT == kAlong ? STEP : ROWS * (int)sizeof(T);  // bytes of an LDS line
   static constexpr int kUnit = sizeof(T) == 2 ? 2 : 4;                        // chunks of a kAcross unit
   static constexpr int kUnits = kLine / (16 * kUnit);
-  // what XOR permutes the chunks of row r by: eight neighbouring rows of one chunk fill 128 bytes
-  __device__ static __forceinline__ int along(int r) { return r & 7; }
-  // what XOR permutes the units of line t by; fragments read 16 lines at a time: the bits that differ among them
+  // what XOR permutes the chunks of row r by: 16 rows, eight of one chunk and eight of its neighbour, fill 256 bytes
+  __device__ static __forceinline__ int along(int r) { return r & (STEP >= 256 ? 15 : 7); }
+  // what XOR permutes the units of line t by.  16-bit fragments read lines 0 .. 3 and 8 .. 11 at a time, which fill 256
+  // bytes: lines of 256 bytes and more differ by three bits, two lines of 128 to 256 bytes by two, four by one.
   __device__ static __forceinline__ int across(int t) {
-    const int f = sizeof(T) == 2 ? (t & 3) | ((t >> 1) & 4) : (t >> 2) & 3;
-    return f & (kUnits - 1);
+    if (sizeof(T) == 4) return ((t >> 2) & 3) & (kUnits - 1);
+    return kUnits >= 8 ? (t & 3) | ((t >> 1) & 4) : kUnits == 4 ? ((t >> 1) & 1) | ((t >> 2) & 2) : (t >> 3) & (kUnits - 1);
   }
   // the line and the chunk of the line whose contents lie at chunk p
   __device__ static __forceinline__ void locate(int p, int& line, int& chunk) {
@@ -302,13 +303,14 @@ template <typename T, int ROWS, int LAYOUT, int STEP, int FR>
 struct Reader {
   using Tl = Tile<T, ROWS, LAYOUT, STEP>;
   int at[LAYOUT == kAlong ? 1 : FR];
-  int half;
+  int half, quarter;
   __device__ __forceinline__ explicit Reader(int row0) {
     const int lane = threadIdx.x & 63, g = lane >> 4, j = lane & 15;
-    half = 0;
+    half = quarter = 0;
     if constexpr (LAYOUT == kAlong) {
       at[0] = (row0 + j) * STEP + ((g ^ Tl::along(j)) << 4);  // (row0 is a multiple of 16)
-      half = (g ^ Tl::along(j)) & 4;  // a half of 64 bytes more flips bit 2 of the chunk and carries into bit 3
+      half = (g ^ Tl::along(j)) & 4;     // 64 bytes more flip bit 2 of the chunk,
+      quarter = (g ^ Tl::along(j)) & 8;  // 128 bytes more bit 3
     } else if constexpr (sizeof(T) == 2) {
       const int t = g * 8 + (j >> 2);
 #pragma unroll
@@ -324,8 +326,9 @@ struct Reader {
 #pragma unroll
     for (int f = 0; f < COUNT; ++f) {
       if constexpr (LAYOUT == kAlong) {
-        out[f].v = *reinterpret_cast<const Pack<T, kChunk<T>>*>(lds + at[0] + (h & 1 ? 64 - 32 * half : 0) + (h >> 1) * 128 +
-                                                                    (FIRST + f) * 16 * STEP);
+        out[f].v = *reinterpret_cast<const Pack<T, kChunk<T>>*>(lds + at[0] + (h & 1 ? 64 - 32 * half : 0) +
+                                                                  (h & 2 ? 128 - 32 * quarter : 0) + (h >> 2) * 256 +
+                                                                  (FIRST + f) * 16 * STEP);
       } else if constexpr (sizeof(T) == 2) {
         const char* const p = lds + at[FIRST + f] + h * 32 * Tl::kLine;
         const S4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((FWDMI_LDS S4*)(p));
@@ -1065,6 +1068,12 @@ int launch_product(Product& P, const Plan& plan, hipStream_t stream) {
       hipLaunchKernelGGL((product_turns_kernel<T, LA, LB, 256, 128, 4, 2, 128, 3>), grid, dim3(512), 0, stream, P);
     if (plan.tile == k128x128Turns)
       hipLaunchKernelGGL((product_turns_kernel<T, LA, LB, 128, 128, 2, 4, 128, 3>), grid, dim3(512), 0, stream, P);
+    if (plan.tile == k64x64Alone) {
+      if constexpr (LA == kAlong && LB == kAlong)
+        hipLaunchKernelGGL((product_kernel<Work<T, LA, LB, 64, 64, 2, 1, 4, 256, 3, true>>), grid, dim3(512), 0, stream, P);
+      else
+        hipLaunchKernelGGL((product_kernel<Work<T, LA, LB, 64, 64, 1, 1, 8, 512, 2, true>>), grid, dim3(512), 0, stream, P);
+    }
   }
   if (plan.tile == k128x128)
     hipLaunchKernelGGL((product_kernel<Work<T, LA, LB, 128, 128, 2, 2, 1, 128, 2, DIRECT>>), grid, dim3(256), 0, stream, P);
