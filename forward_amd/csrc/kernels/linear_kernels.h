@@ -242,8 +242,8 @@ struct Loader {
   }
 
   // ---- through registers
-  // Chunk i of a step that has `t_left` elements of t, zeros where nothing exists.
-  __device__ __forceinline__ Pack<T, kChunk<T>> some(int i, int t_left) const {
+  // Chunk i of the step at `base` that has `t_left` elements of t, zeros where nothing exists.
+  __device__ __forceinline__ Pack<T, kChunk<T>> some(const T FWDMI_GLOBAL* base, int i, int t_left) const {
     const int r = LAYOUT == kAlong ? line[i] : chunk[i] * kChunk<T>;
     const int t = LAYOUT == kAlong ? chunk[i] * kChunk<T> : line[i];
     const int n = r < rows && t < t_left ? (LAYOUT == kAlong ? t_left - t : rows - r) : 0;
@@ -275,7 +275,7 @@ struct Loader {
       }
     } else if (t_left > 0) {
 #pragma unroll
-      for (int i = 0; i < kLoads; ++i) held[SET][i] = some(i, t_left);
+      for (int i = 0; i < kLoads; ++i) held[SET][i] = some(base, i, t_left);
     }
     base += step_elems;
     t_left -= Tl::kT;
@@ -285,10 +285,14 @@ struct Loader {
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) put(lds, i, held[SET][i]);
   }
-  // The last, partial step of DIRECT loads.
-  __device__ __forceinline__ void tail(char* lds, int t_left) const {
+  // The last, partial step of DIRECT loads, `steps` past `base`.
+  __device__ __forceinline__ void tail(char* lds, int steps, int t_left) const {
+    const T FWDMI_GLOBAL* const at = base + steps * step_elems;
+    Pack<T, kChunk<T>> v[kLoads];
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) put(lds, i, some(i, t_left));
+    for (int i = 0; i < kLoads; ++i) v[i] = some(at, i, t_left);
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) put(lds, i, v[i]);
   }
 };
 
@@ -649,6 +653,14 @@ __device__ __forceinline__ void Work<T, LA, LB, TI, TJ, WI, WJ, WK, STEP, STAGES
       lb.load(s_tile + k * kBuffer + TileA::kBytes);
     }
     int now = 0, next = (STAGES - 1) * kBuffer;
+    if (steps.tail > 0) {
+      // The end of t comes first, through the buffer that nothing is on its way to: its loads, which have to be waited for,
+      // take the time that the first steps' take anyway.
+      la.tail(s_tile + next, steps.whole - (STAGES - 1), steps.tail);
+      lb.tail(s_tile + next + TileA::kBytes, steps.whole - (STAGES - 1), steps.tail);
+      __syncthreads();
+      multiply_step(s_tile + next);
+    }
     for (int s = 0; s < steps.whole; ++s) {
       __builtin_amdgcn_sched_barrier(0);
       __builtin_amdgcn_s_waitcnt(wait_loads(kAhead));  // this step's are in
@@ -661,16 +673,6 @@ __device__ __forceinline__ void Work<T, LA, LB, TI, TJ, WI, WJ, WK, STEP, STAGES
       next = next + kBuffer == STAGES * kBuffer ? 0 : next + kBuffer;
     }
     __builtin_amdgcn_s_waitcnt(wait_loads(0));  // loads past the end write zeros: before the buffers are used again
-    if (steps.tail > 0) {
-      // (`base` has run ahead of the tail by the steps in flight)
-      __syncthreads();
-      la.base -= (STAGES - 1) * la.step_elems;
-      lb.base -= (STAGES - 1) * lb.step_elems;
-      la.tail(s_tile, steps.tail);
-      lb.tail(s_tile + TileA::kBytes, steps.tail);
-      __syncthreads();
-      multiply_step(s_tile);
-    }
   } else if (const int n = steps.whole + (steps.tail > 0 ? 1 : 0); n > 0) {
     const int t = steps.whole * TileA::kT + steps.tail;
     LoadA la(P.a, P.lda, i0, P.ni, steps.first, n, t);
@@ -783,10 +785,6 @@ __global__ __launch_bounds__(512) void product_turns_kernel(const Product P) {
     la.load(s_tile + k * kBuffer);
     lb.load(s_tile + k * kBuffer + TileA::kBytes);
   }
-  __builtin_amdgcn_s_waitcnt(wait_loads(kAhead));
-  __builtin_amdgcn_s_barrier();
-  if (wave >= 4) __builtin_amdgcn_s_barrier();
-  __builtin_amdgcn_sched_barrier(0);
   Frag<T> fa[4], fb[kFJ];
   auto change = [&] {
     __builtin_amdgcn_sched_barrier(0);
@@ -801,6 +799,23 @@ __global__ __launch_bounds__(512) void product_turns_kernel(const Product P) {
       for (int i = 0; i < 4; ++i) acc[j][kFirst + i] = multiply<T>(fb[j], fa[i], acc[j][kFirst + i]);
   };
   int now_at = 0, next_at = (STAGES - 1) * kBuffer;
+  if (steps.tail > 0) {  // the end of t comes first, as in Work
+    char* const end = s_tile + next_at;
+    la.tail(end, steps.whole - (STAGES - 1), steps.tail);
+    lb.tail(end + TileA::kBytes, steps.whole - (STAGES - 1), steps.tail);
+    __syncthreads();
+    unrolled(std::make_integer_sequence<int, kPhases>{}, [&](auto phase) {
+      constexpr int ph = decltype(phase)::value, h = ph / kQ, q = ph % kQ;
+      if constexpr (q == 0) rb.read(end + TileA::kBytes, h, fb);
+      ra.template read<q * 4, 4>(end, h, fa);
+      multiply_block(std::integral_constant<int, q * 4>{});
+    });
+  }
+  __builtin_amdgcn_sched_barrier(0);
+  __builtin_amdgcn_s_waitcnt(wait_loads(kAhead));
+  __builtin_amdgcn_s_barrier();
+  if (wave >= 4) __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_sched_barrier(0);
   for (int s = 0; s < steps.whole; ++s) {
     const char* const now = s_tile + now_at;
     char* const next = s_tile + next_at;
@@ -822,20 +837,6 @@ __global__ __launch_bounds__(512) void product_turns_kernel(const Product P) {
   }
   if (wave < 4) __builtin_amdgcn_s_barrier();
   __builtin_amdgcn_s_waitcnt(wait_loads(0));  // loads past the end write zeros: before the buffers are used again
-  if (steps.tail > 0) {
-    __syncthreads();
-    la.base -= (STAGES - 1) * la.step_elems;
-    lb.base -= (STAGES - 1) * lb.step_elems;
-    la.tail(s_tile, steps.tail);
-    lb.tail(s_tile + TileA::kBytes, steps.tail);
-    __syncthreads();
-    unrolled(std::make_integer_sequence<int, kPhases>{}, [&](auto phase) {
-      constexpr int ph = decltype(phase)::value, h = ph / kQ, q = ph % kQ;
-      if constexpr (q == 0) rb.read(s_tile + TileA::kBytes, h, fb);
-      ra.template read<q * 4, 4>(s_tile, h, fa);
-      multiply_block(std::integral_constant<int, q * 4>{});
-    });
-  }
   if constexpr (kFJ == 4) {  // (a wave's 64 columns are whole 128-byte lines)
     if (j0 + TJ <= P.nj)
       return leave_registers<T, TI, TJ, WI, WJ, LA == kAlong && LB == kAlong>(P, acc, i0, j0, split);
