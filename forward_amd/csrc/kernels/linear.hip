@@ -347,9 +347,12 @@ int fwdmi_linear_backward(void* stream, int64_t m, int64_t n, int64_t k, const v
   bool direct = false;
   const bool joint = any && dx && dw && together(X, W, dtype, G, direct);
   // few rows are summed straight from dy by the joint launch
-  const bool sum_dy = joint && act == FWDMI_ACT_NONE && !copy && m <= 1024;
+  const bool sum_dy = joint && act == FWDMI_ACT_NONE && m <= 1024;
   int rc = FWDMI_OK;
-  if (any && (copy || (dbias && !sum_dy))) {
+  if (copy && act == FWDMI_ACT_NONE && (sum_dy || !dbias)) {  // (a plain copy, 4 us for 771 x 1011; 5 with partial sums)
+    rc = run_widen(Widen{{dy, nullptr}, {ws, nullptr}, {m, 0}, (int)n, (int)space.ld_dz}, s);
+    if (rc != FWDMI_OK) return rc;
+  } else if (any && (copy || (dbias && !sum_dy))) {
     Slope S{};
     S.dy = dy;
     S.z = act != FWDMI_ACT_NONE ? preact : nullptr;

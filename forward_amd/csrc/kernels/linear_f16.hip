@@ -7,8 +7,9 @@ namespace {
 // Bound by memory, a read and a write: 4099 x 1531 and 4096 x 1531 (50 MB in all) take 11 us, and the product behind them then loads
 // directly.  Eight elements per lane; an element past the line's end becomes a zero.
 __global__ __launch_bounds__(256) void widen_kernel(const Widen W) {
-  const int which = blockIdx.y, per = W.ld_out / 8;
-  const int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x, line = q / per;
+  const uint32_t which = blockIdx.y, per = W.ld_out / 8;
+  const uint32_t q = blockIdx.x * 256 + threadIdx.x;  // (a launch holds fewer than 2^32 lanes)
+  const int64_t line = q / per;
   if (line >= W.lines[which]) return;
   const int c = (int)(q % per) * 8;
   const uint16_t FWDMI_GLOBAL* const p = gconst<uint16_t>(W.in[which]) + line * W.ld + c;

@@ -931,8 +931,8 @@ __global__ __launch_bounds__(1024) void product_few_kernel(const Product P) {
 // 13 us, 5.8 TB/s, the partials partly from cache); eight neighbours of a row per lane.
 template <typename T>
 __global__ __launch_bounds__(256) void finish_kernel(const Product P, int splits) {
-  const int per = (P.nj + 7) / 8;
-  const int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const uint32_t per = (P.nj + 7) / 8;
+  const uint32_t q = blockIdx.x * 256 + threadIdx.x;  // (a launch holds fewer than 2^32 lanes)
   const int64_t i = q / per;
   if (i >= P.ni) return;
   const int j = (int)(q % per) * 8;
