@@ -136,6 +136,33 @@ def test_shapes(shape, dtype):
     check_backward(s, ACTS[(m + k) % 5], bias=k % 2 == 0)
 
 
+# (rows, columns, sum): each tile with one workgroup per CU and several, with the sum whole and split, and ends of a step; a
+# line of more than 4 MiB; a sum of fewer elements than a load
+PRODUCTS = [(36, 38, 36), (36, 38, 1962), (194, 1154, 36), (98, 332, 2934), (114, 334, 3916), (132, 2732, 38), (226, 424, 4272),
+            (514, 1808, 46), (1154, 860, 2624), (200, 4222, 66), (2658, 3056, 38), (4828, 772, 38), (1306, 966, 4102), (2882, 2840, 138),
+            (2380, 3382, 76), (800, 2840, 4842), (4892, 848, 3442), (36, 2097154, 36), (36, 38, 5), (194, 1154, 5), (132, 2732, 5), (660, 2990, 5)]
+
+
+@pytest.mark.parametrize("offset", [0, 1])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", PRODUCTS)
+def test_each_product_alone(shape, dtype, offset):
+    """y, dx and dw of these sizes, each in a call of its own; with the offset 16-bit operands go through registers."""
+    ni, nj, nt = shape
+    e, tiny, seed = half(dtype), torch.finfo(dtype).tiny, ni + nj + nt
+    check_linear(make(ni, nj, nt, dtype, seed, offset), "silu", bias=True, residual=True, preact=True)
+    s = make(ni, nt, nj, dtype, seed + 1, offset)
+    dx, = ops.linear_backward(s["dy"], s["x"], s["w"], want_dweight=False, want_dbias=False)
+    dy, w = s["dy"].double(), s["w"].double()
+    want, bound = dy @ w, (nt + 8) * 2 * U * (dy.abs() @ w.abs())
+    check(dx, want, bound + e * (want.abs() + bound) + tiny, "dx")
+    s = make(nt, ni, nj, dtype, seed + 2, offset)
+    dw, = ops.linear_backward(s["dy"], s["x"], s["w"], want_dx=False, want_dbias=False)
+    dy, x = s["dy"].double().t(), s["x"].double()
+    want, bound = dy @ x, (nt + 8) * 2 * U * (dy.abs() @ x.abs())
+    check(dw, want, bound + e * (want.abs() + bound) + tiny, "dw")
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("act", ACTS)
 def test_activations(act, dtype):
