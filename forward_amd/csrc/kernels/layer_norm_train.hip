@@ -282,8 +282,8 @@ __device__ __forceinline__ void ln_columns(const LnTrain& L, int block, float (*
 }
 
 // Bound by memory and, with the column sums, by the registers that two operands, their successors and three sums per
-// element take (one workgroup of 512 per CU): 8192 x 1024 bf16 with a skip and a bias, 67 MB, 15.8 us and 3.9 for the sum of
-// the partials; 4099 x 1531 fp16 with dsum (no 16-byte alignment), 50 MB, 16.3 and 3.9 us; 509 x 768 fp32 jointly with
+// element take (one workgroup of 512 or 1024 lanes per CU): 8192 x 1024 bf16 with a skip and a bias, 67 MB, 15.8 us and 3.9 for the sum of
+// the partials; 4099 x 1531 fp16 with dsum (no 16-byte alignment), 50 MB, 14.7 and 3.9 us; 509 x 768 fp32 jointly with
 // its columns 6.2 us.
 //
 // SUMS: the column sums ride along in registers.  Rows of more than 16 elements per lane have none left for them
@@ -668,6 +668,10 @@ __global__ __launch_bounds__(256) void ln_backward_columns_kernel(const LnTrain 
 constexpr int kMaxParts = 256;       // rows of partials a backward launch leaves (its workgroups)
 constexpr int kLongParts = 32;       // the same for long rows, whose column sums are a launch of their own
 constexpr int kBackwardWG = 512;
+// Lanes of a backward workgroup (one per CU) that sums columns in registers.  Rows of 256 lanes with one slice each have few
+// bytes in flight and registers for twice the lanes: 8192 x 2048 fp16 24.3 us for 26.6, 4099 x 1531 16.5 for 17.8.  With
+// 64 lanes it is no gain (4099 x 509 9.1 for 8.4, 20000 x 300 15.8 for 16.9), and two fp32 slices spill.
+constexpr int sums_wg(int vec, int nv, int lpr) { return vec == 8 && nv == 1 && lpr == 256 ? 1024 : kBackwardWG; }
 
 // Lanes per row and steps per lane of a row of `ld` elements in slices of VEC; steps == 0: streamed.
 struct Shape {
@@ -718,9 +722,10 @@ int launch_backward(const LnTrain& L, unsigned grid, hipStream_t stream) {
   const bool columns = (int)grid > L.row_blocks;  // workgroups that sum columns
   with_full<VEC, NV, LPR>(L.ld, [&](auto full) {
     auto launch = [&](auto bias, auto sums) {
-      hipLaunchKernelGGL((ln_backward_kernel<T, VEC, NV, kBackwardWG, LPR, decltype(full)::value, decltype(bias)::value,
+      constexpr int kWG = decltype(sums)::value ? sums_wg(VEC, NV, LPR) : kBackwardWG;
+      hipLaunchKernelGGL((ln_backward_kernel<T, VEC, NV, kWG, LPR, decltype(full)::value, decltype(bias)::value,
                                              decltype(sums)::value>),
-                         dim3(grid), dim3(kBackwardWG), 0, stream, L);
+                         dim3(grid), dim3(kWG), 0, stream, L);
     };
     if (columns)
       launch(std::false_type{}, std::false_type{});
@@ -779,11 +784,11 @@ bool long_rows(int ld, int dtype) {
   return s.lpr == 0 || s.nv * vec > 16;
 }
 
-// Workgroups of rows of a backward call with column sums in registers.
-int64_t row_groups(int ld, int64_t rows, int dtype) {
+// Workgroups of rows of a backward call with column sums in registers, or with workgroups for them.
+int64_t row_groups(int ld, int64_t rows, int dtype, bool joint) {
   const int vec = dtype == FWDMI_F32 ? 4 : 8;
   const Shape s = ld < vec ? Shape{8, 1} : row_shape(ld, vec);
-  const int per = kBackwardWG / s.lpr;
+  const int per = (joint ? kBackwardWG : sums_wg(vec, s.nv, s.lpr)) / s.lpr;
   return (rows + per - 1) / per;
 }
 
@@ -791,14 +796,14 @@ int64_t row_groups(int ld, int64_t rows, int dtype) {
 // two launches, and 5 us less on the host).
 constexpr int64_t kFewRows = 1024;
 bool joint_rows(int ld, int64_t rows, int dtype, bool bias) {
-  return !bias && rows <= kFewRows && !long_rows(ld, dtype) && row_groups(ld, rows, dtype) > 1;
+  return !bias && rows <= kFewRows && !long_rows(ld, dtype) && row_groups(ld, rows, dtype, true) > 1;
 }
 
 // Rows of partials of a backward call.
 int64_t backward_parts(int ld, int64_t rows, int dtype, bool bias) {
   if (rows == 0 || joint_rows(ld, rows, dtype, bias)) return 0;
   if (long_rows(ld, dtype)) return std::min<int64_t>((rows + 3) / 4, kLongParts);
-  return std::min<int64_t>(row_groups(ld, rows, dtype), kMaxParts);
+  return std::min<int64_t>(row_groups(ld, rows, dtype, false), kMaxParts);
 }
 
 template <typename T>
@@ -820,7 +825,7 @@ int backward_typed(LnTrain& L, int64_t parts, bool long_row, hipStream_t stream)
   int64_t grid = parts;
   if (parts == 0) {
     const int dtype = sizeof(T) == 4 ? FWDMI_F32 : FWDMI_F16;
-    L.row_blocks = (int)row_groups(L.ld, L.rows, dtype);
+    L.row_blocks = (int)row_groups(L.ld, L.rows, dtype, true);
     grid = L.row_blocks + ((int64_t)L.ld + 63) / 64;
   } else {
     if (long_row) grid = std::min<int64_t>(L.rows, (int64_t)device_cus() * 2);

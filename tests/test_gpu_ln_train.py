@@ -129,6 +129,15 @@ def test_rows(rows, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("ld", [3, 64, 128, 200, 512, 768, 1024, 1030, 1531, 2048, 4096, 8192])
+@pytest.mark.parametrize("bias", [False, True])
+def test_more_rows_than_one_launch_sums(ld, bias, dtype):
+    s = make(1027, ld, dtype, ld + bias, skip=ld % 3 == 0, bias=bias, dsum=ld % 4 == 0)
+    _, mean, rstd = check_forward(s, 1e-5, False)
+    check_backward(s, mean, rstd)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("offset", [1, 2, 3, 7])
 def test_operands_start_at_any_element(offset, dtype):
     for ld in (5, 96, 1024, 1040):
