@@ -31,13 +31,37 @@ struct Operands {
 //         384 x 1024 x 4096                   10 with 48 x 32, 11 with 64 x 32, 14 with 32 x 32, 15 with 64 x 64
 //         256 x 1024 x 4096                   8 with 32 x 32, 9 with 48 x 32, 10 with 64 x 32
 //   fp32  512 x 512 x 512                     7 with 32 x 32, 9 with 64 x 32, 13 with 64 x 64
-//         1003 x 517 x 1001                   21 with 32 x 32, 25 with 64 x 64, 28 with 64 x 32
+//         1003 x 517 x 1024                   15 with 48 x 48, 20 with 32 x 32, 23 with 64 x 64
 //         256 x 1024 x 4096                   26 with 64 x 64 and four splits, 27 with 32 x 32 and two, 48 with 32 x 32 alone
-const double kRate[3][kTileKinds] = {{6.0e6, 4.6e6, 3.7e6, 3.5e6, 4.0e6, 3.5e6, 3.0e6, 3.0e6, 2.0e6},
-                                     {6.0e6, 4.6e6, 2.9e6, 1.9e6, 3.7e6, 3.0e6, 1.4e6, 0.0, 0.9e6},
-                                     {6.0e6, 4.3e6, 2.9e6, 1.8e6, 2.2e6, 2.8e6, 1.4e6, 0.0, 0.8e6}};
-const double kStep32[2][kTileKinds] = {{0, 0, 0, 0, 2.2, 1.2, 0.8, 0, 0.5}, {0, 0, 0, 0, 2.1, 1.15, 0.65, 0, 0.36}};
-const double kRound[kTileKinds] = {9.0, 4.0, 3.0, 1.5, 3.0, 1.5, 1.0, 1.0, 1.0};
+//         768 x 768 x 768                     13 with 48 x 48, 16 with 32 x 32, 17 with 64 x 64
+//         1024 x 1024 x 1024                  23 with 64 x 64 and steps of 512 bytes, 24 with 256
+//         100 x 1024 x 1024                   9 with 32 x 32 and steps of 512 bytes, 10 with 256
+const double kRate[3][kTileKinds] = {{6.0e6, 4.6e6, 3.7e6, 3.5e6, 4.0e6, 3.5e6, 3.0e6, 0, 3.0e6, 2.0e6, 0},
+                                     {6.0e6, 4.6e6, 2.9e6, 1.9e6, 3.7e6, 3.0e6, 1.4e6, 0, 0, 0.9e6, 0},
+                                     {6.0e6, 4.3e6, 2.9e6, 1.8e6, 2.2e6, 2.8e6, 1.4e6, 0, 0, 0.8e6, 0}};
+const double kStep32[2][kTileKinds] = {{0, 0, 0, 2.4, 2.2, 1.2, 0.8, 1.55, 0, 0.78, 0.5},
+                                       {0, 0, 0, 2.4, 2.1, 1.15, 0.65, 1.6, 0, 0.78, 0.36}};
+const double kRound[kTileKinds] = {9.0, 4.0, 3.0, 1.5, 3.0, 1.5, 1.0, 1.5, 1.0, 1.0, 1.0};
+
+// Where a tile is offered, with `wgs` workgroups on the fullest CU.  Tiles that fill a CU's LDS with one workgroup's deep or
+// many buffers replace those of which several fit a CU where there is no second one to fit.
+bool offered(TileKind kind, const Operands& o, double wgs) {
+  const bool half = o.elem == 2, alone = wgs <= 1;
+  switch (kind) {
+    case k256x256:
+    case k256x128: return half && o.direct;
+    case k128x128Turns: return half && o.direct && alone;
+    case k64x64Alone: return o.direct && alone;
+    case k128x128: return !(half && o.direct && alone);
+    case k64x64: return !(o.direct && alone);
+    case k48x48: return !half && o.direct && o.layouts == 0;
+    case k48x32: return half && o.direct && o.layouts == 0;
+    case k32x32Deep: return o.direct && (half || alone);
+    case k32x32: return !half && !(o.direct && alone);
+    default: return true;
+  }
+}
+
 // One step of each of `wgs` workgroups on a CU.
 double step_us(TileKind kind, const Operands& o, double wgs) {
   const TileShape t = kTiles[kind];
@@ -60,34 +84,35 @@ Plan few_plan(int ni, int nj, int nt, int elem) {
 
 Plan make_plan(int ni, int nj, int nt, const Operands& o) {
   if (o.layouts == 0 && ni <= kFewRows) return few_plan(ni, nj, nt, o.elem);
+  // (a call plans up to ten times before its launch: few divisions, none of 64 bits in the common case)
   const int cus = device_cus();
   Plan best{};
-  double best_us = 1e30;
-  for (int kind = o.elem == 2 && o.direct ? k256x256 : k128x128; kind <= (o.elem == 2 && !o.direct ? k64x32 : k32x32); ++kind) {
-    if (kind == k48x32 && (o.elem == 4 || o.layouts != 0)) continue;
+  best.us = 1e30;
+  for (int i = 0; i < kTileKinds; ++i) {
+    const TileKind kind = (TileKind)i;
+    if (!offered(kind, o, 1.0) && !offered(kind, o, 2.0)) continue;
     const TileShape t = kTiles[kind];
-    Plan p{(TileKind)kind, 1, 0, 0, 0, 0.0};
-    tail_of(nt, step_bytes(p.tile, o.layouts, o.elem, o.direct) / o.elem, o.end, p.whole_steps, p.tail);
-    const int all = p.whole_steps + (p.tail > 0);
-    const int64_t tiles = (int64_t)ceil_div(ni, t.ti) * ceil_div(nj, t.tj);
+    const int depth = step_bytes(kind, o.layouts, o.elem, o.direct) / o.elem;
+    const int all = (int)(((unsigned)nt + (unsigned)depth - 1) >> __builtin_ctz(depth));  // steps, whatever their end
+    const int64_t tiles = (int64_t)(((unsigned)ni + t.ti - 1) / (unsigned)t.ti) * (((unsigned)nj + t.tj - 1) / (unsigned)t.tj);
     for (int target = 0; target <= 2; ++target) {  // one workgroup per tile, or splits for one or two per CU
-      const int64_t want = target == 0 ? 1 : target * (int64_t)cus / tiles;
-      if (target > 0 && want < 2) continue;
-      const int splits = (int)std::min<int64_t>(want, std::max(1, all / 2));
-      p.steps_per_split = std::max(1, ceil_div(all, splits));
-      p.splits = std::max(1, ceil_div(all, p.steps_per_split));
-      const double wgs = ceil_div(tiles * p.splits, cus);
-      if ((kind == k128x128Turns || kind == k64x64Alone) && wgs > 1) continue;
-      if ((kind == k128x128 || kind == k64x64) && wgs <= 1 && o.elem == 2 && o.direct) continue;  // (those instead)
-      double us = 2.0 + wgs * kRound[kind] + p.steps_per_split * step_us((TileKind)kind, o, wgs);
-      if (p.splits > 1) us += 3.0 + 6.0 * p.splits * ni * nj / 5.0e6;
-      if (us < best_us) {
-        best_us = us;
-        best = p;
-        best.us = us;
+      int splits = 1, per = std::max(1, all);
+      if (target > 0) {
+        if (tiles * 2 > (int64_t)target * cus) continue;
+        const int want = std::min(target * cus / (int)tiles, all / 2);
+        if (want < 2) continue;
+        per = (all + want - 1) / want;
+        splits = (all + per - 1) / per;
       }
+      const int64_t total = tiles * splits;
+      const double wgs = total <= cus ? 1 : ceil_div(total, cus);
+      if (!offered(kind, o, wgs)) continue;
+      double us = 2.0 + wgs * kRound[kind] + per * step_us(kind, o, wgs);
+      if (splits > 1) us += 3.0 + 6.0 * splits * ni * nj / 5.0e6;
+      if (us < best.us) best = Plan{kind, splits, 0, 0, per, us};
     }
   }
+  tail_of(nt, step_bytes(best.tile, o.layouts, o.elem, o.direct) / o.elem, o.end, best.whole_steps, best.tail);
   return best;
 }
 
@@ -162,14 +187,12 @@ bool together(const Product& x, const Product& w, int dtype, Gradients& G, bool&
   return found;
 }
 
-// Partial products of any plan that `run` may choose for these sizes (that depends on the operands' alignment too).
+// Partial products of any plan that `run` may choose for these sizes: that depends on the operands' alignment too, but not
+// on how the end of t is loaded.
 size_t product_bytes(int layouts, int64_t ni, int64_t nj, int64_t nt, int elem) {
   size_t bytes = 0;
-  for (const Operands& o : {Operands{layouts, elem, true, kWhole}, Operands{layouts, elem, true, kTail},
-                            Operands{layouts, elem, true, kTailLine}, Operands{layouts, elem, false, kTail}}) {
-    if (o.end == kTailLine && layouts == 0) continue;
+  for (const Operands& o : {Operands{layouts, elem, true, kWhole}, Operands{layouts, elem, false, kTail}})
     bytes = std::max(bytes, partial_bytes(make_plan((int)ni, (int)nj, (int)nt, o), (int)ni, (int)nj));
-  }
   return bytes;
 }
 

@@ -436,7 +436,7 @@ __device__ __forceinline__ void leave_tile(const Product& P, const F4 (&acc)[FJ]
   constexpr int kFP = FI / kPhases;                // fragments of i a wave leaves per phase
   constexpr int kRowsPhase = TI / kPhases;          // rows of all waves per phase
   constexpr int kRowsWave = kRowsPhase / WI;
-  constexpr int kMix = (TJ / 4 < 16 ? TJ / 4 : 16) - 1;
+  constexpr int kMix = ((TJ / 4 & -(TJ / 4)) < 16 ? TJ / 4 & -(TJ / 4) : 16) - 1;  // of a row's chunks, an even share
   constexpr int kSlab = kRowsPhase * TJ;            // elements of a wave group's part of the sum over t
   float* const s_out = reinterpret_cast<float*>(s_tile);
   float* const s_mine = s_out + wave / (WI * WJ) * kSlab;
@@ -596,8 +596,8 @@ __device__ __forceinline__ void leave_registers(const Product& P, const F4 (&acc
 
 // The work of workgroup `block` of `blocks` on product P.  Products of these sizes are bound by the latency of their few
 // steps and by what a CU loads, 90 KB/us (384 x 1024 x 4096 fp16: 9.6 us, 335 TFLOP/s, of which 7.1 are its 640 KB), or, in fp32, by the matrix
-// instructions and LDS in turn (1003 x 517 x 1001: 22 us, 46 TFLOP/s; 8192 x 1024 x 4096: 126, where a large library product
-// reaches 145).  The waves are WI x WJ over the tile and WK over the halves of
+// instructions and LDS in turn (1003 x 517 x 1024: 15.5 us, 69 TFLOP/s; 8192 x 1024 x 4096: 126, where a large library
+// product reaches 145).  The waves are WI x WJ over the tile and WK over the halves of
 // a step (their sums meet in LDS): small tiles, whose waves would otherwise have little to do between two barriers.
 template <typename T, int LA, int LB, int TI, int TJ, int WI, int WJ, int WK, int STEP, int STAGES, bool DIRECT>
 struct Work {
@@ -1062,41 +1062,43 @@ int launch_product(Product& P, const Plan& plan, hipStream_t stream) {
   const int64_t tiles = (int64_t)P.tiles_i * P.tiles_j * plan.splits;
   if (const int rc = check_launch(tiles, 512)) return rc;
   const dim3 grid((unsigned)tiles);
-  if constexpr (sizeof(T) == 2 && DIRECT) {
+#define FWDMI_PRODUCT(KIND_, ...)                                                                                  \
+  if (plan.tile == KIND_) {                                                                                       \
+    using W = Work<T, LA, LB, __VA_ARGS__, DIRECT>;                                                               \
+    hipLaunchKernelGGL((product_kernel<W>), grid, dim3(W::kThreads), 0, stream, P);                               \
+  }
+  constexpr bool kHalf = sizeof(T) == 2, kBothAlong = LA == kAlong && LB == kAlong;
+  if constexpr (kHalf && DIRECT) {
     if (plan.tile == k256x256)
       hipLaunchKernelGGL((product_turns_kernel<T, LA, LB, 256, 256, 2, 4, 128, 2>), grid, dim3(512), 0, stream, P);
     if (plan.tile == k256x128)
       hipLaunchKernelGGL((product_turns_kernel<T, LA, LB, 256, 128, 4, 2, 128, 3>), grid, dim3(512), 0, stream, P);
     if (plan.tile == k128x128Turns)
       hipLaunchKernelGGL((product_turns_kernel<T, LA, LB, 128, 128, 2, 4, 128, 3>), grid, dim3(512), 0, stream, P);
-    if (plan.tile == k64x64Alone) {
-      if constexpr (LA == kAlong && LB == kAlong)
-        hipLaunchKernelGGL((product_kernel<Work<T, LA, LB, 64, 64, 2, 1, 4, 256, 3, true>>), grid, dim3(512), 0, stream, P);
-      else
-        hipLaunchKernelGGL((product_kernel<Work<T, LA, LB, 64, 64, 1, 1, 8, 512, 2, true>>), grid, dim3(512), 0, stream, P);
+  }
+  FWDMI_PRODUCT(k128x128, 128, 128, 2, 2, 1, 128, 2)
+  FWDMI_PRODUCT(k64x64, 64, 64, 2, 1, 4, 256, 2)
+  if constexpr (DIRECT) {
+    FWDMI_PRODUCT(k32x32Deep, 32, 32, 1, 1, 8, 512, 3)
+    if constexpr (kHalf && kBothAlong) {
+      FWDMI_PRODUCT(k64x64Alone, 64, 64, 2, 1, 4, 256, 3)
+      FWDMI_PRODUCT(k48x32, 48, 32, 1, 1, 8, 512, 3)
+    } else {
+      FWDMI_PRODUCT(k64x64Alone, 64, 64, 1, 1, 8, 512, 2)
     }
   }
-  if (plan.tile == k128x128)
-    hipLaunchKernelGGL((product_kernel<Work<T, LA, LB, 128, 128, 2, 2, 1, 128, 2, DIRECT>>), grid, dim3(256), 0, stream, P);
-  if (plan.tile == k64x64)
-    hipLaunchKernelGGL((product_kernel<Work<T, LA, LB, 64, 64, 2, 1, 4, 256, 2, DIRECT>>), grid, dim3(512), 0, stream, P);
-  if constexpr (sizeof(T) == 2 && DIRECT) {
-    if (plan.tile == k64x32)
-      hipLaunchKernelGGL((product_kernel<Work<T, LA, LB, 64, 32, 2, 1, 4, 512, 3, true>>), grid, dim3(512), 0, stream, P);
-    if constexpr (LA == kAlong && LB == kAlong)
-      if (plan.tile == k48x32)
-        hipLaunchKernelGGL((product_kernel<Work<T, LA, LB, 48, 32, 1, 1, 8, 512, 3, true>>), grid, dim3(512), 0, stream, P);
-    if (plan.tile == k32x32)
-      hipLaunchKernelGGL((product_kernel<Work<T, LA, LB, 32, 32, 1, 1, 8, 512, 3, true>>), grid, dim3(512), 0, stream, P);
+  if constexpr (kHalf && DIRECT) {
+    FWDMI_PRODUCT(k64x32, 64, 32, 2, 1, 4, 512, 3)
   } else {
-    if (plan.tile == k64x32)
-      hipLaunchKernelGGL((product_kernel<Work<T, LA, LB, 64, 32, 2, 1, 4, 256, DIRECT ? 4 : 2, DIRECT>>), grid, dim3(512), 0,
-                         stream, P);
+    FWDMI_PRODUCT(k64x32, 64, 32, 2, 1, 4, 256, (DIRECT ? 4 : 2))
   }
-  if constexpr (sizeof(T) == 4) {
-    if (plan.tile == k32x32)
-      hipLaunchKernelGGL((product_kernel<Work<T, LA, LB, 32, 32, 1, 1, 4, 256, 2, DIRECT>>), grid, dim3(256), 0, stream, P);
+  if constexpr (!kHalf) {
+    FWDMI_PRODUCT(k32x32, 32, 32, 1, 1, 4, 256, 2)
+    if constexpr (DIRECT && kBothAlong) {
+      FWDMI_PRODUCT(k48x48, 48, 48, 1, 1, 8, 512, 3)
+    }
   }
+#undef FWDMI_PRODUCT
   FWDMI_HIP_CHECK(hipGetLastError());
   return plan.splits > 1 ? launch_finish<T>(P, plan.splits, stream) : FWDMI_OK;
 }

@@ -40,28 +40,29 @@ struct Slope {
   int32_t act;
 };
 
-// The tiles there are.  The first three are the eight-wave kernel of 16-bit operands (product_turns_kernel).
-// Those and k64x64Alone, k48x32 and 16-bit k32x32 take operands that are loaded directly.  k128x128Turns and k64x64Alone
-// are for launches of at most one workgroup per CU, where they replace k128x128 and k64x64, of which two fit a CU; k48x32
-// is for operands along t.  kFew: product_few_kernel, at most kFewRows rows of x.
+// The tiles there are; `offered` in linear.hip says where.  The first three are the eight-wave kernel of 16-bit operands
+// (product_turns_kernel), the others product_kernel with one shape of waves, step and buffers or another.  kFew:
+// product_few_kernel, at most kFewRows rows of x.
 enum TileKind {
-  k256x256, k256x128, k128x128Turns, k64x64Alone, k128x128, k64x64, k64x32, k48x32, k32x32, kTileKinds, kFew = kTileKinds
+  k256x256, k256x128, k128x128Turns, k64x64Alone, k128x128, k64x64, k64x32, k48x48, k48x32, k32x32Deep, k32x32, kTileKinds,
+  kFew = kTileKinds
 };
 constexpr int kFewRows = 32;
 struct TileShape {
   int ti, tj;
 };
-constexpr TileShape kTiles[kTileKinds] = {{256, 256}, {256, 128}, {128, 128}, {64, 64}, {128, 128},
-                                          {64, 64},   {64, 32},   {48, 32},   {32, 32}};
+constexpr TileShape kTiles[kTileKinds] = {{256, 256}, {256, 128}, {128, 128}, {64, 64}, {128, 128}, {64, 64},
+                                          {64, 32},   {48, 48},   {48, 32},   {32, 32}, {32, 32}};
 
-// Bytes of t in a step.  The smallest tiles have the least to do between two barriers: 16-bit operands straight from memory,
-// which need no registers on the way, take 512 (512 x 1024 x 4096: 10.5 us, with 256 11.8).  So does k64x64Alone with
-// operands across t: a wave then multiplies all of the tile, which halves what it reads of it (1024 x 1024 x 4096, b
-// across: 22 us, 26 with three buffers of 256); with both along t three buffers are better (15 us, 19).
+// Bytes of t in a step.  The smallest tiles have the least to do between two barriers: operands straight from memory, which
+// need no registers on the way, take 512 (fp16 512 x 1024 x 4096: 10.5 us, with 256 11.8).  So does k64x64Alone: a wave
+// then multiplies all of the tile, which halves what it reads of it (bf16 1024 x 1024 x 4096, b across: 22 us, 26 with
+// three buffers of 256); but 16-bit operands along t are better off with three buffers (15 us, 19).
 inline int step_bytes(TileKind kind, int layouts, int elem, bool direct) {
   if (kind <= k128x128Turns || kind == k128x128) return 128;
-  if (kind == k64x64Alone) return layouts == 0 ? 256 : 512;
-  return kind >= k64x32 && elem == 2 && direct ? 512 : 256;
+  if (kind == k64x64Alone) return layouts == 0 && elem == 2 ? 256 : 512;
+  if (kind == k64x32) return elem == 2 && direct ? 512 : 256;
+  return kind == k48x48 || kind == k48x32 || kind == k32x32Deep ? 512 : 256;
 }
 
 struct Plan {
