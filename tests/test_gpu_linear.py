@@ -21,7 +21,7 @@ TYPES = [torch.float32, torch.float16, torch.bfloat16]
 ACTS = ["none", "relu", "gelu", "gelu_tanh", "silu"]
 # (m, n, k): single elements, rows that are no whole 16-byte lines, tile edges on every side, empty sums, long sums of
 # few tiles (split), and enough tiles for each tile size
-SHAPES = [(1, 1, 1), (1, 17, 5), (3, 64, 64), (5, 130, 72), (16, 24, 0), (64, 64, 64), (65, 63, 129), (128, 128, 8),
+SHAPES = [(1, 1, 1), (1, 1, 4111), (1, 17, 5), (3, 64, 64), (5, 130, 72), (16, 24, 0), (64, 64, 64), (65, 63, 129), (128, 128, 8),
           (1, 1024, 2048), (9, 40, 9001), (30, 136, 8200), (7, 264, 4104), (200, 1000, 136), (257, 511, 1031), (1000, 517, 1001), (300, 4096, 1024),
           (250, 1000, 1034), (380, 1002, 520), (500, 1000, 2050), (900, 1026, 2050), (1000, 7, 8000), (1111, 2048, 72), (1931, 1930, 2042), (4000, 3336, 136)]
 
