@@ -364,6 +364,9 @@ class Linear(torch.nn.Module):
         out.weight, out.bias, out.activation = m.weight, m.bias, activation
         return out
 
+    in_features = property(lambda self: self.weight.shape[1])
+    out_features = property(lambda self: self.weight.shape[0])
+
     def forward(self, x, residual=None):
         keep = self.activation != "none" and torch.is_grad_enabled() and (
             x.requires_grad or self.weight.requires_grad or (self.bias is not None and self.bias.requires_grad)
@@ -375,12 +378,13 @@ class Linear(torch.nn.Module):
 
 class LayerNorm(torch.nn.Module):
     """``nn.LayerNorm`` over the last axis of ``x (+ skip) (+ bias)``, for training and serving.  ``forward(x, skip, bias)``
-    returns the normalised rows, with ``keep_sum`` ``(rows, sum)``: the residual stream of a pre-norm layer."""
+    returns the normalised rows, with ``keep_sum`` ``(rows, sum)``: the residual stream of a pre-norm layer.  The parameters
+    have ``nn.LayerNorm``'s names."""
 
     def __init__(self, size, eps=1e-5, keep_sum=False, device=None, dtype=None):
         super().__init__()
-        self.gamma = torch.nn.Parameter(torch.ones(size, device=device, dtype=dtype))
-        self.beta = torch.nn.Parameter(torch.zeros(size, device=device, dtype=dtype))
+        self.weight = torch.nn.Parameter(torch.ones(size, device=device, dtype=dtype))
+        self.bias = torch.nn.Parameter(torch.zeros(size, device=device, dtype=dtype))
         self.eps, self.keep_sum = float(eps), keep_sum
 
     @classmethod
@@ -390,12 +394,16 @@ class LayerNorm(torch.nn.Module):
             raise NotImplementedError("layer norm over one axis, with weight and bias")
         out = cls.__new__(cls)
         torch.nn.Module.__init__(out)
-        out.gamma, out.beta, out.eps, out.keep_sum = m.weight, m.bias, float(m.eps), keep_sum
+        out.weight, out.bias, out.eps, out.keep_sum = m.weight, m.bias, float(m.eps), keep_sum
         return out
+
+    gamma = property(lambda self: self.weight)
+    beta = property(lambda self: self.bias)
+    normalized_shape = property(lambda self: tuple(self.weight.shape))
 
     def forward(self, x, skip=None, bias=None):
         op = torch.ops.fwdmi.layer_norm_train_sum if self.keep_sum else torch.ops.fwdmi.layer_norm_train
-        got = op(x, skip, self.gamma, self.beta, bias, self.eps)
+        got = op(x, skip, self.weight, self.bias, bias, self.eps)
         return got[:2] if self.keep_sum else got[0]
 
 
@@ -512,7 +520,7 @@ def replace_embedding_modules(model):
 
 def replace_dense_modules(model):
     """Swaps every ``nn.Linear`` and every ``nn.LayerNorm`` over one axis (with weight and bias) in place; the parameters
-    are shared, so an optimizer that holds them keeps working."""
+    are shared and keep their names, so an optimizer that holds them and checkpoints of the model keep working."""
     for name, child in list(model.named_children()):
         if type(child) is torch.nn.Linear:
             setattr(model, name, Linear.from_torch(child))

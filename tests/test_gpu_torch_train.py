@@ -48,8 +48,8 @@ def pair(hidden, inner, activation, dtype, seed=0):
         ref.norm.weight.normal_(1.0, 0.2)
         ref.norm.bias.normal_(0.0, 0.2)
     mine = torch_ops.FeedForward(hidden, inner, activation=activation, eps=1e-5, device="cuda", dtype=dtype)
-    names = (("up.weight",) * 2, ("up.bias",) * 2, ("down.weight",) * 2, ("down.bias",) * 2, ("norm.gamma", "norm.weight"),
-             ("norm.beta", "norm.bias"))
+    names = (("up.weight",) * 2, ("up.bias",) * 2, ("down.weight",) * 2, ("down.bias",) * 2, ("norm.weight",) * 2,
+             ("norm.bias",) * 2)
     own, theirs = dict(mine.named_parameters()), dict(ref.named_parameters())
     with torch.no_grad():
         for a, b in names:
