@@ -346,6 +346,28 @@ layer_norm_train.register_autograd(_norm_grad, setup_context=_norm_setup)
 layer_norm_train_sum.register_autograd(_norm_grad, setup_context=_norm_setup)
 
 
+_HOOKS = ("_forward_hooks", "_forward_pre_hooks", "_backward_hooks", "_backward_pre_hooks", "_state_dict_hooks",
+          "_state_dict_pre_hooks", "_load_state_dict_pre_hooks", "_load_state_dict_post_hooks")
+
+
+def _is_plain(m):
+    """Whether layer ``m`` is its weight and its bias and nothing else, so that a module which shares them can stand in its
+    place.  A weight that a hook or a parametrization computes from others (weight_norm, spectral_norm, pruning) is no
+    parameter of the layer; hooks, buffers and a ``forward`` of its own would be lost."""
+    return (set(m._parameters) == {"weight", "bias"} and m.weight is not None and not m._buffers and not m._modules
+            and "forward" not in m.__dict__ and not any(getattr(m, h, None) for h in _HOOKS))
+
+
+def _stand_in(cls, m, what):
+    """A module of ``cls`` that shares the parameters of ``m``."""
+    if not _is_plain(m):
+        raise NotImplementedError("%s with weight and bias of its own and without hooks" % what)
+    out = cls.__new__(cls)
+    torch.nn.Module.__init__(out)
+    out.weight, out.bias = m.weight, m.bias
+    return out
+
+
 class Linear(torch.nn.Module):
     """``nn.Linear`` with its activation and a residual in the product's epilogue: ``act(x W^T + b) (+ residual)``.
     Trains and serves; ``activation`` is a key of ``ops.ACTIVATIONS``."""
@@ -358,10 +380,10 @@ class Linear(torch.nn.Module):
 
     @classmethod
     def from_torch(cls, m, activation="none"):
-        """Shares the parameters of an ``nn.Linear``."""
-        out = cls.__new__(cls)
-        torch.nn.Module.__init__(out)
-        out.weight, out.bias, out.activation = m.weight, m.bias, activation
+        """Shares the parameters of an ``nn.Linear``.  One whose weight is recomputed (weight_norm and its like) or that has
+        hooks is refused."""
+        out = _stand_in(cls, m, "a linear layer")
+        out.activation = activation
         return out
 
     in_features = property(lambda self: self.weight.shape[1])
@@ -389,12 +411,12 @@ class LayerNorm(torch.nn.Module):
 
     @classmethod
     def from_torch(cls, m, keep_sum=False):
-        """Shares the parameters of an ``nn.LayerNorm`` over one axis with weight and bias."""
+        """Shares the parameters of an ``nn.LayerNorm`` over one axis with weight and bias.  One whose parameters are
+        recomputed or that has hooks is refused."""
         if len(m.normalized_shape) != 1 or m.weight is None or m.bias is None:
             raise NotImplementedError("layer norm over one axis, with weight and bias")
-        out = cls.__new__(cls)
-        torch.nn.Module.__init__(out)
-        out.weight, out.bias, out.eps, out.keep_sum = m.weight, m.bias, float(m.eps), keep_sum
+        out = _stand_in(cls, m, "a layer norm")
+        out.eps, out.keep_sum = float(m.eps), keep_sum
         return out
 
     gamma = property(lambda self: self.weight)
@@ -519,14 +541,19 @@ def replace_embedding_modules(model):
 
 
 def replace_dense_modules(model):
-    """Swaps every ``nn.Linear`` and every ``nn.LayerNorm`` over one axis (with weight and bias) in place; the parameters
-    are shared and keep their names, so an optimizer that holds them and checkpoints of the model keep working."""
+    """Swaps the ``nn.Linear`` and the ``nn.LayerNorm`` over one axis (with weight and bias) below ``model`` in place; the
+    parameters are shared and keep their names, so an optimizer that holds them and checkpoints of the model keep working.
+
+    Layers that are more than their parameters stay as they are: a weight that is recomputed from others (weight_norm,
+    spectral_norm, pruning, parametrizations), hooks, a ``forward`` of the instance's own.  So does ``model`` itself
+    (``Linear.from_torch`` takes a layer that stands alone)."""
     for name, child in list(model.named_children()):
         if type(child) is torch.nn.Linear:
-            setattr(model, name, Linear.from_torch(child))
-        elif type(child) is torch.nn.LayerNorm and len(child.normalized_shape) == 1 and child.weight is not None \
-                and child.bias is not None:
-            setattr(model, name, LayerNorm.from_torch(child))
+            if _is_plain(child):
+                setattr(model, name, Linear.from_torch(child))
+        elif type(child) is torch.nn.LayerNorm:
+            if _is_plain(child) and len(child.normalized_shape) == 1 and child.bias is not None:
+                setattr(model, name, LayerNorm.from_torch(child))
         else:
             replace_dense_modules(child)
     return model
