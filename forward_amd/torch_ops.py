@@ -359,12 +359,12 @@ def _is_plain(m):
 
 
 def _stand_in(cls, m, what):
-    """A module of ``cls`` that shares the parameters of ``m``."""
+    """A module of ``cls`` that shares the parameters of ``m`` and its training flag."""
     if not _is_plain(m):
         raise NotImplementedError("%s with weight and bias of its own and without hooks" % what)
     out = cls.__new__(cls)
     torch.nn.Module.__init__(out)
-    out.weight, out.bias = m.weight, m.bias
+    out.weight, out.bias, out.training = m.weight, m.bias, m.training
     return out
 
 

@@ -90,6 +90,13 @@ def test_a_weight_under_weight_norm_still_trains_and_loads():
     assert torch.equal(model(x), before)
 
 
+def test_the_training_flag_goes_along():
+    model = torch.nn.Sequential(torch.nn.Linear(4, 4), torch.nn.LayerNorm(4)).eval()
+    torch_ops.replace_dense_modules(model)
+    assert isinstance(model[0], torch_ops.Linear) and not any(m.training for m in model.modules())
+    assert torch_ops.Linear.from_torch(torch.nn.Linear(4, 4)).training
+
+
 def test_the_model_itself_is_returned_as_it_is():
     layer = torch.nn.Linear(4, 4)
     assert torch_ops.replace_dense_modules(layer) is layer and type(layer) is torch.nn.Linear
