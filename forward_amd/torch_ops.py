@@ -547,13 +547,25 @@ def replace_dense_modules(model):
     Layers that are more than their parameters stay as they are: a weight that is recomputed from others (weight_norm,
     spectral_norm, pruning, parametrizations), hooks, a ``forward`` of the instance's own.  So does ``model`` itself
     (``Linear.from_torch`` takes a layer that stands alone)."""
-    for name, child in list(model.named_children()):
-        if type(child) is torch.nn.Linear:
-            if _is_plain(child):
-                setattr(model, name, Linear.from_torch(child))
-        elif type(child) is torch.nn.LayerNorm:
-            if _is_plain(child) and len(child.normalized_shape) == 1 and child.bias is not None:
-                setattr(model, name, LayerNorm.from_torch(child))
-        else:
-            replace_dense_modules(child)
+    _swap_dense(model, {})
     return model
+
+
+def _swap_dense(model, seen):
+    for name, child in list(model._modules.items()):
+        if child is None:
+            continue
+        if id(child) not in seen:              # (a layer that stands in two places stays one layer)
+            new = child
+            if type(child) is torch.nn.Linear:
+                if _is_plain(child):
+                    new = Linear.from_torch(child)
+            elif type(child) is torch.nn.LayerNorm:
+                if _is_plain(child) and len(child.normalized_shape) == 1 and child.bias is not None:
+                    new = LayerNorm.from_torch(child)
+            seen[id(child)] = (child, new)     # (the layer too, so that no other one gets its id)
+            if new is child:
+                _swap_dense(child, seen)
+        new = seen[id(child)][1]
+        if new is not child:
+            setattr(model, name, new)

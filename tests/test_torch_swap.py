@@ -97,6 +97,16 @@ def test_the_training_flag_goes_along():
     assert torch_ops.Linear.from_torch(torch.nn.Linear(4, 4)).training
 
 
+def test_a_layer_in_two_places_stays_one():
+    layer, norm = torch.nn.Linear(4, 4), torch.nn.LayerNorm(4)
+    model = torch.nn.Sequential(layer, norm, layer, torch.nn.Sequential(layer, norm), torch.nn.ModuleDict({"a": layer}))
+    count = sum(1 for _ in model.parameters())
+    torch_ops.replace_dense_modules(model)
+    assert isinstance(model[0], torch_ops.Linear) and isinstance(model[1], torch_ops.LayerNorm)
+    assert model[2] is model[0] and model[3][0] is model[0] and model[3][1] is model[1] and model[4]["a"] is model[0]
+    assert sum(1 for _ in model.parameters()) == count and model[0].weight is layer.weight
+
+
 def test_the_model_itself_is_returned_as_it_is():
     layer = torch.nn.Linear(4, 4)
     assert torch_ops.replace_dense_modules(layer) is layer and type(layer) is torch.nn.Linear
