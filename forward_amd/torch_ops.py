@@ -370,7 +370,8 @@ def _stand_in(cls, m, what):
 
 class Linear(torch.nn.Module):
     """``nn.Linear`` with its activation and a residual in the product's epilogue: ``act(x W^T + b) (+ residual)``.
-    Trains and serves; ``activation`` is a key of ``ops.ACTIVATIONS``."""
+    Trains and serves; ``activation`` is a key of ``ops.ACTIVATIONS``.  ``forward(x, residual, add_bias=False)`` leaves the
+    bias to a norm that follows (``LayerNorm.forward``'s ``bias``)."""
 
     def __init__(self, in_features, out_features, bias=True, activation="none", device=None, dtype=None):
         super().__init__()
@@ -389,13 +390,14 @@ class Linear(torch.nn.Module):
     in_features = property(lambda self: self.weight.shape[1])
     out_features = property(lambda self: self.weight.shape[0])
 
-    def forward(self, x, residual=None):
+    def forward(self, x, residual=None, add_bias=True):
+        bias = self.bias if add_bias else None
         keep = self.activation != "none" and torch.is_grad_enabled() and (
-            x.requires_grad or self.weight.requires_grad or (self.bias is not None and self.bias.requires_grad)
+            x.requires_grad or self.weight.requires_grad or (bias is not None and bias.requires_grad)
             or (residual is not None and residual.requires_grad))
         if keep:
-            return torch.ops.fwdmi.linear_preact(x, self.weight, self.bias, residual, self.activation)[0]
-        return torch.ops.fwdmi.linear(x, self.weight, self.bias, residual, self.activation)
+            return torch.ops.fwdmi.linear_preact(x, self.weight, bias, residual, self.activation)[0]
+        return torch.ops.fwdmi.linear(x, self.weight, bias, residual, self.activation)
 
 
 class LayerNorm(torch.nn.Module):
@@ -440,7 +442,7 @@ class FeedForward(torch.nn.Module):
         self.norm = LayerNorm(hidden, eps=eps, device=device, dtype=dtype)
 
     def forward(self, x):
-        f = torch.ops.fwdmi.linear(self.up(x), self.down.weight, None, None, "none")
+        f = self.down(self.up(x), add_bias=False)      # (a call of the module: its hooks run)
         return self.norm(f, skip=x, bias=self.down.bias)
 
 
