@@ -386,7 +386,8 @@ def emb_layer_norm(input_ids, segment_ids, input_mask, word, pos, tok, gamma, be
 # plain integers, the stream handle comes without a Stream object around it, and nothing is allocated that the result
 # does not need.
 
-_raw_stream = torch._C._cuda_getCurrentRawStream
+# (a PyTorch without device support lacks the first; no call gets as far there, but the module is imported)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 _current_device = torch.cuda.current_device
 
 
