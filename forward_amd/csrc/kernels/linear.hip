@@ -155,7 +155,8 @@ int64_t whole_tiles(Product& P, TileKind kind, const Operands& o) {
 }
 
 // Whether both products of a gradient are faster in one launch of unsplit tiles than in launches of their own (whose gap
-// is about 3 us), and if so that launch, but for dbias.  771 x 1011 x 768 fp16: 12 us together, 10 and 8 us apart.
+// is about 3 us), and if so that launch, but for dbias.  771 x 1011 x 768 fp16: 12 us together, 10 and 8 us apart.  (Tiles of
+// both and the columns of dbias that one launch cannot hold stay apart, where each product may still fit.)
 bool together(const Product& x, const Product& w, int dtype, Gradients& G, bool& direct) {
   const int elem = elem_size(dtype), cus = device_cus();
   Operands ox = operands_of(x, 1, elem), ow = operands_of(w, 2, elem);
@@ -170,6 +171,7 @@ bool together(const Product& x, const Product& w, int dtype, Gradients& G, bool&
     if (kind == k32x32 && elem == 2) break;
     Product px = x, pw = w;
     const int64_t tx = whole_tiles(px, kind, ox), tw = whole_tiles(pw, kind, ow);
+    if (!launchable(tx + tw + ceil_div(w.ni, 64), kTiles[kind].ti * 8)) continue;
     const int sx = px.steps_per_split, sw = pw.steps_per_split;
     const double wgs = ceil_div(tx + tw, cus), mean = ((double)tx * sx + (double)tw * sw) / (double)(tx + tw);
     const double us = 2.0 + wgs * kRound[kind] +

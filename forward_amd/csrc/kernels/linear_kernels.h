@@ -1115,7 +1115,9 @@ int run_product(Product& P, int layouts, const Plan& plan, bool direct, hipStrea
 }
 template <typename T>
 int run_gradients(const Gradients& G, bool direct, hipStream_t stream) {
-  const dim3 grid((unsigned)(G.blocks_x + G.blocks_w + (G.dbias ? ceil_div(G.n, 64) : 0)));
+  const int64_t blocks = (int64_t)G.blocks_x + G.blocks_w + (G.dbias ? ceil_div(G.n, 64) : 0);
+  if (const int rc = check_launch(blocks, kTiles[G.tile].ti * 8)) return rc;
+  const dim3 grid((unsigned)blocks);
   if (G.tile == k64x64) {
     if (direct)
       hipLaunchKernelGGL((gradients_kernel<T, 64, true>), grid, dim3(512), 0, stream, G);

@@ -82,8 +82,9 @@ __global__ __launch_bounds__(64 * kSumWaves) void column_sums_kernel(const Colum
 }
 
 // A launch holds fewer than 2^32 work-items.
+inline bool launchable(int64_t workgroups, int threads) { return workgroups <= 0xffffffffll / threads; }
 inline int check_launch(int64_t workgroups, int threads) {
-  if (workgroups <= 0xffffffffll / threads) return FWDMI_OK;
+  if (launchable(workgroups, threads)) return FWDMI_OK;
   return set_error(FWDMI_ERR_UNSUPPORTED, "a launch of %lld workgroups of %d", (long long)workgroups, threads);
 }
 
