@@ -144,6 +144,15 @@ int run(Product& P, int layouts, int dtype, void* workspace, hipStream_t stream)
                                : run_product_f32(P, layouts, plan, o.direct, stream);
 }
 
+// Whether the launches that `run` would make hold this product (asked for where a call makes several, before the first).
+int check_product(const Product& P, int layouts, int dtype) {
+  constexpr int kMost = 512;  // work-items of a workgroup; the smallest tile is 32 x 32, and what is split has few tiles
+  if (launchable(((int64_t)P.ni + 31) / 32 * (((int64_t)P.nj + 31) / 32), kMost)) return FWDMI_OK;
+  const Plan plan = make_plan(P.ni, P.nj, P.nt, operands_of(P, layouts, elem_size(dtype)));
+  const TileShape t = kTiles[plan.tile];
+  return check_launch((int64_t)ceil_div(P.ni, t.ti) * ceil_div(P.nj, t.tj) * plan.splits, kMost);
+}
+
 // Fills in P as one unsplit pass over tiles of `kind`; returns the number of tiles.
 int64_t whole_tiles(Product& P, TileKind kind, const Operands& o) {
   const TileShape t = kTiles[kind];
@@ -374,6 +383,11 @@ int fwdmi_linear_backward(void* stream, int64_t m, int64_t n, int64_t k, const v
   // few rows are summed straight from dy by the joint launch
   const bool sum_dy = joint && act == FWDMI_ACT_NONE && m <= 1024;
   int rc = FWDMI_OK;
+  if (!joint) {  // (a joint launch is one that holds both)
+    if (dx) rc = check_product(X, 1, dtype);
+    if (dw && rc == FWDMI_OK) rc = check_product(W, 2, dtype);
+    if (rc != FWDMI_OK) return rc;
+  }
   if (copy && act == FWDMI_ACT_NONE && (sum_dy || !dbias)) {  // (a plain copy, 4 us for 771 x 1011; 5 with partial sums)
     rc = run_widen(Widen{{dy, nullptr}, {ws, nullptr}, {m, 0}, (int)n, (int)space.ld_dz}, s);
     if (rc != FWDMI_OK) return rc;

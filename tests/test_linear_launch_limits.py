@@ -12,7 +12,7 @@ def test_both_products_are_held_to_the_limit_of_each(dtype):
     d, p, big = lib.dll, 1 << 20, (1 << 64) - 1
     call = lambda m, n, k, dx, dw, db: d.fwdmi_linear_backward(None, m, n, k, p, p, p, None, dx, dw, db, 0, dtype, p, big)
     seen = set()
-    for m, n in ((33, 33), (40, 48), (300, 300)):
+    for m, n in ((33, 33), (40, 48), (64, 2), (300, 300)):
         for k in (1 << 12, 1 << 26, (1 << 27) - 8, 1 << 28, 1 << 29, (1 << 30) - 1, 1 << 30):
             alone = {call(m, n, k, p, None, None), call(m, n, k, None, p, None)}
             # (ERR_HIP: no device here, it got as far as the launch)
