@@ -91,6 +91,13 @@ __device__ __forceinline__ float row_sum(float x, float* scratch) {
   }
 }
 
+// 1 / sqrt(v) to 1 ulp.  The instruction takes subnormal numbers for zero: rows of values near 1e-19 (fp32, bf16) without an
+// eps have such variances, and are scaled by powers of two, which changes no bit of any other row's result.
+__device__ __forceinline__ float inverse_root(float v) {
+  const bool small = v < 0x1p-100f;
+  return __builtin_amdgcn_rsqf(small ? v * 0x1p100f : v) * (small ? 0x1p50f : 1.0f);
+}
+
 // Where a lane's slices lie: columns col[j] .. col[j] + VEC, of which the first drop[j] belong to another lane
 // (the row's end) or to nobody (drop == VEC).  FULL: ld == LPR * VEC * NV, every element is the lane's own.
 template <int VEC, int NV, int LPR, bool FULL>
@@ -196,7 +203,7 @@ __global__ __launch_bounds__(WG) void ln_forward_kernel(const LnTrain L) {
         m2 = __builtin_fmaf(d, d, m2);
       }
     m2 = row_sum<WG, LPR>(m2, s_red + (phase * 2 + 1) * (WG / 64));
-    const float rs = __builtin_amdgcn_rsqf(__builtin_fmaf(m2, inv_n, L.eps));  // 1 ulp
+    const float rs = inverse_root(__builtin_fmaf(m2, inv_n, L.eps));
     if (row_ok) {
       if (gl == 0) {
         gmut<float>(L.mean)[r] = mu;
@@ -536,7 +543,7 @@ __global__ __launch_bounds__(kStreamWG) void ln_forward_stream_kernel(const LnTr
         a = __builtin_fmaf(d, d, a);
       }
     });
-    const float rs = __builtin_amdgcn_rsqf(__builtin_fmaf(wg_sum<kStreamWG>(a, s_red), inv_n, L.eps));
+    const float rs = inverse_root(__builtin_fmaf(wg_sum<kStreamWG>(a, s_red), inv_n, L.eps));
     if (threadIdx.x == 0) {
       gmut<float>(L.mean)[r] = mu;
       gmut<float>(L.rstd)[r] = rs;
