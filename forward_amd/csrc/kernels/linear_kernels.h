@@ -37,11 +37,29 @@ typedef short S4 __attribute__((ext_vector_type(4)));
 
 __device__ __forceinline__ float exp_(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504088896341f); }
 
-// Phi(x), the normal distribution function: 1 - q(x) or q(|x|) with q the upper tail.  16-bit results take the
-// tail from Abramowitz and Stegun 7.1.26 (absolute error of erf at most 1.5e-7), fp32 results from erfc itself.
+// EXACT, for fp32 results: a rounding of an exponent's argument enters the result times the argument (silu(-16) was 16 units
+// of 2^-24 off, gelu_tanh(-9) 200), so arguments are formed in 64 bits and go in as a sum of two floats.  16-bit results round
+// by a thousand times more.
+struct Two {
+  float hi, lo;
+  __device__ __forceinline__ explicit Two(double a) : hi((float)a), lo((float)(a - (double)(float)a)) {}
+};
+// e^-a for a >= 0 (2^-24 relative, a few units; from a = 200 on it is 0)
+__device__ __forceinline__ float exp_minus(double a) {
+  const Two t(fmin(a, 200.0));
+  return expf(-t.hi) * (1.0f - t.lo);
+}
+
+// Phi(x), the normal distribution function: 1 - q(x) or q(|x|) with q the upper tail.  fp32 results take it from erfc itself,
+// at the rounded argument and with the slope for the rest.  16-bit results take the tail from Abramowitz and Stegun 7.1.26
+// (absolute error of erf at most 1.5e-7; of the tail's own value 0.05 % at x = -4, 0.16 % at -5, 0.4 % at -6, where bf16
+// rounds by as much, 1 % at -8, 3.7 % at -13).
 template <bool EXACT>
 __device__ __forceinline__ float normal_cdf(float x) {
-  if (EXACT) return 0.5f * erfcf(-0.70710678118654752f * x);
+  if (EXACT) {
+    const Two u(fmin(fmax((double)x * -0.70710678118654752440, -30.0), 30.0));
+    return __builtin_fmaf(exp_(-u.hi * u.hi) * -0.56418958354775629f, u.lo, 0.5f * erfcf(u.hi));
+  }
   const float u = fabsf(x) * 0.70710678118654752f;
   const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3275911f, u, 1.0f));
   float p = __builtin_fmaf(t, 1.061405429f, -1.453152027f);
@@ -51,32 +69,57 @@ __device__ __forceinline__ float normal_cdf(float x) {
   const float q = 0.5f * p * t * exp_(-u * u);
   return x < 0.0f ? q : 1.0f - q;
 }
-// 1 / (1 + e^-x); e^-x overflows to infinity and the quotient to 0, as the limit is.
-__device__ __forceinline__ float logistic(float x) { return __builtin_amdgcn_rcpf(1.0f + exp_(-x)); }
+// The normal density times sqrt(2 pi).
+template <bool EXACT>
+__device__ __forceinline__ float bell(float x) {
+  return EXACT ? exp_minus(0.5 * (double)x * (double)x) : exp_(-0.5f * x * x);
+}
+
+// p = 1 / (1 + e^-a) and 1 - p.
+struct Logistic {
+  float p, rest;
+};
+template <bool EXACT, typename A>
+__device__ __forceinline__ Logistic logistic(A a) {
+  if (EXACT) {  // neither cancels nor overflows; what is below 2^-126 is 0, here as there (silu(-100) is -0)
+    const float e = exp_minus(fabs((double)a)), t = e < 0x1p-126f ? 0.0f : e, r = __builtin_amdgcn_rcpf(1.0f + t);
+    return a < 0 ? Logistic{t * r, r} : Logistic{r, t * r};
+  }
+  // e^-a overflows to infinity and the quotient to 0, as the limit is
+  const float p = __builtin_amdgcn_rcpf(1.0f + exp_(-(float)a));
+  return Logistic{p, 1.0f - p};
+}
 
 constexpr float kTanhIn = 1.59576912160573071f;  // 2 sqrt(2 / pi): (1 + tanh(u)) / 2 = logistic(2 u)
+template <bool EXACT>
+__device__ __forceinline__ Logistic gelu_tanh(float z) {
+  if (EXACT) {
+    const double d = z;
+    return logistic<true>(1.59576912160573071 * d * __builtin_fma(0.044715 * d, d, 1.0));
+  }
+  return logistic<false>(kTanhIn * __builtin_fmaf(0.044715f * z, z * z, z));
+}
 
 template <int ACT, bool EXACT>
 __device__ __forceinline__ float activate(float z) {
   if (ACT == FWDMI_ACT_RELU) return z < 0.0f ? 0.0f : z;  // NaN stays NaN
   if (ACT == FWDMI_ACT_GELU) return z * normal_cdf<EXACT>(z);
-  if (ACT == FWDMI_ACT_GELU_TANH) return z * logistic(kTanhIn * __builtin_fmaf(0.044715f * z, z * z, z));
-  if (ACT == FWDMI_ACT_SILU) return z * logistic(z);
+  if (ACT == FWDMI_ACT_GELU_TANH) return z * gelu_tanh<EXACT>(z).p;
+  if (ACT == FWDMI_ACT_SILU) return z * logistic<EXACT>(z).p;
   return z;
 }
 template <int ACT, bool EXACT>
 __device__ __forceinline__ float slope(float z) {
   if (ACT == FWDMI_ACT_RELU) return z <= 0.0f ? 0.0f : 1.0f;
-  if (ACT == FWDMI_ACT_GELU)
-    return __builtin_fmaf(z * 0.39894228040143268f, exp_(-0.5f * z * z), normal_cdf<EXACT>(z));
+  if (ACT == FWDMI_ACT_GELU) return __builtin_fmaf(z * 0.39894228040143268f, bell<EXACT>(z), normal_cdf<EXACT>(z));
   if (ACT == FWDMI_ACT_GELU_TANH) {
-    const float p = logistic(kTanhIn * __builtin_fmaf(0.044715f * z, z * z, z));
+    const Logistic l = gelu_tanh<EXACT>(z);
     const float zz = fminf(z * z, 1e30f);  // (where it would overflow p (1 - p) is zero; NaN comes back with p)
-    return __builtin_fmaf(z * p * (1.0f - p) * kTanhIn, __builtin_fmaf(0.134145f, zz, 1.0f), p);
+    return __builtin_fmaf(z * l.p * l.rest * kTanhIn, __builtin_fmaf(0.134145f, zz, 1.0f), l.p);
   }
   if (ACT == FWDMI_ACT_SILU) {
-    const float p = logistic(z);
-    return p * __builtin_fmaf(z, 1.0f - p, 1.0f);
+    const Logistic l = logistic<EXACT>(z);
+    return l.p * __builtin_fmaf(z, l.rest, 1.0f);
   }
   return 1.0f;
 }
