@@ -390,6 +390,11 @@ class Linear(torch.nn.Module):
     in_features = property(lambda self: self.weight.shape[1])
     out_features = property(lambda self: self.weight.shape[0])
 
+    def extra_repr(self):
+        return "in_features=%d, out_features=%d, bias=%s%s" % (
+            self.in_features, self.out_features, self.bias is not None,
+            "" if self.activation == "none" else ", activation=%r" % self.activation)
+
     def forward(self, x, residual=None, add_bias=True):
         bias = self.bias if add_bias else None
         keep = self.activation != "none" and torch.is_grad_enabled() and (
@@ -424,6 +429,9 @@ class LayerNorm(torch.nn.Module):
     gamma = property(lambda self: self.weight)
     beta = property(lambda self: self.bias)
     normalized_shape = property(lambda self: tuple(self.weight.shape))
+
+    def extra_repr(self):
+        return "%s, eps=%s%s" % (self.normalized_shape, self.eps, ", keep_sum=True" if self.keep_sum else "")
 
     def forward(self, x, skip=None, bias=None):
         op = torch.ops.fwdmi.layer_norm_train_sum if self.keep_sum else torch.ops.fwdmi.layer_norm_train
