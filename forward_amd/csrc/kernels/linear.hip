@@ -285,6 +285,32 @@ BackwardSpace backward_space(int64_t m, int64_t n, int64_t k, int act, int dtype
   return s;
 }
 
+// What the forward product reads: x and w, or their copies with whole lines at the workspace's beginning.
+Product forward_product(int64_t m, int64_t n, int64_t k, const ForwardSpace& space, const void* x, const void* w, char* ws) {
+  Product P{};
+  P.a = space.x ? ws : x;
+  P.b = space.x ? ws + space.x : w;
+  P.lda = P.ldb = space.x ? widened(k) : k;
+  P.ni = (int)m;
+  P.nj = (int)n;
+  P.nt = (int)k;
+  return P;
+}
+
+// What the gradient's products read: dz or dy, and x and w or their copies with whole lines behind dz and its partials.
+void backward_products(int64_t m, int64_t n, int64_t k, const BackwardSpace& space, const void* dy, const void* x,
+                       const void* w, char* ws, bool copy, bool widen, Product& X, Product& W) {
+  char* const wide = ws + space.dz + space.part;
+  X.a = W.a = copy ? ws : dy;
+  X.lda = W.lda = space.ld_dz;
+  X.b = widen ? wide + space.x : w;
+  W.b = widen ? wide : x;
+  X.ldb = W.ldb = widen ? widened(k) : k;
+  X.ni = W.nt = (int)m;
+  X.nt = W.ni = (int)n;
+  X.nj = W.nj = (int)k;
+}
+
 }  // namespace
 }  // namespace fwdmi
 
@@ -312,20 +338,11 @@ int fwdmi_linear(void* stream, int64_t m, int64_t n, int64_t k, const void* x, c
                 "linear: workspace of %zu bytes, %zu needed", workspace ? workspace_size : (size_t)0, space.total());
   hipStream_t s = static_cast<hipStream_t>(stream);
   char* const ws = static_cast<char*>(workspace);
-  Product P{};
-  P.a = x;
-  P.b = w;
-  P.lda = P.ldb = k;
   if (space.x) {
     const int rc = run_widen(Widen{{x, w}, {ws, ws + space.x}, {m, n}, (int)k, (int)widened(k)}, s);
     if (rc != FWDMI_OK) return rc;
-    P.a = ws;
-    P.b = ws + space.x;
-    P.lda = P.ldb = widened(k);
   }
-  P.ni = (int)m;
-  P.nj = (int)n;
-  P.nt = (int)k;
+  Product P = forward_product(m, n, k, space, x, w, ws);
   P.c = y;
   P.preact = preact;
   P.bias = bias;
@@ -367,14 +384,7 @@ int fwdmi_linear_backward(void* stream, int64_t m, int64_t n, int64_t k, const v
   dw = n > 0 && k > 0 ? dw : nullptr;  // (m == 0 likewise)
   const bool copy = space.dz && (dx || dw), widen = space.x && (dx || dw);
   Product X{}, W{};
-  X.a = W.a = copy ? ws : dy;
-  X.lda = W.lda = space.ld_dz;
-  X.b = widen ? wide + space.x : w;
-  W.b = widen ? wide : x;
-  X.ldb = W.ldb = widen ? widened(k) : k;
-  X.ni = W.nt = (int)m;
-  X.nt = W.ni = (int)n;
-  X.nj = W.nj = (int)k;
+  backward_products(m, n, k, space, dy, x, w, ws, copy, widen, X, W);
   X.c = dx;
   W.c = dw;
   Gradients G{};
@@ -437,6 +447,50 @@ int fwdmi_linear_backward(void* stream, int64_t m, int64_t n, int64_t k, const v
     if (rc != FWDMI_OK) return rc;
   }
   return dw ? run(W, 2, dtype, partial, s) : FWDMI_OK;
+}
+
+int fwdmi_linear_plan(int64_t m, int64_t n, int64_t k, int32_t what, int32_t act, int32_t dtype, int32_t on_boundary,
+                      fwdmi_linear_plan_info* plan) {
+  using namespace fwdmi;
+  clear_error();
+  if (!is_train_dtype(dtype)) return set_error(FWDMI_ERR_UNSUPPORTED, "linear plan: unsupported dtype %d", dtype);
+  FWDMI_REQUIRE(plan && what >= 0 && what <= 3 && act >= FWDMI_ACT_NONE && act <= FWDMI_ACT_SILU, "linear plan: null plan, or unknown product %d or activation %d", what, act);
+  FWDMI_REQUIRE(dims_ok(m, n, k) && m > 0 && n > 0 && k > 0, "linear plan: m=%lld n=%lld k=%lld", (long long)m, (long long)n,
+                (long long)k);
+  *plan = fwdmi_linear_plan_info{};
+  // (addresses that are looked at and never read: on a boundary, or one element past it)
+  const int elem = elem_size(dtype);
+  char* const ws = reinterpret_cast<char*>((uintptr_t)1 << 20);
+  const char* const at = ws + (on_boundary ? 0 : elem);
+  Plan p{};
+  Operands o{};
+  if (what == 0) {
+    const Product P = forward_product(m, n, k, forward_space(m, n, k, dtype), at, at, ws);
+    o = operands_of(P, 0, elem);
+    p = make_plan(P.ni, P.nj, P.nt, o);
+  } else {
+    const BackwardSpace space = backward_space(m, n, k, act, dtype);
+    Product X{}, W{};
+    backward_products(m, n, k, space, at, at, at, ws, space.dz != 0, space.x != 0, X, W);
+    if (what == 3) {
+      Gradients G{};
+      if (!together(X, W, dtype, G, o.direct)) return FWDMI_OK;  // (zeros: each product in a launch of its own)
+      p.tile = G.tile;
+      p.splits = 1;
+      o.end = o.direct ? std::max(operands_of(X, 1, elem).end, operands_of(W, 2, elem).end) : kTail;
+    } else {
+      const Product& P = what == 1 ? X : W;
+      o = operands_of(P, what, elem);
+      p = make_plan(P.ni, P.nj, P.nt, o);
+    }
+  }
+  plan->tile = p.tile;
+  plan->tile_rows = p.tile == kFew ? (m <= 16 ? 16 : kFewRows) : kTiles[p.tile].ti;
+  plan->tile_columns = p.tile == kFew ? 16 : kTiles[p.tile].tj;
+  plan->splits = p.splits;
+  plan->direct = p.tile != kFew && o.direct;
+  plan->end = p.tile == kFew ? 0 : o.end;
+  return FWDMI_OK;
 }
 
 }  // extern "C"

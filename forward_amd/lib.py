@@ -43,6 +43,10 @@ class EmbExt(C.Structure):
                 ("beta2", C.c_void_p), ("bias2", C.c_void_p), ("emb_output", C.c_void_p)]
 
 
+class LinearPlan(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("tile", "tile_rows", "tile_columns", "splits", "direct", "end")]
+
+
 class BagTable(C.Structure):
     _fields_ = [("data", C.c_void_p), ("input", C.c_void_p), ("input_2", C.c_void_p), ("count", C.c_int64),
                 ("input_size", C.c_int64), ("data_offset", C.c_int64), ("out_col", C.c_int64),
@@ -107,6 +111,7 @@ SIGNATURES = {
     "fwdmi_layer_norm_backward_workspace": (_sz, [_i32, _i64, _i32, _i32]),
     "fwdmi_layer_norm_backward": (C.c_int, [_vp, _i32, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
                                             _vp, _sz, _i32]),
+    "fwdmi_linear_plan": (C.c_int, [_i64, _i64, _i64, _i32, _i32, _i32, _i32, C.POINTER(LinearPlan)]),
     "fwdmi_linear_workspace": (_sz, [_i64, _i64, _i64, _i32]),
     "fwdmi_linear": (C.c_int, [_vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _vp, _sz]),
     "fwdmi_linear_backward_workspace": (_sz, [_i64, _i64, _i64, _i32, _i32]),

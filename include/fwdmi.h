@@ -370,6 +370,22 @@ int fwdmi_linear_backward(void* stream, int64_t m, int64_t n, int64_t k, const v
                           const void* preact, void* dx, void* dw, float* dbias, int32_t act, int32_t dtype,
                           void* workspace, size_t workspace_size);
 
+/*
+ * What a call of the linear layer of these sizes would launch on the current device: for tests that have to reach every
+ * variant, and for reading a measurement.  Host arithmetic alone, nothing is launched.
+ *   what: 0 the forward product, 1 dx alone, 2 dw alone, 3 dx and dw in one launch (tile_rows == 0: in launches of their own);
+ *   on_boundary: whether the operands begin on 16-byte boundaries, or one element past them; m, n, k of at least 1.
+ */
+typedef struct {
+  int32_t tile;                    /* number of the variant among those of one product */
+  int32_t tile_rows, tile_columns; /* of the result per workgroup */
+  int32_t splits;                  /* parts of the sum, added by a second launch where there are several */
+  int32_t direct;                  /* operands from memory straight to LDS, or through registers */
+  int32_t end;                     /* direct: 0 whole chunks to the end of the sum, 1 its last elements apart, 2 so is the last line */
+} fwdmi_linear_plan_info;
+int fwdmi_linear_plan(int64_t m, int64_t n, int64_t k, int32_t what, int32_t act, int32_t dtype, int32_t on_boundary,
+                      fwdmi_linear_plan_info* plan);
+
 /* ========================================================================================= *
  *  2. Plugin objects (opaque handles over the C++ classes in fwdmi_plugin.h)
  * ========================================================================================= */
