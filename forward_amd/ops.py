@@ -389,6 +389,7 @@ def emb_layer_norm(input_ids, segment_ids, input_mask, word, pos, tok, gamma, be
 # (a PyTorch without device support lacks the first; no call gets as far there, but the module is imported)
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 _current_device = torch.cuda.current_device
+_MAX_LD = 1 << 26         # of a norm's rows; checked here because the launcher's own argument has 32 bits, which wrap
 
 
 def _away(x, stream):
@@ -446,8 +447,8 @@ def layer_norm_forward(x, gamma, beta, skip=None, bias=None, eps=0.0, want_sum=F
     """
     dt, shape, at = _train_dtype(x), x.shape, x.get_device()
     ld = shape[-1] if shape else 0
-    if ld <= 0:
-        _require(False, 'input has a last axis of at least one element')
+    if not 0 < ld <= _MAX_LD:
+        _require(False, 'input has a last axis of 1 to 2^26 elements')
     pg, pb = _vector(gamma, ld, at, "gamma"), _vector(beta, ld, at, "beta")
     pi = None if bias is None else _vector(bias, ld, at, "bias")
     ps = None if skip is None else _plane(skip, shape, x.dtype, at, "skip")
@@ -478,8 +479,8 @@ def layer_norm_backward(dy, x, gamma, mean, rstd, skip=None, bias=None, dsum=Non
     """
     dt, shape, at, n = _train_dtype(x), x.shape, x.get_device(), x.numel()
     ld = shape[-1] if shape else 0
-    if ld <= 0:
-        _require(False, 'input has a last axis of at least one element')
+    if not 0 < ld <= _MAX_LD:
+        _require(False, 'input has a last axis of 1 to 2^26 elements')
     pdy = _plane(dy, shape, x.dtype, at, "dy")
     pg = _vector(gamma, ld, at, "gamma")
     pm, pr = _vector(mean, n // ld, at, "mean"), _vector(rstd, n // ld, at, "rstd")
