@@ -562,8 +562,8 @@ __global__ __launch_bounds__(kStreamWG) void ln_forward_stream_kernel(const LnTr
   }
 }
 
-// Two passes, likewise, and the columns' kernel reads dy and x a third time: 2700 x 12288 fp32 takes 146 us in all, 129 of
-// them what its 660 MB from and to memory take at a large copy's rate.
+// Two passes, likewise, and the columns' kernel reads dy and x a third time: 2700 x 12288 fp32 takes 146 us in all.  Its three
+// planes alone (398 MB) take 77 at a large copy's rate, with dy and x read twice from memory 129.
 template <typename T>
 __global__ __launch_bounds__(kStreamWG) void ln_backward_stream_kernel(const LnTrain L) {
   constexpr int VEC = 16 / sizeof(T);
@@ -696,7 +696,7 @@ Shape row_shape(int ld, int vec) {
     if (slices <= 256 * nv) return {256, nv};
   if (slices <= 512 * deep) return {512, deep};
   // fp32 rows of more than 16 elements per lane do not fit its registers: 2700 x 12288 took 124 us forward and 275 us
-  // backward that way, 74 and 146 streamed
+  // backward that way, 74 and 146 streamed (a row of up to some 40000 elements would fit LDS, which is not tried)
   if (vec == 8 && slices <= 1024 * deep) return {512, 2 * deep};
   return {0, 0};
 }

@@ -72,7 +72,9 @@ double step_us(TileKind kind, const Operands& o, double wgs) {
 }
 // A few rows: whole rows of w per workgroup, unless there are so few workgroups and so long rows that a second launch to
 // add splits costs less than it gains.  A CU draws w and x at 38 KB/us through registers: 16 x 4096 x 1024 fp32 takes 16 us
-// on 64 CUs, 9 with four splits and their sum.
+// on 64 CUs, 9 with four splits and their sum.  No tile competes with it up to 32 rows, which is right where w has enough
+// rows (replayed from a graph, 32 x 4096 x 1024 fp16 5.0 us, 33 rows in tiles 4.3; one row 3.4) and not where w has few: 32 x
+// 1024 x 4096 fp16 12.8 us, 33 rows in tiles 7.9, one row 6.5; fp32 10.7, 12.4 and 6.9.
 Plan few_plan(int ni, int nj, int nt, int elem) {
   const int pieces = nt / (128 / elem), wgs = ceil_div(nj, 16);
   const double us = (16.0 + (ni <= 16 ? 16 : 32)) * nt * elem / (38.0 * 1024);

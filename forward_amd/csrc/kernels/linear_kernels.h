@@ -638,7 +638,7 @@ __device__ __forceinline__ void leave_registers(const Product& P, const F4 (&acc
 }
 
 // The work of workgroup `block` of `blocks` on product P.  Products of these sizes are bound by the latency of their few
-// steps and by what a CU loads, 90 KB/us (384 x 1024 x 4096 fp16: 9.6 us, 335 TFLOP/s, of which 7.1 are its 640 KB), or, in fp32, by the matrix
+// steps and by what a CU loads, 90 KB/us (384 x 1024 x 4096 fp16: 10.5 us, 306 TFLOP/s, of which 7.1 are its 640 KB), or, in fp32, by the matrix
 // instructions and LDS in turn (1003 x 517 x 1024: 15.5 us, 69 TFLOP/s; 8192 x 1024 x 4096: 126, where a large library
 // product reaches 145).  The waves are WI x WJ over the tile and WK over the halves of
 // a step (their sums meet in LDS): small tiles, whose waves would otherwise have little to do between two barriers.

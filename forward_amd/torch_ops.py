@@ -323,7 +323,9 @@ def _norm_setup(ctx, inputs, output):
     ctx.set_materialize_grads(False)
     ctx.has_sum = len(output) == 4
     ctx.types = (skip is not None, gamma.dtype, beta.dtype, None if bias is None else bias.dtype)
-    if ctx.has_sum and bias is None:      # the kept sum stands for x and skip
+    # The kept sum stands for x and skip, which then need not be: one tensor that the next layer holds anyhow.  It is rounded,
+    # the statistics are of the unrounded sum: xhat is off by half a step of h times rstd.  (A bias needs its own sum of dx.)
+    if ctx.has_sum and bias is None:
         x, skip = output[1], None
     ctx.save_for_backward(x, skip, gamma, bias, mean, rstd)
 
